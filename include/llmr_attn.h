@@ -96,8 +96,11 @@ int llmr_ctx_set_sm_budget(llmr_ctx *ctx, int sms);
 int llmr_timeline_set(llmr_ctx *ctx, void *device_buffer, size_t bytes);
 void *llmr_get_stream(llmr_ctx *ctx);
 const char *llmr_last_error(llmr_ctx *ctx);
-/* Wait for all work on the context stream; reports device-side timeouts.
- * Replaces RenderGraph.checkpoint/flush (lib/vulkan/graph.c3:96-107). */
+/* Wait for all work on the context stream; reports device-side timeouts
+ * (LLMR_ETIMEOUT) and what the causal and paged operators found wrong in
+ * device memory (LLMR_EINVAL: a length, offset, slot, position or page out of
+ * range; LLMR_ENOMEM: llmr_paged_plan ran out of pages). Replaces
+ * RenderGraph.checkpoint/flush (lib/vulkan/graph.c3:96-107). */
 int llmr_sync(llmr_ctx *ctx);
 /* Number of kernels this context has launched (for launch accounting). */
 uint64_t llmr_launch_count(llmr_ctx *ctx);
@@ -416,6 +419,133 @@ int llmr_attention_merge(llmr_ctx *ctx, float *o_a, float *lse_a,
 int llmr_rope_tables(const int32_t *pos, uint32_t seq_len, uint32_t n_axes,
                      const uint32_t *axes_dims, float theta, float *cos_out,
                      float *sin_out);
+
+/* ---- Text models: causal prompts and a paged cache -----------------------
+ * The text encoders beside the diffusion models (the reference's llm_text
+ * attention_prefill, attention, head_norm_rope: dependencies/llm_text.c3l/
+ * shaders/llm.slang:2754, :914, :2907) attend causally, share each key/value
+ * head among n_heads / n_kv_heads query heads, and keep keys and values for
+ * later tokens. Here those are pages of a cache that many requests share:
+ *
+ *   llmr_paged_plan      pages, slots and positions of this step's tokens
+ *   llmr_paged_prologue  norm + RoPE of Q and K; K and V into their slots
+ *   llmr_attention_paged the new tokens' attention over their requests' pages
+ *   llmr_attention_causal  whole prompts, without a cache
+ *
+ * Lengths, offsets and page numbers are int32 in DEVICE memory and are read
+ * when the kernels run, so a captured step replays with other lengths. What is
+ * out of range there is never followed: the requests concerned are skipped
+ * and llmr_sync returns LLMR_EINVAL. Query head h uses key/value head
+ * h / (n_heads / n_kv_heads). head_dim is 64 or 128. Element strides of 0
+ * select the dense default [token][head][dim]; bases and strides must be
+ * multiples of 16 bytes. The calls run on the context's device whatever the
+ * current device is, and leave that as it was. Calls of one context share its
+ * workspace: graphs captured from one context must not replay at the same
+ * time, and llmr_ctx_reserve must not grow the workspace after a capture. */
+
+/* Causal attention of packed prompts. Sequence i is rows cu_seqlens[i] ..
+ * cu_seqlens[i+1] of q [total_tokens][n_heads][head_dim] and of k, v
+ * [total_tokens][n_kv_heads][head_dim]; its row r attends to rows 0 .. r of the
+ * same sequence: o = softmax(scale q k^T) v. cu_seqlens holds n_seqs + 1
+ * ascending values from 0 to at most total_tokens; a sequence may be empty,
+ * and rows behind the last sequence are left as they were in o and lse.
+ * lse: fp32 [n_heads][total_tokens] natural-log sum-exp, or NULL. Scores,
+ * softmax and sums are fp32; the softmax numerators enter the second product
+ * in the inputs' type. A non-finite element of k or v reaches no sequence
+ * but its own; within it, one in v may reach up to 127 rows before it. */
+typedef struct {
+  uint32_t n_seqs, total_tokens, n_heads, n_kv_heads, head_dim;
+  llmr_dtype dtype;     /* of q, k, v: LLMR_F16 or LLMR_BF16 */
+  llmr_dtype out_dtype; /* of o */
+  float scale;
+  uint64_t q_row_stride, k_row_stride, v_row_stride, o_row_stride;
+  uint64_t q_head_stride, k_head_stride, v_head_stride, o_head_stride;
+} llmr_causal_desc;
+int llmr_attention_causal(llmr_ctx *ctx, const llmr_causal_desc *desc,
+                          const int32_t *cu_seqlens, const void *q, const void *k,
+                          const void *v, void *o, float *lse);
+
+/* Attention of new tokens over a paged cache. Request i owns the query rows
+ * cu_q[i] .. cu_q[i+1] (its newest tokens, any number, also 0) and kv_lens[i]
+ * keys, the new tokens' own included: key j is row j % page_size of page
+ * block_table[i][j / page_size] of k_cache and v_cache [num_pages][page_size]
+ * [n_kv_heads][head_dim]. Query row r (of n) attends to keys 0 ..
+ * kv_lens[i] - n + r; one without a key gives o = 0 and lse = -inf. Rows
+ * behind the last request are left as they were. What a page holds behind a
+ * request's last key may be anything, NaN included. max_q_len bounds the
+ * rows of any request (and picks the kernel). page_size: 16, 32, 64, 128 or
+ * 256. lse as above. */
+typedef struct {
+  uint32_t n_seqs, total_tokens, max_q_len, n_heads, n_kv_heads, head_dim;
+  llmr_dtype dtype;     /* of q and the caches: LLMR_F16 or LLMR_BF16 */
+  llmr_dtype out_dtype; /* of o */
+  float scale;
+  uint32_t page_size, num_pages;
+  uint32_t max_pages;       /* columns of block_table */
+  uint64_t table_stride;    /* elements between rows of block_table; 0 = max_pages */
+  uint64_t q_row_stride, o_row_stride, q_head_stride, o_head_stride;
+  uint64_t k_page_stride, k_row_stride, k_head_stride;
+  uint64_t v_page_stride, v_row_stride, v_head_stride;
+} llmr_paged_desc;
+/* Workspace the call needs (0 for a desc that it would refuse). It depends on
+ * n_seqs, total_tokens, max_q_len, the head counts and head_dim alone. */
+size_t llmr_attention_paged_workspace_bytes(const llmr_paged_desc *desc);
+int llmr_attention_paged(llmr_ctx *ctx, const llmr_paged_desc *desc, const int32_t *cu_q,
+                         const int32_t *kv_lens, const int32_t *block_table, const void *q,
+                         const void *k_cache, const void *v_cache, void *o, float *lse);
+
+/* Plans one step: request i has ctx_lens[i] cached tokens and adds new_lens[i]
+ * (0 or more). Pages it then lacks come off the top of the stack
+ * free_pages[0 .. n_free), requests in order, and are entered into its row of
+ * block_table. Written: cu_q [n_seqs+1] offsets of the new tokens, kv_lens
+ * [n_seqs] = ctx + new, and for each of max_tokens places the token's position
+ * in its request and its slot (page * page_size + row), or position 0 and slot
+ * -1 behind the last token; n_free_out what is left. kv_lens may be ctx_lens
+ * and n_free_out may be n_free (then a replayed step advances by itself); no
+ * other two arrays may overlap. If the pages do not suffice, or a length is
+ * negative or too long for block_table or max_tokens, nothing is planned:
+ * cu_q is 0, slots -1, kv_lens = ctx_lens, n_free_out = n_free, block_table as it
+ * was, and llmr_sync reports it. A request is released by putting its pages
+ * back on the stack. n_seqs: at most 4096. */
+typedef struct {
+  uint32_t n_seqs, max_tokens;
+  uint32_t page_size, num_pages; /* num_pages * page_size < 2^31 */
+  uint32_t free_capacity;        /* elements of free_pages */
+  uint32_t max_pages;            /* columns of block_table */
+  uint64_t table_stride;         /* elements between its rows; 0 = max_pages */
+} llmr_plan_desc;
+int llmr_paged_plan(llmr_ctx *ctx, const llmr_plan_desc *desc, const int32_t *ctx_lens,
+                    const int32_t *new_lens, const int32_t *free_pages, const int32_t *n_free,
+                    int32_t *block_table, int32_t *cu_q, int32_t *kv_lens,
+                    int32_t *positions, int32_t *slots, int32_t *n_free_out);
+
+/* The step before llmr_attention_paged: for each token t with slots[t] >= 0,
+ * Q and K rows get the per-head RMSNorm (LLMR_NORM_Q, LLMR_NORM_K: gains
+ * [head_dim]) and the rotation by row positions[t] of the tables (LLMR_ROPE:
+ * cos_t, sin_t [rope_rows][head_dim/2], pairs (2i, 2i+1); with
+ * LLMR_ROPE_HALF pairs (i, i + head_dim/2)), all in fp32, rounded once; Q goes
+ * to q_out [token][n_heads][head_dim], K and V to row slots[t] % page_size of
+ * page slots[t] / page_size. Tokens with a negative slot are left out. No two
+ * tokens may share a slot. q_out may be q (same type and strides); q may be
+ * NULL with q_out (K and V alone). positions may be NULL without LLMR_ROPE. */
+enum { LLMR_ROPE_HALF = 1u << 6 };
+typedef struct {
+  uint32_t total_tokens, n_heads, n_kv_heads, head_dim;
+  llmr_dtype in_dtype;  /* of q, k, v: any */
+  llmr_dtype dtype;     /* of q_out and the caches: LLMR_F16 or LLMR_BF16 */
+  uint32_t flags;       /* LLMR_NORM_Q | LLMR_NORM_K | LLMR_ROPE | LLMR_ROPE_HALF */
+  float eps;
+  uint32_t page_size, num_pages, rope_rows;
+  uint64_t q_row_stride, k_row_stride, v_row_stride, q_out_row_stride;
+  uint64_t q_head_stride, k_head_stride, v_head_stride, q_out_head_stride;
+  uint64_t k_page_stride, k_cache_row_stride, k_cache_head_stride;
+  uint64_t v_page_stride, v_cache_row_stride, v_cache_head_stride;
+} llmr_paged_prologue_desc;
+int llmr_paged_prologue(llmr_ctx *ctx, const llmr_paged_prologue_desc *desc,
+                        const int32_t *positions, const int32_t *slots, const void *q,
+                        const void *k, const void *v, const float *q_gain,
+                        const float *k_gain, const float *cos_t, const float *sin_t,
+                        void *q_out, void *k_cache, void *v_cache);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,7 @@
 #include <string>
 
 #include "../../include/llmr_attn.h"
+#include "ctx.cuh"
 #include "exact_tc.cuh"
 #include "fa_tc.cuh"
 #include "fa_wide.cuh"
@@ -29,74 +30,7 @@
 
 using namespace llmr;
 
-constexpr size_t kSyncInts = 1 + 65536;
-
-struct llmr_ctx {
-  int device = 0;
-  cudaStream_t stream = nullptr;
-  bool own_stream = false;
-  void *ws = nullptr;
-  size_t ws_bytes = 0;
-  int *d_err = nullptr;
-  int *d_sync = nullptr;  // fused-prologue piece counters (self-resetting)
-  unsigned long long *timeline = nullptr;  // LLMR_TIMELINE builds: event buffer
-  uint64_t launches = 0;
-  int num_sms = 0;
-  bool prof_on = false;
-  bool prof_valid = false;
-  cudaEvent_t prof_ev[3] = {nullptr, nullptr, nullptr};
-  std::string err;
-};
-
 namespace {
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t,
-                                  void *, const cuuint64_t *, const cuuint64_t *,
-                                  const cuuint32_t *, const cuuint32_t *,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-int fail(llmr_ctx *ctx, int code, const char *fmt, ...) {
-  if (ctx) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    ctx->err = buf;
-  }
-  return code;
-}
-
-#define CUDA_TRY(ctx, call)                                                   \
-  do {                                                                        \
-    cudaError_t e_ = (call);                                                  \
-    if (e_ != cudaSuccess)                                                    \
-      return fail(ctx, LLMR_ECUDA, "%s: %s", #call, cudaGetErrorString(e_));  \
-  } while (0)
-
-// Checks the launch that was just enqueued.
-int after_launch(llmr_ctx *ctx, const char *what) {
-  ctx->launches++;
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess)
-    return fail(ctx, LLMR_ECUDA, "%s launch: %s", what, cudaGetErrorString(e));
-  return LLMR_OK;
-}
-
-EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
-  return fn;
-}
 
 // 4-D fp16 tensor map over (d, s, h, b) with a 64 x box_rows x 1 x 1 box and
 // 128-byte swizzle: one box is one SW128 K-major operand chunk.
@@ -723,7 +657,16 @@ int llmr_sync(llmr_ctx *ctx) {
   CUDA_TRY(ctx, cudaMemcpy(&h, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost));
   if (h) {
     CUDA_TRY(ctx, cudaMemset(ctx->d_err, 0, sizeof(int)));
-    return fail(ctx, LLMR_ETIMEOUT, "a device-side wait exceeded its limit; results are invalid");
+    if (h & kErrTimeout) {
+      // A kernel that gave up may have left its counters part-way.
+      CUDA_TRY(ctx, cudaMemset(ctx->d_sync, 0, kSyncInts * sizeof(int)));
+      return fail(ctx, LLMR_ETIMEOUT, "a device-side wait exceeded its limit; results are invalid");
+    }
+    if (h & kErrInput)
+      return fail(ctx, LLMR_EINVAL, "a length, offset, slot, position or page in device memory is "
+                                    "out of range; the requests it belongs to were skipped");
+    return fail(ctx, LLMR_ENOMEM, "the free list holds fewer pages than the step needs; nothing "
+                                  "was planned");
   }
   return LLMR_OK;
 }

@@ -1,0 +1,383 @@
+// Host side of the causal and paged operators of include/llmr_attn.h:
+// argument checks, tensor maps, the choice of kernel and the launches.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <string.h>
+
+#include "ctx.cuh"
+#include "kattr.cuh"
+#include "paged_kernels.cuh"
+
+using namespace llmr;
+
+namespace {
+
+// Makes the context's device current for one call and puts the caller's back.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    if (cudaGetDevice(&old_) != cudaSuccess) old_ = device;
+    ok_ = old_ == device || cudaSetDevice(device) == cudaSuccess;
+    changed_ = old_ != device;
+  }
+  ~OnDevice() {
+    if (changed_) cudaSetDevice(old_);
+  }
+  bool ok() const { return ok_; }
+
+ private:
+  int old_ = 0;
+  bool ok_ = false, changed_ = false;
+};
+
+#define ENTER(ctx)                                   \
+  if (!(ctx)) return LLMR_EINVAL;                    \
+  OnDevice on_device_((ctx)->device);                \
+  if (!on_device_.ok()) return fail(ctx, LLMR_ECUDA, "cudaSetDevice(%d) failed", (ctx)->device)
+
+bool is16(llmr_dtype t) { return t == LLMR_F16 || t == LLMR_BF16; }
+bool known(llmr_dtype t) { return t == LLMR_F32 || is16(t); }
+size_t size_of(llmr_dtype t) { return t == LLMR_F32 ? 4 : 2; }
+bool a16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool a4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+long long either(uint64_t given, long long dense) { return given ? (long long)given : dense; }
+// Strides that are whole 16-byte pieces and below the 2^40 bytes a tensor
+// map can hold.
+bool strides16(std::initializer_list<long long> st, size_t es) {
+  for (long long s : st)
+    if (s < 0 || s >= (1ll << 40) / (long long)es || (s * (long long)es) % 16) return false;
+  return true;
+}
+
+// What is wrong with the head geometry, or null.
+const char *bad_heads(uint32_t H, uint32_t Hk, uint32_t D) {
+  if (D != 64 && D != 128) return "head_dim must be 64 or 128";
+  if (H < 1 || Hk < 1 || H > 65535 || H % Hk) return "n_heads must be a multiple of n_kv_heads";
+  if (H / Hk > 128) return "more than 128 query heads per key/value head";
+  return nullptr;
+}
+
+const char *bad_page(uint32_t page, uint32_t num_pages) {
+  if (page != 16 && page != 32 && page != 64 && page != 128 && page != 256)
+    return "page_size must be 16, 32, 64, 128 or 256";
+  if (num_pages < 1 || (uint64_t)num_pages * page > 0x7fffffffull)
+    return "num_pages must be at least 1 and num_pages * page_size below 2^31";
+  return nullptr;
+}
+
+const char *bad_paged(const llmr_paged_desc *d) {
+  if (const char *e = bad_heads(d->n_heads, d->n_kv_heads, d->head_dim)) return e;
+  if (const char *e = bad_page(d->page_size, d->num_pages)) return e;
+  if (!is16(d->dtype) || !known(d->out_dtype)) return "q and the caches must be fp16 or bf16";
+  if (!(d->scale > 0.0f) || !isfinite(d->scale)) return "scale must be finite and > 0";
+  if (d->n_seqs > 0x3fffffffu || d->total_tokens > 0x3fffffffu) return "problem too large";
+  if (d->max_pages < 1 || (uint64_t)d->max_pages * d->page_size > 0x7fffffffull)
+    return "max_pages must be at least 1 and max_pages * page_size below 2^31";
+  if (d->table_stride && d->table_stride < d->max_pages) return "table_stride is below max_pages";
+  return nullptr;
+}
+
+template <int D, typename T, typename OutT>
+int launch_rows(llmr_ctx *ctx, const RowsParams &p) {
+  const long long warps = (long long)p.tokens * p.H;
+  rows_attention_kernel<D, T, OutT><<<(unsigned)((warps + 7) / 8), 256, 0, ctx->stream>>>(p);
+  return after_launch(ctx, "rows_attention");
+}
+
+template <int D, typename T>
+int launch_rows_o(llmr_ctx *ctx, llmr_dtype od, const RowsParams &p) {
+  if (od == LLMR_F32) return launch_rows<D, T, float>(ctx, p);
+  if (od == LLMR_F16) return launch_rows<D, T, __half>(ctx, p);
+  return launch_rows<D, T, __nv_bfloat16>(ctx, p);
+}
+
+int launch_rows_any(llmr_ctx *ctx, int D, llmr_dtype dt, llmr_dtype od, const RowsParams &p) {
+  if (D == 128)
+    return dt == LLMR_F16 ? launch_rows_o<128, __half>(ctx, od, p)
+                          : launch_rows_o<128, __nv_bfloat16>(ctx, od, p);
+  return dt == LLMR_F16 ? launch_rows_o<64, __half>(ctx, od, p)
+                        : launch_rows_o<64, __nv_bfloat16>(ctx, od, p);
+}
+
+template <int D, typename InT, typename OutT>
+int launch_paged_prologue(llmr_ctx *ctx, bool half, PagedRopeParams &p) {
+  constexpr int per_warp = (32 / (D / 16)) * kRopeSteps;
+  const int rows = (p.q ? p.hq : 0) + 2 * p.hk;
+  p.chunks = (rows + per_warp - 1) / per_warp;
+  const long long warps = (long long)p.tokens * p.chunks;
+  const unsigned grid = (unsigned)((warps + 7) / 8);
+  if (half)
+    paged_prologue_kernel<D, InT, OutT, true><<<grid, 256, 0, ctx->stream>>>(p);
+  else
+    paged_prologue_kernel<D, InT, OutT, false><<<grid, 256, 0, ctx->stream>>>(p);
+  return after_launch(ctx, "paged_prologue");
+}
+
+template <int D, typename InT>
+int launch_paged_prologue_o(llmr_ctx *ctx, llmr_dtype od, bool half, PagedRopeParams &p) {
+  return od == LLMR_F16 ? launch_paged_prologue<D, InT, __half>(ctx, half, p)
+                        : launch_paged_prologue<D, InT, __nv_bfloat16>(ctx, half, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int llmr_attention_causal(llmr_ctx *ctx, const llmr_causal_desc *d, const int32_t *cu_seqlens,
+                          const void *q, const void *k, const void *v, void *o, float *lse) {
+  ENTER(ctx);
+  if (!d) return fail(ctx, LLMR_EINVAL, "null argument");
+  if (const char *e = bad_heads(d->n_heads, d->n_kv_heads, d->head_dim))
+    return fail(ctx, LLMR_EINVAL, "%s", e);
+  if (!is16(d->dtype) || !known(d->out_dtype))
+    return fail(ctx, LLMR_EINVAL, "q, k and v must be fp16 or bf16");
+  if (!(d->scale > 0.0f) || !isfinite(d->scale))
+    return fail(ctx, LLMR_EINVAL, "scale must be finite and > 0");
+  if (d->n_seqs > 0x3fffffffu || d->total_tokens > 0x3fffffffu)
+    return fail(ctx, LLMR_EINVAL, "problem too large");
+  if (d->n_seqs == 0 || d->total_tokens == 0) return LLMR_OK;
+  if (!cu_seqlens || !q || !k || !v || !o) return fail(ctx, LLMR_EINVAL, "null argument");
+  const long long D = d->head_dim, H = d->n_heads, Hk = d->n_kv_heads;
+  RowsParams p = {};
+  p.n = (int)d->n_seqs;
+  p.tokens = (int)d->total_tokens;
+  p.H = (int)H;
+  p.Hk = (int)Hk;
+  p.page = 1;
+  p.num_pages = 1;
+  p.cu = cu_seqlens;
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.o = o;
+  p.lse = lse;
+  p.qs[0] = either(d->q_row_stride, H * D);
+  p.qs[1] = either(d->q_head_stride, D);
+  p.ks[1] = either(d->k_row_stride, Hk * D);
+  p.ks[2] = either(d->k_head_stride, D);
+  p.vs[1] = either(d->v_row_stride, Hk * D);
+  p.vs[2] = either(d->v_head_stride, D);
+  p.os[0] = either(d->o_row_stride, H * D);
+  p.os[1] = either(d->o_head_stride, D);
+  p.scale = d->scale;
+  p.err = ctx->d_err;
+  if (!a16(q) || !a16(k) || !a16(v) || !a16(o) ||
+      !strides16({p.qs[0], p.qs[1], p.ks[1], p.ks[2], p.vs[1], p.vs[2]}, 2) ||
+      !strides16({p.os[0], p.os[1]}, size_of(d->out_dtype)))
+    return fail(ctx, LLMR_EINVAL, "q, k, v, o and their strides must be 16-byte aligned");
+  if (!a4(cu_seqlens) || !a4(lse)) return fail(ctx, LLMR_EINVAL, "cu_seqlens or lse is misaligned");
+  return launch_rows_any(ctx, (int)D, d->dtype, d->out_dtype, p);
+}
+
+size_t llmr_attention_paged_workspace_bytes(const llmr_paged_desc *d) {
+  if (!d || bad_paged(d)) return 0;
+  return 16;
+}
+
+int llmr_attention_paged(llmr_ctx *ctx, const llmr_paged_desc *d, const int32_t *cu_q,
+                         const int32_t *kv_lens, const int32_t *block_table, const void *q,
+                         const void *k_cache, const void *v_cache, void *o, float *lse) {
+  ENTER(ctx);
+  if (!d) return fail(ctx, LLMR_EINVAL, "null argument");
+  if (const char *e = bad_paged(d)) return fail(ctx, LLMR_EINVAL, "%s", e);
+  if (d->n_seqs == 0 || d->total_tokens == 0) return LLMR_OK;
+  if (d->max_q_len == 0) return fail(ctx, LLMR_EINVAL, "max_q_len must be at least 1");
+  if (!cu_q || !kv_lens || !block_table || !q || !k_cache || !v_cache || !o)
+    return fail(ctx, LLMR_EINVAL, "null argument");
+  const size_t need = llmr_attention_paged_workspace_bytes(d);
+  if (need > ctx->ws_bytes)
+    return fail(ctx, LLMR_ENOMEM, "workspace %zu bytes < %zu needed (llmr_ctx_reserve)",
+                ctx->ws_bytes, need);
+  const long long D = d->head_dim, H = d->n_heads, Hk = d->n_kv_heads, P = d->page_size;
+  RowsParams p = {};
+  p.n = (int)d->n_seqs;
+  p.tokens = (int)d->total_tokens;
+  p.H = (int)H;
+  p.Hk = (int)Hk;
+  p.page = (int)P;
+  p.num_pages = (int)d->num_pages;
+  p.max_pages = (int)d->max_pages;
+  p.max_q = (int)(d->max_q_len < d->total_tokens ? d->max_q_len : d->total_tokens);
+  p.paged = true;
+  p.cu = cu_q;
+  p.kv_lens = kv_lens;
+  p.table = block_table;
+  p.table_stride = either(d->table_stride, d->max_pages);
+  p.q = q;
+  p.k = k_cache;
+  p.v = v_cache;
+  p.o = o;
+  p.lse = lse;
+  p.qs[0] = either(d->q_row_stride, H * D);
+  p.qs[1] = either(d->q_head_stride, D);
+  p.os[0] = either(d->o_row_stride, H * D);
+  p.os[1] = either(d->o_head_stride, D);
+  p.ks[0] = either(d->k_page_stride, P * Hk * D);
+  p.ks[1] = either(d->k_row_stride, Hk * D);
+  p.ks[2] = either(d->k_head_stride, D);
+  p.vs[0] = either(d->v_page_stride, P * Hk * D);
+  p.vs[1] = either(d->v_row_stride, Hk * D);
+  p.vs[2] = either(d->v_head_stride, D);
+  p.scale = d->scale;
+  p.err = ctx->d_err;
+  if (!a16(q) || !a16(k_cache) || !a16(v_cache) || !a16(o) ||
+      !strides16({p.qs[0], p.qs[1], p.ks[0], p.ks[1], p.ks[2], p.vs[0], p.vs[1], p.vs[2]}, 2) ||
+      !strides16({p.os[0], p.os[1]}, size_of(d->out_dtype)))
+    return fail(ctx, LLMR_EINVAL, "q, the caches, o and their strides must be 16-byte aligned");
+  if (!a4(cu_q) || !a4(kv_lens) || !a4(block_table) || !a4(lse))
+    return fail(ctx, LLMR_EINVAL, "cu_q, kv_lens, block_table or lse is misaligned");
+  return launch_rows_any(ctx, (int)D, d->dtype, d->out_dtype, p);
+}
+
+int llmr_paged_plan(llmr_ctx *ctx, const llmr_plan_desc *d, const int32_t *ctx_lens,
+                    const int32_t *new_lens, const int32_t *free_pages, const int32_t *n_free,
+                    int32_t *block_table, int32_t *cu_q, int32_t *kv_lens, int32_t *positions,
+                    int32_t *slots, int32_t *n_free_out) {
+  ENTER(ctx);
+  if (!d || !n_free || !cu_q || !n_free_out) return fail(ctx, LLMR_EINVAL, "null argument");
+  if (d->n_seqs && (!ctx_lens || !new_lens || !block_table || !kv_lens))
+    return fail(ctx, LLMR_EINVAL, "null argument");
+  if ((d->free_capacity && !free_pages) || (d->max_tokens && (!positions || !slots)))
+    return fail(ctx, LLMR_EINVAL, "null argument");
+  if (d->n_seqs > (uint32_t)kPlanMaxSeqs)
+    return fail(ctx, LLMR_EINVAL, "n_seqs %u exceeds %d", d->n_seqs, kPlanMaxSeqs);
+  if (const char *e = bad_page(d->page_size, d->num_pages)) return fail(ctx, LLMR_EINVAL, "%s", e);
+  if (d->max_tokens > 0x3fffffffu || d->free_capacity > 0x3fffffffu ||
+      (uint64_t)d->max_pages * d->page_size > 0x7fffffffull)
+    return fail(ctx, LLMR_EINVAL, "problem too large");
+  if (d->table_stride && d->table_stride < d->max_pages)
+    return fail(ctx, LLMR_EINVAL, "table_stride is below max_pages");
+  for (const void *x : {(const void *)ctx_lens, (const void *)new_lens, (const void *)free_pages,
+                        (const void *)n_free, (const void *)block_table, (const void *)cu_q,
+                        (const void *)kv_lens, (const void *)positions, (const void *)slots,
+                        (const void *)n_free_out})
+    if (!a4(x)) return fail(ctx, LLMR_EINVAL, "an array is misaligned");
+  PlanParams p;
+  p.n = (int)d->n_seqs;
+  p.max_tokens = (int)d->max_tokens;
+  p.page = (int)d->page_size;
+  p.num_pages = (int)d->num_pages;
+  p.free_cap = (int)d->free_capacity;
+  p.max_pages = (int)d->max_pages;
+  p.table_stride = either(d->table_stride, d->max_pages);
+  p.ctx_lens = ctx_lens;
+  p.new_lens = new_lens;
+  p.free_pages = free_pages;
+  p.n_free = n_free;
+  p.table = block_table;
+  p.cu_q = cu_q;
+  p.kv_lens = kv_lens;
+  p.positions = positions;
+  p.slots = slots;
+  p.n_free_out = n_free_out;
+  p.err = ctx->d_err;
+  // One CTA until there is work for two rounds of its threads.
+  const long long items = (long long)d->max_tokens + d->n_seqs;
+  const int threads = items <= 256 ? 256 : kPlanThreads;
+  int ctas = 1;
+  while (ctas < 8 && items > 2ll * ctas * threads) ctas *= 2;
+  const int smem = (3 * p.n + 2) * (int)sizeof(int);
+  CUDA_TRY(ctx, set_smem_once(paged_plan_kernel, (3 * kPlanMaxSeqs + 2) * (int)sizeof(int)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, paged_plan_kernel, p));
+  return after_launch(ctx, "paged_plan");
+}
+
+int llmr_paged_prologue(llmr_ctx *ctx, const llmr_paged_prologue_desc *d,
+                        const int32_t *positions, const int32_t *slots, const void *q,
+                        const void *k, const void *v, const float *q_gain, const float *k_gain,
+                        const float *cos_t, const float *sin_t, void *q_out, void *k_cache,
+                        void *v_cache) {
+  ENTER(ctx);
+  if (!d) return fail(ctx, LLMR_EINVAL, "null argument");
+  if (const char *e = bad_heads(d->n_heads, d->n_kv_heads, d->head_dim))
+    return fail(ctx, LLMR_EINVAL, "%s", e);
+  if (const char *e = bad_page(d->page_size, d->num_pages)) return fail(ctx, LLMR_EINVAL, "%s", e);
+  if (!known(d->in_dtype) || !is16(d->dtype))
+    return fail(ctx, LLMR_EINVAL, "q_out and the caches must be fp16 or bf16");
+  if (d->flags & ~(uint32_t)(LLMR_NORM_Q | LLMR_NORM_K | LLMR_ROPE | LLMR_ROPE_HALF))
+    return fail(ctx, LLMR_EINVAL, "only NORM_Q, NORM_K, ROPE and ROPE_HALF apply here");
+  if ((d->flags & LLMR_ROPE_HALF) && !(d->flags & LLMR_ROPE))
+    return fail(ctx, LLMR_EINVAL, "LLMR_ROPE_HALF needs LLMR_ROPE");
+  if (d->total_tokens > 0x3fffffffu) return fail(ctx, LLMR_EINVAL, "problem too large");
+  if (!isfinite(d->eps) || d->eps < 0.0f) return fail(ctx, LLMR_EINVAL, "eps must be finite and >= 0");
+  if (d->total_tokens == 0) return LLMR_OK;
+  if (!slots || !k || !v || !k_cache || !v_cache || (q != nullptr) != (q_out != nullptr))
+    return fail(ctx, LLMR_EINVAL, "null argument");
+  if ((d->flags & LLMR_NORM_Q) && !q_gain) return fail(ctx, LLMR_EINVAL, "LLMR_NORM_Q needs q_gain");
+  if ((d->flags & LLMR_NORM_K) && !k_gain) return fail(ctx, LLMR_EINVAL, "LLMR_NORM_K needs k_gain");
+  if ((d->flags & LLMR_ROPE) && (!cos_t || !sin_t || !positions || !d->rope_rows))
+    return fail(ctx, LLMR_EINVAL, "LLMR_ROPE needs cos/sin tables and positions");
+  if (d->rope_rows > 0x7fffffffu) return fail(ctx, LLMR_EINVAL, "problem too large");
+  const long long D = d->head_dim, H = d->n_heads, Hk = d->n_kv_heads, P = d->page_size;
+  PagedRopeParams p = {};
+  p.tokens = (int)d->total_tokens;
+  p.hq = (int)H;
+  p.hk = (int)Hk;
+  p.page = (int)P;
+  p.num_pages = (int)d->num_pages;
+  p.rope_rows = (int)d->rope_rows;
+  p.eps = d->eps;
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.q_out = q_out;
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.qs[0] = either(d->q_row_stride, H * D);
+  p.qs[1] = either(d->q_head_stride, D);
+  p.ks[0] = either(d->k_row_stride, Hk * D);
+  p.ks[1] = either(d->k_head_stride, D);
+  p.vs[0] = either(d->v_row_stride, Hk * D);
+  p.vs[1] = either(d->v_head_stride, D);
+  p.os[0] = either(d->q_out_row_stride, H * D);
+  p.os[1] = either(d->q_out_head_stride, D);
+  p.kc[0] = either(d->k_page_stride, P * Hk * D);
+  p.kc[1] = either(d->k_cache_row_stride, Hk * D);
+  p.kc[2] = either(d->k_cache_head_stride, D);
+  p.vc[0] = either(d->v_page_stride, P * Hk * D);
+  p.vc[1] = either(d->v_cache_row_stride, Hk * D);
+  p.vc[2] = either(d->v_cache_head_stride, D);
+  p.positions = positions;
+  p.slots = slots;
+  const bool rope = d->flags & LLMR_ROPE;
+  p.q_gain = (d->flags & LLMR_NORM_Q) ? q_gain : nullptr;
+  p.k_gain = (d->flags & LLMR_NORM_K) ? k_gain : nullptr;
+  p.cos_t = rope ? cos_t : nullptr;
+  p.sin_t = rope ? sin_t : nullptr;
+  p.err = ctx->d_err;
+  const size_t es = size_of(d->in_dtype);
+  if (!a16(q) || !a16(k) || !a16(v) || !a16(q_out) || !a16(k_cache) || !a16(v_cache) ||
+      !a16(p.q_gain) || !a16(p.k_gain) || !a16(p.cos_t) || !a16(p.sin_t) ||
+      !strides16({p.qs[0], p.qs[1], p.ks[0], p.ks[1], p.vs[0], p.vs[1]}, es) ||
+      !strides16({p.os[0], p.os[1], p.kc[0], p.kc[1], p.kc[2], p.vc[0], p.vc[1], p.vc[2]}, 2))
+    return fail(ctx, LLMR_EINVAL, "tensors, gains, tables and strides must be 16-byte aligned");
+  if (!a4(positions) || !a4(slots)) return fail(ctx, LLMR_EINVAL, "positions or slots is misaligned");
+  if (q != nullptr && q == q_out &&
+      (d->in_dtype != d->dtype || p.qs[0] != p.os[0] || p.qs[1] != p.os[1]))
+    return fail(ctx, LLMR_EINVAL, "q_out may be q only with its type and strides");
+  const bool half = d->flags & LLMR_ROPE_HALF;
+#define LLMR_PP(DD)                                                                         \
+  return d->in_dtype == LLMR_F32   ? launch_paged_prologue_o<DD, float>(ctx, d->dtype, half, p)   \
+         : d->in_dtype == LLMR_F16 ? launch_paged_prologue_o<DD, __half>(ctx, d->dtype, half, p)  \
+                                   : launch_paged_prologue_o<DD, __nv_bfloat16>(ctx, d->dtype, half, p)
+  if (D == 128) LLMR_PP(128);
+  LLMR_PP(64);
+#undef LLMR_PP
+}
+
+}  // extern "C"

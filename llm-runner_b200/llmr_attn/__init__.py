@@ -16,7 +16,15 @@ argument order, over the C-ABI library `libllmr_attn.so` (include/llmr_attn.h):
     split_qkv(ctx, qkv, q, k, v, dim, n_rows)
 
 plus the fused op `attention_fused` that replaces the whole 8-dispatch
-sequence of a DiT attention block. Buffers are torch CUDA tensors (device
+sequence of a DiT attention block, and, for the text models beside it
+(grouped heads, causal):
+
+    attention_causal(ctx, q, k, v, o, cu_seqlens, scale=)       whole packed prompts
+    paged_plan(ctx, ctx_lens, new_lens, ...)                    pages, slots, positions
+    paged_prologue(ctx, q, k, v, q_out, k_cache, v_cache, ...)  norm + RoPE + cache write
+    attention_paged(ctx, q, k_cache, v_cache, o, cu_q, kv_lens, block_table, ...)
+
+Buffers are torch CUDA tensors (device
 memory and streams only; all compute is in the library's CUDA kernels).
 There is no CPU fallback: importing this package without the built library
 raises, and every op on a machine without an sm_100 GPU fails with
@@ -42,7 +50,7 @@ _STATUS_NAMES = {0: "LLMR_OK", 1: "LLMR_EINVAL", 2: "LLMR_ENOMEM", 3: "LLMR_ECUD
 
 F32, F16, BF16 = 0, 1, 2
 BSHD, BHSD = 0, 1
-NORM_Q, NORM_K, ROPE, EXACT, LSE, MERGE = 1, 2, 4, 8, 16, 32
+NORM_Q, NORM_K, ROPE, EXACT, LSE, MERGE, ROPE_HALF = 1, 2, 4, 8, 16, 32, 64
 
 
 class LlmrError(RuntimeError):
@@ -92,6 +100,49 @@ class ProjDesc(ctypes.Structure):
         ("dtype", ctypes.c_int), ("split_row", ctypes.c_uint32),
         ("o_row_stride", ctypes.c_uint64), ("hidden_row_stride", ctypes.c_uint64),
     ]
+
+
+class CausalDesc(ctypes.Structure):
+    """llmr_causal_desc (include/llmr_attn.h)."""
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("n_seqs", "total_tokens", "n_heads", "n_kv_heads",
+                                                "head_dim")]
+                + [("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int), ("scale", ctypes.c_float)]
+                + [(n, ctypes.c_uint64) for n in (
+                    "q_row_stride", "k_row_stride", "v_row_stride", "o_row_stride",
+                    "q_head_stride", "k_head_stride", "v_head_stride", "o_head_stride")])
+
+
+class PagedDesc(ctypes.Structure):
+    """llmr_paged_desc (include/llmr_attn.h)."""
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("n_seqs", "total_tokens", "max_q_len", "n_heads",
+                                                "n_kv_heads", "head_dim")]
+                + [("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int), ("scale", ctypes.c_float)]
+                + [(n, ctypes.c_uint32) for n in ("page_size", "num_pages", "max_pages")]
+                + [(n, ctypes.c_uint64) for n in (
+                    "table_stride", "q_row_stride", "o_row_stride", "q_head_stride",
+                    "o_head_stride", "k_page_stride", "k_row_stride", "k_head_stride",
+                    "v_page_stride", "v_row_stride", "v_head_stride")])
+
+
+class PlanDesc(ctypes.Structure):
+    """llmr_plan_desc (include/llmr_attn.h)."""
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("n_seqs", "max_tokens", "page_size", "num_pages",
+                                                "free_capacity", "max_pages")]
+                + [("table_stride", ctypes.c_uint64)])
+
+
+class PagedPrologueDesc(ctypes.Structure):
+    """llmr_paged_prologue_desc (include/llmr_attn.h)."""
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("total_tokens", "n_heads", "n_kv_heads",
+                                                "head_dim")]
+                + [("in_dtype", ctypes.c_int), ("dtype", ctypes.c_int),
+                   ("flags", ctypes.c_uint32), ("eps", ctypes.c_float)]
+                + [(n, ctypes.c_uint32) for n in ("page_size", "num_pages", "rope_rows")]
+                + [(n, ctypes.c_uint64) for n in (
+                    "q_row_stride", "k_row_stride", "v_row_stride", "q_out_row_stride",
+                    "q_head_stride", "k_head_stride", "v_head_stride", "q_out_head_stride",
+                    "k_page_stride", "k_cache_row_stride", "k_cache_head_stride",
+                    "v_page_stride", "v_cache_row_stride", "v_cache_head_stride")])
 
 
 class IpcHandle(ctypes.Structure):
@@ -149,6 +200,11 @@ def _load() -> ctypes.CDLL:
                                         vp, vp, vp, vp, vp]),
         "llmr_out_project": (i32, [vp, ctypes.POINTER(ProjDesc), vp, vp, vp, vp, vp, vp, vp,
                                    vp]),
+        "llmr_attention_causal": (i32, [vp, ctypes.POINTER(CausalDesc), vp, vp, vp, vp, vp, vp]),
+        "llmr_attention_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedDesc)]),
+        "llmr_attention_paged": (i32, [vp, ctypes.POINTER(PagedDesc)] + [vp] * 8),
+        "llmr_paged_plan": (i32, [vp, ctypes.POINTER(PlanDesc)] + [vp] * 10),
+        "llmr_paged_prologue": (i32, [vp, ctypes.POINTER(PagedPrologueDesc)] + [vp] * 12),
         "llmr_ipc_export": (i32, [vp, vp, ctypes.POINTER(IpcHandle)]),
         "llmr_ipc_open": (i32, [vp, ctypes.POINTER(IpcHandle), ctypes.POINTER(vp)]),
         "llmr_ipc_close": (i32, [vp, vp]),
@@ -504,6 +560,253 @@ def out_project(ctx: Context, o, hidden, w0, w1=None, *, batch: int, seq_len: in
                                    _ptr(hidden)))
 
 
+# ------------------------------------------------- causal prompts and a paged cache
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise LlmrError(EINVAL, what)
+
+
+def _stride(t, dim: int) -> int:
+    """The element stride of a dimension; 0 (the dense default) where it is never stepped."""
+    if t.shape[dim] <= 1:
+        return 0
+    _need(t.stride(dim) > 0, "a broadcast (stride 0) dimension is not supported")
+    return t.stride(dim)
+
+
+def _rows(t, name: str, dtypes, tokens: int, heads: int, dim: int):
+    """`t` as [tokens, heads, dim] with dense elements (an output may be [tokens, heads*dim])."""
+    _need(t.dim() in (2, 3), f"{name} must be [tokens, heads, head_dim]")
+    if t.dim() == 2:
+        _need(t.shape[1] == heads * dim and (t.shape[0] == 0 or t.stride(1) == 1),
+              f"{name} must be [{tokens}, {heads * dim}]")
+        t = t.unflatten(1, (heads, dim))
+    _need(tuple(t.shape) == (tokens, heads, dim),
+          f"{name} is {tuple(t.shape)}, not {(tokens, heads, dim)}")
+    _need(t.numel() == 0 or t.stride(2) == 1, f"{name}: elements of a row must be dense")
+    _need(_dtype_code(t) in dtypes, f"{name}: unsupported dtype {t.dtype}")
+    return t
+
+
+def _vector(t, name: str, length: int, dtype: str = "int32") -> None:
+    _need(t.dim() == 1 and t.shape[0] == length and (length <= 1 or t.stride(0) == 1),
+          f"{name} must be a dense vector of {length}")
+    _need(str(t.dtype) == f"torch.{dtype}", f"{name} must be {dtype}")
+
+
+def _on_device(ctx: "Context", **tensors) -> None:
+    for name, t in tensors.items():
+        _need(t is None or (t.device.type == "cuda" and t.device.index == ctx.device),
+              f"{name} must be on cuda:{ctx.device}")
+
+
+def _lse(lse, heads: int, tokens: int) -> None:
+    if lse is not None:
+        _need(tuple(lse.shape) == (heads, tokens) and lse.is_contiguous()
+              and str(lse.dtype) == "torch.float32", f"lse must be fp32 [{heads}, {tokens}], dense")
+
+
+def _heads(q, name_k: str, kv_heads: int) -> None:
+    _need(q.dim() == 3, "q must be [tokens, heads, head_dim]")
+    _need(q.shape[2] in (64, 128), "head_dim must be 64 or 128")
+    _need(kv_heads > 0 and q.shape[1] > 0 and q.shape[1] % kv_heads == 0,
+          f"q's {q.shape[1]} heads are no multiple of {name_k}'s {kv_heads}")
+
+
+def attention_causal(ctx: Context, q, k, v, o, cu_seqlens, *, scale: float, lse=None) -> None:
+    """Causal attention of packed prompts with grouped heads.
+
+    q [tokens, heads, D], k/v [tokens, kv_heads, D] (fp16 or bf16, any row and
+    head strides); o [tokens, heads, D] or [tokens, heads*D] (fp16, bf16 or
+    fp32). Sequence i is rows cu_seqlens[i]:cu_seqlens[i+1] (int32, on the
+    device); rows behind the last keep what o and lse hold. lse: fp32
+    [heads, tokens]."""
+    _need(k.dim() == 3, "k must be [tokens, kv_heads, head_dim]")
+    _heads(q, "k", k.shape[1])
+    t, h, dim = q.shape
+    hk = k.shape[1]
+    q = _rows(q, "q", (F16, BF16), t, h, dim)
+    k = _rows(k, "k", (_dtype_code(q),), t, hk, dim)
+    v = _rows(v, "v", (_dtype_code(q),), t, hk, dim)
+    o = _rows(o, "o", (F32, F16, BF16), t, h, dim)
+    _need(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "cu_seqlens must be [n_seqs + 1]")
+    _vector(cu_seqlens, "cu_seqlens", cu_seqlens.shape[0])
+    _lse(lse, h, t)
+    _on_device(ctx, q=q, k=k, v=v, o=o, cu_seqlens=cu_seqlens, lse=lse)
+    d = CausalDesc(n_seqs=cu_seqlens.shape[0] - 1, total_tokens=t, n_heads=h, n_kv_heads=hk,
+                   head_dim=dim, dtype=_dtype_code(q), out_dtype=_dtype_code(o), scale=scale,
+                   q_row_stride=_stride(q, 0), q_head_stride=_stride(q, 1),
+                   k_row_stride=_stride(k, 0), k_head_stride=_stride(k, 1),
+                   v_row_stride=_stride(v, 0), v_head_stride=_stride(v, 1),
+                   o_row_stride=_stride(o, 0), o_head_stride=_stride(o, 1))
+    ctx.check(lib.llmr_attention_causal(ctx.handle, ctypes.byref(d), _ptr(cu_seqlens), _ptr(q),
+                                        _ptr(k), _ptr(v), _ptr(o), _ptr(lse)))
+
+
+def _cache(t, name: str, dtype: int, shape=None):
+    _need(t.dim() == 4, f"{name} must be [pages, page_size, kv_heads, head_dim]")
+    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name} is {tuple(t.shape)}, not {shape}")
+    _need(t.numel() > 0 and t.stride(3) == 1, f"{name}: elements of a row must be dense")
+    _need(_dtype_code(t) == dtype, f"{name}: dtype {t.dtype} differs")
+
+
+def attention_paged_workspace_bytes(*, n_seqs: int, total_tokens: int, max_q_len: int,
+                                    n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Workspace of attention_paged for these bounds (ctx.reserve)."""
+    d = PagedDesc(n_seqs=n_seqs, total_tokens=total_tokens, max_q_len=max_q_len, n_heads=n_heads,
+                  n_kv_heads=n_kv_heads, head_dim=head_dim, dtype=F16, out_dtype=F16, scale=1.0,
+                  page_size=16, num_pages=1, max_pages=1)
+    n = int(lib.llmr_attention_paged_workspace_bytes(ctypes.byref(d)))
+    _need(n > 0, "head_dim must be 64 or 128 and n_heads a multiple of n_kv_heads")
+    return n
+
+
+def attention_paged(ctx: Context, q, k_cache, v_cache, o, cu_q, kv_lens, block_table, *,
+                    scale: float, max_q_len: int, lse=None) -> None:
+    """Attention of new tokens over a paged cache.
+
+    q, o: packed rows as in attention_causal, request i's newest tokens at
+    cu_q[i]:cu_q[i+1]; caches [pages, page_size, kv_heads, D] of q's type (any
+    strides); kv_lens[i] keys (the new ones included) in the pages
+    block_table[i, :]. cu_q, kv_lens, block_table are int32 on the device.
+    max_q_len: at least the new tokens of any one request. Needs
+    attention_paged_workspace_bytes of workspace."""
+    _need(k_cache.dim() == 4, "k_cache must be [pages, page_size, kv_heads, head_dim]")
+    _heads(q, "k_cache", k_cache.shape[2])
+    t, h, dim = q.shape
+    q = _rows(q, "q", (F16, BF16), t, h, dim)
+    pages, page, hk, _ = k_cache.shape
+    _cache(k_cache, "k_cache", _dtype_code(q), (pages, page, hk, dim))
+    _cache(v_cache, "v_cache", _dtype_code(q), (pages, page, hk, dim))
+    o = _rows(o, "o", (F32, F16, BF16), t, h, dim)
+    _need(kv_lens.dim() == 1, "kv_lens must be [n_seqs]")
+    n = kv_lens.shape[0]
+    _vector(kv_lens, "kv_lens", n)
+    _vector(cu_q, "cu_q", n + 1)
+    _table(block_table, n)
+    _lse(lse, h, t)
+    _need(max_q_len >= 0, "max_q_len must not be negative")
+    _on_device(ctx, q=q, k_cache=k_cache, v_cache=v_cache, o=o, cu_q=cu_q, kv_lens=kv_lens,
+               block_table=block_table, lse=lse)
+    d = PagedDesc(n_seqs=n, total_tokens=t, max_q_len=min(max_q_len, t), n_heads=h, n_kv_heads=hk,
+                  head_dim=dim, dtype=_dtype_code(q), out_dtype=_dtype_code(o), scale=scale,
+                  page_size=page, num_pages=pages, max_pages=block_table.shape[1],
+                  table_stride=_stride(block_table, 0),
+                  q_row_stride=_stride(q, 0), q_head_stride=_stride(q, 1),
+                  o_row_stride=_stride(o, 0), o_head_stride=_stride(o, 1),
+                  k_page_stride=_stride(k_cache, 0), k_row_stride=_stride(k_cache, 1),
+                  k_head_stride=_stride(k_cache, 2), v_page_stride=_stride(v_cache, 0),
+                  v_row_stride=_stride(v_cache, 1), v_head_stride=_stride(v_cache, 2))
+    ctx.check(lib.llmr_attention_paged(ctx.handle, ctypes.byref(d), _ptr(cu_q), _ptr(kv_lens),
+                                       _ptr(block_table), _ptr(q), _ptr(k_cache), _ptr(v_cache),
+                                       _ptr(o), _ptr(lse)))
+
+
+def _table(block_table, n: int) -> None:
+    _need(block_table.dim() == 2 and block_table.shape[0] == n and block_table.shape[1] >= 1
+          and (block_table.shape[1] == 1 or block_table.stride(1) == 1)
+          and str(block_table.dtype) == "torch.int32",
+          f"block_table must be int32 [{n}, max_pages] with dense rows")
+
+
+def paged_plan(ctx: Context, ctx_lens, new_lens, free_pages, n_free, block_table, cu_q, kv_lens,
+               positions, slots, n_free_out, *, page_size: int,
+               num_pages: Optional[int] = None) -> None:
+    """Plans one step on the device (llmr_paged_plan): request i holds
+    ctx_lens[i] tokens and adds new_lens[i]; the pages it lacks come off the
+    top of the stack free_pages[:n_free[0]] into its row of block_table.
+    Writes cu_q [n+1], kv_lens [n], and per token place positions and slots
+    (0 and -1 behind the last token), and n_free_out [1]. kv_lens may be
+    ctx_lens and n_free_out may be n_free. All tensors int32 on the device.
+    num_pages: pages of the cache, against which page numbers are checked."""
+    _need(ctx_lens.dim() == 1 and free_pages.dim() == 1 and positions.dim() == 1,
+          "ctx_lens, free_pages and positions must be vectors")
+    n = ctx_lens.shape[0]
+    for name, t, length in (("ctx_lens", ctx_lens, n), ("new_lens", new_lens, n),
+                            ("free_pages", free_pages, free_pages.shape[0]),
+                            ("n_free", n_free, 1), ("cu_q", cu_q, n + 1), ("kv_lens", kv_lens, n),
+                            ("positions", positions, positions.shape[0]),
+                            ("slots", slots, positions.shape[0]), ("n_free_out", n_free_out, 1)):
+        _vector(t, name, length)
+    _table(block_table, n)
+    _need(page_size > 0, "page_size must be positive")
+    _on_device(ctx, ctx_lens=ctx_lens, new_lens=new_lens, free_pages=free_pages, n_free=n_free,
+               block_table=block_table, cu_q=cu_q, kv_lens=kv_lens, positions=positions,
+               slots=slots, n_free_out=n_free_out)
+    d = PlanDesc(n_seqs=n, max_tokens=positions.shape[0], page_size=page_size,
+                 num_pages=0x7fffffff // page_size if num_pages is None else num_pages,
+                 free_capacity=free_pages.shape[0], max_pages=block_table.shape[1],
+                 table_stride=_stride(block_table, 0))
+    ctx.check(lib.llmr_paged_plan(ctx.handle, ctypes.byref(d), _ptr(ctx_lens), _ptr(new_lens),
+                                  _ptr(free_pages), _ptr(n_free), _ptr(block_table), _ptr(cu_q),
+                                  _ptr(kv_lens), _ptr(positions), _ptr(slots), _ptr(n_free_out)))
+
+
+def paged_prologue(ctx: Context, q, k, v, q_out, k_cache, v_cache, positions, slots, *,
+                   eps: float = 1e-6, q_gain=None, k_gain=None, cos=None, sin=None,
+                   half: bool = False) -> None:
+    """Norm + RoPE of the new tokens' Q and K, K and V into the cache.
+
+    q [tokens, heads, D], k/v [tokens, kv_heads, D] (fp32, fp16 or bf16, one
+    type); q_out of the caches' type (may be q); slots [tokens] from
+    paged_plan (negative: the token is left out). q_gain / k_gain: fp32 [D],
+    None = no norm of that tensor. cos / sin: fp32 [rows, D/2], indexed by
+    positions [tokens]; None = no rotation. half: pairs (i, i + D/2) instead
+    of (2i, 2i+1). q and q_out may both be None (K and V alone)."""
+    _need(k.dim() == 3 and k_cache.dim() == 4, "k must be [tokens, kv_heads, head_dim]")
+    t, hk, dim = k.shape
+    code = _dtype_code(k_cache)
+    _need(code in (F16, BF16), "the caches must be fp16 or bf16")
+    pages, page = k_cache.shape[:2]
+    _cache(k_cache, "k_cache", code, (pages, page, hk, dim))
+    _cache(v_cache, "v_cache", code, (pages, page, hk, dim))
+    k = _rows(k, "k", (F32, F16, BF16), t, hk, dim)
+    v = _rows(v, "v", (_dtype_code(k),), t, hk, dim)
+    _need((q is None) == (q_out is None), "q and q_out go together")
+    h = hk
+    if q is not None:
+        _heads(q, "k", hk)
+        h = q.shape[1]
+        q = _rows(q, "q", (_dtype_code(k),), t, h, dim)
+        q_out = _rows(q_out, "q_out", (code,), t, h, dim)
+    _vector(slots, "slots", t)
+    _need((cos is None) == (sin is None), "cos and sin go together")
+    rows = 0
+    if cos is not None:
+        rows = cos.shape[0]
+        for name, x in (("cos", cos), ("sin", sin)):
+            _need(tuple(x.shape) == (rows, dim // 2) and x.is_contiguous()
+                  and str(x.dtype) == "torch.float32", f"{name} must be fp32 [rows, {dim // 2}]")
+        _need(positions is not None, "cos and sin need positions")
+    _need(cos is not None or not half, "half needs cos and sin")
+    if positions is not None:
+        _vector(positions, "positions", t)
+    for name, g in (("q_gain", q_gain), ("k_gain", k_gain)):
+        if g is not None:
+            _vector(g, name, dim, "float32")
+    _need(q is not None or q_gain is None, "q_gain needs q")
+    _on_device(ctx, q=q, k=k, v=v, q_out=q_out, k_cache=k_cache, v_cache=v_cache,
+               positions=positions, slots=slots, q_gain=q_gain, k_gain=k_gain, cos=cos, sin=sin)
+    d = PagedPrologueDesc(
+        total_tokens=t, n_heads=h, n_kv_heads=hk, head_dim=dim, in_dtype=_dtype_code(k), dtype=code,
+        flags=((NORM_Q if q_gain is not None else 0) | (NORM_K if k_gain is not None else 0)
+               | (ROPE if cos is not None else 0) | (ROPE_HALF if half else 0)),
+        eps=eps, page_size=page, num_pages=pages, rope_rows=rows,
+        k_row_stride=_stride(k, 0), k_head_stride=_stride(k, 1), v_row_stride=_stride(v, 0),
+        v_head_stride=_stride(v, 1), k_page_stride=_stride(k_cache, 0),
+        k_cache_row_stride=_stride(k_cache, 1), k_cache_head_stride=_stride(k_cache, 2),
+        v_page_stride=_stride(v_cache, 0), v_cache_row_stride=_stride(v_cache, 1),
+        v_cache_head_stride=_stride(v_cache, 2))
+    if q is not None:
+        d.q_row_stride, d.q_head_stride = _stride(q, 0), _stride(q, 1)
+        d.q_out_row_stride, d.q_out_head_stride = _stride(q_out, 0), _stride(q_out, 1)
+    ctx.check(lib.llmr_paged_prologue(ctx.handle, ctypes.byref(d), _ptr(positions), _ptr(slots),
+                                      _ptr(q), _ptr(k), _ptr(v), _ptr(q_gain), _ptr(k_gain),
+                                      _ptr(cos), _ptr(sin), _ptr(q_out), _ptr(k_cache),
+                                      _ptr(v_cache)))
+
+
 # --------------------------------------------------------------------- peer buffers
 
 _TYPESTR = {"float16": "<f2", "bfloat16": None, "float32": "<f4", "uint8": "|u1"}
@@ -612,5 +915,7 @@ __all__ = [
     "mrope", "spatial_attention", "vae_attention", "split_qkv", "attention_fused",
     "attention_merge", "rope_tables", "DeviceBuffer", "PeerMapping", "copy_async",
     "copy2d_async", "qkv_project", "QkvDesc", "out_project", "ProjDesc", "attention_varlen",
+    "attention_causal", "attention_paged", "attention_paged_workspace_bytes", "paged_plan",
+    "paged_prologue", "CausalDesc", "PagedDesc", "PlanDesc", "PagedPrologueDesc",
     "IpcHandle", "LIB_PATH", "lib",
 ]

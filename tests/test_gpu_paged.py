@@ -1,0 +1,720 @@
+"""GPU: causal prompts, paged attention, the planner and the paged prologue
+against plain 64-bit forms (paged_reference.py), at the lengths, head
+layouts, strides and masks where they can go wrong, and run together as a
+serving step runs them."""
+import math
+
+import pytest
+import torch
+
+import llmr_attn as L
+import paged_reference as R
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def cumulative(lens):
+    out = [0]
+    for x in lens:
+        out.append(out[-1] + x)
+    return out
+
+
+def randn(seed, *shape, dtype=BF16, size=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * size).to(dtype)
+
+
+# ------------------------------------------------------------- causal prompts
+
+def run_causal(ctx, lens, h, hk, d, dtype, out_dtype, *, pad=0, size=1.0, scale=None, seed=0,
+               qkv=None, o=None):
+    scale = scale or d ** -0.5
+    t = sum(lens) + pad
+    if qkv is None:
+        qkv = (randn(seed, t, h, d, dtype=dtype, size=size), randn(seed + 1, t, hk, d, dtype=dtype, size=size),
+               randn(seed + 2, t, hk, d, dtype=dtype))
+    q, k, v = qkv
+    if pad:   # rows behind the last sequence: whatever they hold must not matter
+        for x in (q, k, v):
+            x[t - pad:] = math.nan
+    if o is None:
+        o = torch.full((t, h, d), 7.0, dtype=out_dtype, device="cuda")
+    lse = torch.full((h, t), 7.0, device="cuda")
+    L.attention_causal(ctx, q, k, v, o, ints(cumulative(lens)), scale=scale, lse=lse)
+    ctx.sync()
+    at = 0
+    for n in lens:
+        if n:
+            w, wl, weight = R.rows_attention(q[at:at + n], k[at:at + n], v[at:at + n], scale)
+            R.check_attention(o[at:at + n], lse[:, at:at + n], w, wl, weight, dtype, d, n,
+                              float(v[at:at + n].abs().max()),
+                              R.score_size(q[at:at + n], k[at:at + n], scale), (lens, at))
+        at += n
+    assert (o[at:] == 7).all() and (lse[:, at:] == 7).all()
+    return o
+
+
+@pytest.mark.parametrize("h,hk,d", [(4, 4, 64), (8, 2, 128), (14, 2, 64), (7, 1, 128), (16, 1, 64),
+                                    (6, 2, 128), (40, 8, 64)])
+@pytest.mark.parametrize("lens", [[1], [77], [0, 5, 0, 300, 1, 0], [128, 129, 127], [641]])
+def test_causal_lengths_and_heads(ctx, lens, h, hk, d):
+    run_causal(ctx, lens, h, hk, d, BF16, BF16, pad=3, seed=len(lens))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("out_dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_causal_types(ctx, dtype, out_dtype, d):
+    run_causal(ctx, [200, 57], 8, 4, d, dtype, out_dtype, seed=3)
+
+
+def test_causal_many_sequences(ctx):
+    """More sequences than a warp searches at once, most of them short or empty."""
+    g = torch.Generator().manual_seed(5)
+    lens = torch.randint(0, 9, (1500,), generator=g).tolist()
+    lens[700] = 400
+    run_causal(ctx, lens, 4, 2, 64, F16, F16, pad=2, seed=5)
+
+
+def test_causal_peaked_rows(ctx):
+    """Scores that jump in later key blocks move the running maximum."""
+    h, hk, d, n = 4, 2, 128, 900
+    q, k, v = randn(1, n, h, d), randn(2, n, hk, d), randn(3, n, hk, d)
+    k[300] *= 6
+    k[650] *= 12
+    run_causal(ctx, [n], h, hk, d, BF16, BF16, qkv=(q, k, v))
+    run_causal(ctx, [n], h, hk, d, F16, F16, qkv=(q.to(F16), k.to(F16), v.to(F16)))
+
+
+def test_causal_long(ctx):
+    run_causal(ctx, [5000], 4, 1, 128, BF16, BF16, seed=9)
+
+
+def test_causal_strides(ctx):
+    """A fused QKV buffer, head-major tensors, and an output with a gap between rows."""
+    lens, h, hk, d = [130, 45], 6, 2, 64
+    t = sum(lens)
+    fused = randn(1, t, (h + 2 * hk) * d, dtype=F16)
+    q, k, v = (x.unflatten(1, (-1, d)) for x in fused.split((h * d, hk * d, hk * d), 1))
+    want = run_causal(ctx, lens, h, hk, d, F16, F16, qkv=(q, k, v))
+    major = [x.permute(1, 0, 2).contiguous().permute(1, 0, 2) for x in (q, k, v)]
+    wide = torch.full((t, h * d + 64), 7.0, dtype=F16, device="cuda")
+    L.attention_causal(ctx, *major, wide[:, :h * d], ints(cumulative(lens)), scale=d ** -0.5)
+    ctx.sync()
+    assert torch.equal(wide[:, :h * d].view(t, h, d), want)
+    assert (wide[:, h * d:] == 7).all()
+
+
+def test_causal_neighbours_do_not_leak(ctx):
+    """NaN and infinities in one sequence leave the others as they were; a NaN key later in
+    the same sequence leaves the rows before it."""
+    lens, h, hk, d = [100, 60, 200], 4, 2, 128
+    t = sum(lens)
+    q, k, v = randn(1, t, h, d), randn(2, t, hk, d), randn(3, t, hk, d)
+    clean = run_causal(ctx, lens, h, hk, d, BF16, BF16, qkv=(q, k, v))
+    k[100:160] = math.nan
+    v[100:160] = math.inf
+    k[330] = math.nan
+    o = torch.zeros_like(clean)
+    L.attention_causal(ctx, q, k, v, o, ints(cumulative(lens)), scale=d ** -0.5)
+    ctx.sync()
+    keep = torch.ones(t, dtype=torch.bool)
+    keep[100:160] = False
+    keep[330:] = False
+    assert torch.equal(o[keep.cuda()], clean[keep.cuda()])
+
+
+def test_causal_same_bits_twice(ctx):
+    a = run_causal(ctx, [700, 3, 250], 8, 2, 128, BF16, BF16, seed=1)
+    b = run_causal(ctx, [700, 3, 250], 8, 2, 128, BF16, BF16, seed=1)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("cu", [[0, 50, 40, 60], [0, 10, 20, 1000], [-5, 10, 20, 30]])
+def test_causal_bad_offsets_are_reported(ctx, cu):
+    q, k, v = randn(1, 60, 4, 64), randn(2, 60, 2, 64), randn(3, 60, 2, 64)
+    o = torch.zeros_like(q)
+    L.attention_causal(ctx, q, k, v, o, ints(cu), scale=0.125)
+    with pytest.raises(L.LlmrError) as e:
+        ctx.sync()
+    assert e.value.status == L.EINVAL
+    ctx.sync()   # reported once
+
+
+# -------------------------------------------------------------- paged attention
+
+class Paged:
+    """Requests over a cache whose unused rows and pages are NaN."""
+
+    def __init__(self, q_lens, kv_lens, h, hk, d, page, dtype, *, pad=0, seed=0, size=1.0,
+                 layout="dense", spare=3):
+        self.q_lens, self.kv_list, self.d, self.dtype = q_lens, kv_lens, d, dtype
+        need = [-(-x // page) for x in kv_lens]
+        pages = sum(need) + spare
+        shape = (pages, page, hk, d)
+        if layout == "dense":
+            kc, vc = (torch.full(shape, math.nan, dtype=dtype, device="cuda") for _ in range(2))
+        elif layout == "together":      # K and V of a page side by side
+            both = torch.full((pages, 2, page, hk, d), math.nan, dtype=dtype, device="cuda")
+            kc, vc = both[:, 0], both[:, 1]
+        else:                           # heads outside the rows of a page
+            kc, vc = (torch.full((pages, hk, page, d), math.nan, dtype=dtype, device="cuda")
+                      .permute(0, 2, 1, 3) for _ in range(2))
+        order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+        table = torch.full((len(kv_lens), max(need + [1]) + 2), -1, dtype=torch.int32)
+        self.k, self.v = [], []
+        for i, n in enumerate(kv_lens):
+            k = randn(seed + 10 * i + 1, n, hk, d, dtype=dtype, size=size)
+            v = randn(seed + 10 * i + 2, n, hk, d, dtype=dtype)
+            for c in range(need[i]):
+                pg = order.pop()
+                table[i, c] = pg
+                part = slice(c * page, min(n, (c + 1) * page))
+                kc[pg, :part.stop - part.start] = k[part]
+                vc[pg, :part.stop - part.start] = v[part]
+            self.k.append(k)
+            self.v.append(v)
+        t = sum(q_lens) + pad
+        self.q = randn(seed + 7, t, h, d, dtype=dtype, size=size)
+        self.kc, self.vc, self.table = kc, vc, table.cuda()
+        self.cu, self.kv = ints(cumulative(q_lens)), ints(kv_lens)
+        self.h, self.hk, self.t = h, hk, t
+
+    def run(self, ctx, out_dtype=None, scale=None, max_q=None):
+        scale = scale or self.d ** -0.5
+        max_q = max_q or max(self.q_lens + [1])
+        self.o = torch.full((self.t, self.h, self.d), 7.0, dtype=out_dtype or self.dtype, device="cuda")
+        self.lse = torch.full((self.h, self.t), 7.0, device="cuda")
+        ctx.reserve(L.attention_paged_workspace_bytes(
+            n_seqs=len(self.q_lens), total_tokens=self.t, max_q_len=max_q, n_heads=self.h,
+            n_kv_heads=self.hk, head_dim=self.d))
+        L.attention_paged(ctx, self.q, self.kc, self.vc, self.o, self.cu, self.kv, self.table,
+                          scale=scale, max_q_len=max_q, lse=self.lse)
+        ctx.sync()
+        return self.o
+
+    def check(self, ctx, **kw):
+        self.run(ctx, **kw)
+        scale = kw.get("scale") or self.d ** -0.5
+        at = 0
+        for i, n in enumerate(self.q_lens):
+            if n:
+                rows = slice(at, at + n)
+                w, wl, weight = R.rows_attention(self.q[rows], self.k[i], self.v[i], scale)
+                vmax = float(self.v[i].abs().max()) if self.kv_list[i] else 0.0
+                R.check_attention(self.o[rows], self.lse[:, rows], w, wl, weight, self.dtype, self.d,
+                                  self.kv_list[i], vmax, R.score_size(self.q[rows], self.k[i], scale),
+                                  (i, n, self.kv_list[i]))
+            at += n
+        assert (self.o[at:] == 7).all() and (self.lse[:, at:] == 7).all()
+        return self.o
+
+
+HEADS = [(4, 4, 64), (8, 2, 128), (14, 2, 64), (7, 1, 128), (32, 2, 64), (6, 2, 128)]
+
+
+@pytest.mark.parametrize("h,hk,d", HEADS)
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_decode(ctx, h, hk, d, page):
+    """One token each: contexts from nothing to several splits, a padded batch."""
+    kv = [1, 17, 0, 128, 700, 129, 2500, 15]
+    Paged([1] * len(kv), kv, h, hk, d, page, BF16, pad=2, seed=page).check(ctx)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("q_lens,kv_lens", [
+    ([5, 1, 0, 3], [300, 40, 90, 3]),
+    ([40, 7], [1000, 7]),
+    ([129, 300], [129, 1111]),
+])
+def test_chunks(ctx, page, q_lens, kv_lens):
+    Paged(q_lens, kv_lens, 8, 2, 128, page, BF16, pad=1, seed=page).check(ctx)
+
+
+@pytest.mark.parametrize("h,hk,d", HEADS)
+@pytest.mark.parametrize("q", [2, 3, 9, 33, 150])
+def test_chunk_heads(ctx, h, hk, d, q):
+    Paged([q, 1, q - 1], [1500, 260, q + 40], h, hk, d, 32, F16, seed=q).check(ctx)
+
+
+@pytest.mark.parametrize("q", [1, 4, 20, 200])
+def test_rows_without_a_key(ctx, q):
+    """More queries than keys: the first rows see nothing and give 0 and -inf."""
+    kv = [q // 2, 0, q, 600]
+    p = Paged([q] * 4, kv, 8, 2, 128, 16, BF16, seed=q)
+    p.check(ctx)
+    assert (p.o[q:2 * q] == 0).all() and (p.lse[:, q:2 * q] == -math.inf).all()
+
+
+@pytest.mark.parametrize("q", [1, 200])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("out_dtype", [F16, BF16, F32])
+def test_paged_types(ctx, q, dtype, out_dtype):
+    Paged([q, q], [333, 1200], 8, 2, 64, 16, dtype, seed=q).check(ctx, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("q", [1, 6, 100])
+@pytest.mark.parametrize("layout", ["together", "heads"])
+def test_cache_layouts(ctx, q, layout):
+    Paged([q, q], [777, 90 + q], 8, 2, 128, 32, BF16, seed=q, layout=layout).check(ctx)
+
+
+@pytest.mark.parametrize("q", [1, 130])
+@pytest.mark.parametrize("h,hk,d", [(8, 1, 128), (4, 2, 64)])
+def test_one_long_request(ctx, q, h, hk, d):
+    """The long axis is split over the card and joined."""
+    p = Paged([q], [20011], h, hk, d, 16, BF16, seed=2)
+    a = p.check(ctx).clone()
+    assert torch.equal(p.run(ctx), a)       # and joined in the same order every time
+
+
+def test_peaked_and_growing_scores(ctx):
+    for q in (1, 130):
+        p = Paged([q], [3000], 8, 2, 128, 16, F16, seed=4)
+        for at, f in ((500, 5), (1500, 10), (2900, 18)):
+            p.k[0][at] *= f
+            pg = int(p.table[0, at // 16])
+            p.kc[pg, at % 16] *= f
+        p.check(ctx)
+
+
+def test_padded_bound_and_ragged_mix(ctx):
+    """max_q_len above every request's rows; decodes and chunks in one call."""
+    q = [1, 64, 1, 5, 0, 200, 1]
+    kv = [900, 64, 1, 3000, 0, 1500, 129]
+    Paged(q, kv, 16, 4, 128, 16, BF16, pad=5, seed=8).check(ctx, max_q=300)
+
+
+def test_many_requests(ctx):
+    g = torch.Generator().manual_seed(3)
+    kv = torch.randint(0, 400, (700,), generator=g).tolist()
+    Paged([1] * 700, kv, 4, 2, 64, 16, F16, seed=1).check(ctx)
+
+
+def test_cache_beyond_32_bit_offsets(ctx):
+    """A cache of more than 2^31 elements: pages at its far end."""
+    h, hk, d, page = 8, 8, 128, 256
+    pages = (1 << 31) // (page * hk * d) + 9
+    kc = torch.empty((pages, page, hk, d), dtype=F16, device="cuda")
+    vc = torch.empty_like(kc)
+    k, v = randn(1, 300, hk, d, dtype=F16), randn(2, 300, hk, d, dtype=F16)
+    table = ints([[pages - 1, pages - 4]])
+    for src, c in ((k, kc), (v, vc)):
+        c[pages - 1] = src[:256]
+        c[pages - 4, :44] = src[256:]
+    for n in (1, 100):
+        q = randn(3, n, h, d, dtype=F16)
+        o = torch.zeros_like(q)
+        ctx.reserve(L.attention_paged_workspace_bytes(n_seqs=1, total_tokens=n, max_q_len=n, n_heads=h,
+                                                      n_kv_heads=hk, head_dim=d))
+        L.attention_paged(ctx, q, kc, vc, o, ints([0, n]), ints([300]), table, scale=d ** -0.5,
+                          max_q_len=n)
+        ctx.sync()
+        w, _, weight = R.rows_attention(q, k, v, d ** -0.5)
+        R.check_attention(o, None, w, None, weight, F16, d, 300, float(v.abs().max()),
+                          R.score_size(q, k, d ** -0.5))
+    slots = ints([(pages - 1) * page + 7])
+    L.paged_prologue(ctx, None, k[:1], v[:1], None, kc, vc, None, slots)
+    ctx.sync()
+    assert torch.equal(kc[pages - 1, 7], k[0]) and torch.equal(vc[pages - 1, 7], v[0])
+
+
+@pytest.mark.parametrize("q,fault", [(130, "max_q")] + [
+    (q, f) for q in (1, 130) for f in ("page_high", "page_low", "kv_long", "kv_negative", "cu")])
+def test_bad_device_values_are_reported(ctx, q, fault):
+    p = Paged([q, q], [500, 700], 8, 2, 128, 16, BF16, seed=1)
+    max_q = q
+    if fault == "page_high":
+        p.table[0, 3] = p.kc.shape[0]
+    elif fault == "page_low":
+        p.table[0, 3] = -9
+    elif fault == "kv_long":
+        p.kv[0] = 1 << 20
+    elif fault == "kv_negative":
+        p.kv[0] = -4
+    elif fault == "cu":
+        p.cu[2] = 2 * q + 9
+    else:
+        max_q = q - 1
+    with pytest.raises(L.LlmrError) as e:
+        p.run(ctx, max_q=max_q)
+    assert e.value.status == L.EINVAL
+    good = Paged([q, q], [500, 700], 8, 2, 128, 16, BF16, seed=1)
+    good.check(ctx)     # and the context goes on
+
+
+# ------------------------------------------------------------------- planner
+
+def run_plan(ctx, ctx_lens, new_lens, page, *, free_n=None, room=None, cols=None, inplace=False,
+             seed=0, table_gap=0):
+    held = [-(-c // page) for c in ctx_lens]
+    last = [-(-(c + n) // page) for c, n in zip(ctx_lens, new_lens)]
+    need = sum(last) - sum(held)
+    free_n = need + 3 if free_n is None else free_n
+    cols = cols or max(last + [1])
+    n = len(ctx_lens)
+    room = sum(new_lens) + 5 if room is None else room
+    order = torch.randperm(sum(held) + free_n + 2, generator=torch.Generator().manual_seed(seed)).tolist()
+    table = [[-1] * cols for _ in range(n)]
+    for i, a in enumerate(held):
+        for c in range(min(a, cols)):
+            table[i][c] = order.pop()
+    free = order[:free_n]
+    dev_table = torch.full((n, cols + table_gap), -7, dtype=torch.int32)
+    dev_table[:, :cols] = torch.tensor(table, dtype=torch.int32).view(n, cols)
+    dev_table = dev_table.cuda()
+    c, new, nf = ints(ctx_lens), ints(new_lens), ints([free_n])
+    fp = ints(free + [99999])       # capacity beyond the stack's top
+    fill = lambda k: torch.full((k,), -55, dtype=torch.int32, device="cuda")
+    cu, pos, slots = fill(n + 1), fill(room), fill(room)
+    kv, nfo = (c, nf) if inplace else (fill(n), fill(1))
+    L.paged_plan(ctx, c, new, fp, nf, dev_table[:, :cols], cu, kv, pos, slots, nfo, page_size=page)
+    got = lambda t: t.cpu().tolist()
+    return (table, free), (lambda: (got(dev_table[:, :cols]), got(cu), got(kv), got(pos), got(slots),
+                                    int(nfo))), dev_table
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("ctx_lens,new_lens", [
+    ([0], [1]), ([16, 15, 17, 0, 64], [1, 1, 1, 1, 1]), ([5, 0, 300], [0, 0, 0]),
+    ([0, 100, 31, 0], [700, 0, 33, 5000]), ([], []),
+])
+def test_plan(ctx, page, inplace, ctx_lens, new_lens):
+    (table, free), read, dev = run_plan(ctx, ctx_lens, new_lens, page, inplace=inplace, table_gap=3)
+    ctx.sync()
+    assert read() == R.plan(ctx_lens, new_lens, free, table, page, sum(new_lens) + 5)
+    assert (dev[:, -3:] == -7).all()
+
+
+@pytest.mark.parametrize("n", [33, 1025, 4096])
+def test_plan_many_requests(ctx, n):
+    g = torch.Generator().manual_seed(n)
+    c = torch.randint(0, 200, (n,), generator=g).tolist()
+    new = torch.randint(0, 12, (n,), generator=g).tolist()
+    (table, free), read, _ = run_plan(ctx, c, new, 16, seed=n)
+    ctx.sync()
+    assert read() == R.plan(c, new, free, table, 16, sum(new) + 5)
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("what", ["pages", "tokens", "table", "negative", "huge"])
+def test_plan_that_cannot_be_made_changes_nothing(ctx, what, inplace):
+    c, new, kw = [40, 3, 16], [20, 50, 1], {}
+    if what == "pages":
+        kw["free_n"] = 4    # 5 are needed
+    elif what == "tokens":
+        kw["room"] = 70
+    elif what == "table":
+        kw["cols"] = 3
+    elif what == "negative":
+        c = [40, -3, 16]
+        kw.update(cols=5, free_n=9)
+    else:
+        new = [2 ** 31 - 1, 2 ** 31 - 1, 1]
+        kw.update(cols=5, free_n=9, room=80)
+    (table, free), read, _ = run_plan(ctx, c, new, 16, inplace=inplace, **kw)
+    with pytest.raises(L.LlmrError) as e:
+        ctx.sync()
+    assert e.value.status == (L.ENOMEM if what == "pages" else L.EINVAL)
+    room = kw.get("room", 76)
+    if what == "negative":
+        room = 76
+    assert read() == (table, [0] * 4, c, [0] * room, [-1] * room, len(free))
+
+
+# ------------------------------------------------------------------ prologue
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("in_dtype,dtype", [(BF16, BF16), (F16, F16), (F32, BF16), (BF16, F16)])
+@pytest.mark.parametrize("tokens,h,hk,norm,rope", [(1, 8, 2, True, True), (37, 14, 2, True, True),
+                                                   (130, 7, 7, False, True), (9, 40, 8, True, False),
+                                                   (3, 1, 1, False, False)])
+def test_prologue(ctx, d, half, in_dtype, dtype, tokens, h, hk, norm, rope):
+    page, rows, eps = 16, 5000, 1e-6
+    pages = -(-tokens // page) + 4
+    g = torch.Generator().manual_seed(tokens)
+    q, k, v = (randn(i, tokens, n, d, dtype=in_dtype) for i, n in ((1, h), (2, hk), (3, hk)))
+    gains = [torch.rand(d, generator=g).cuda() * 0.4 + 0.8 for _ in range(2)]
+    angle = torch.arange(rows)[:, None].double() * 10000.0 ** (-torch.arange(0, d, 2).double() / d)
+    cos, sin = angle.cos().float().cuda(), angle.sin().float().cuda()
+    pos = torch.randint(0, rows, (tokens,), generator=g).int().cuda()
+    slots = torch.randperm(pages * page, generator=g)[:tokens].int().cuda()
+    kc, vc = (torch.full((pages, page, hk, d), 7.0, dtype=dtype, device="cuda") for _ in range(2))
+    q_out = torch.full((tokens, h, d), 7.0, dtype=dtype, device="cuda")
+    if tokens > 4:
+        slots[2] = -1       # padding
+    L.paged_prologue(ctx, q, k, v, q_out, kc, vc, pos, slots, eps=eps,
+                     q_gain=gains[0] if norm else None, k_gain=gains[1] if norm else None,
+                     cos=cos if rope else None, sin=sin if rope else None, half=half and rope)
+    ctx.sync()
+    want = []
+    for x, gain in ((q, gains[0]), (k, gains[1])):
+        x = R.norm(x, gain, eps) if norm else x.double()
+        want.append(R.rotate(x, cos[pos.long()], sin[pos.long()], half) if rope else x)
+    live = slots >= 0
+    at = slots[live].long()
+    # The norm and the rotation in fp32: at most 16 roundings of values whose
+    # size the row's largest bounds, the sum of D squares halved by the root;
+    # then the output's own half step.
+    def close(got, w):
+        size = w.abs().amax(-1, keepdim=True)
+        tol = w.abs() * R.half_step(dtype) + size * (16 + d / 2) * 2.0 ** -24 + 2.0 ** -25
+        assert ((got.double() - w).abs() <= tol).all()
+    close(q_out[live], want[0][live])
+    close(kc.view(-1, hk, d)[at], want[1][live])
+    assert torch.equal(vc.view(-1, hk, d)[at], v[live].to(dtype))
+    rest = torch.ones(pages * page, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    assert (kc.view(-1, hk, d)[rest] == 7).all() and (vc.view(-1, hk, d)[rest] == 7).all()
+    assert (q_out[~live] == 7).all()
+
+
+def test_prologue_in_place_and_strided(ctx):
+    """q_out = q in a fused buffer, a cache with K and V side by side."""
+    t, h, hk, d = 50, 6, 2, 128
+    fused = randn(1, t, (h + 2 * hk) * d)
+    keep = fused.clone()
+    q, k, v = (x.unflatten(1, (-1, d)) for x in fused.split((h * d, hk * d, hk * d), 1))
+    both = torch.zeros((4, 2, 16, hk, d), dtype=BF16, device="cuda")
+    gain = torch.rand(d, device="cuda") + 0.5
+    slots = ints(list(range(t))[::-1])
+    plain = [torch.zeros((t, h, d), dtype=BF16, device="cuda"), torch.zeros_like(both[:, 0]),
+             torch.zeros_like(both[:, 1])]
+    L.paged_prologue(ctx, q, k, v, plain[0], plain[1], plain[2], None, slots, q_gain=gain)
+    L.paged_prologue(ctx, q, k, v, q, both[:, 0], both[:, 1], None, slots, q_gain=gain)
+    ctx.sync()
+    assert torch.equal(q, plain[0]) and torch.equal(both[:, 0], plain[1])
+    assert torch.equal(both[:, 1], plain[2]) and torch.equal(fused[:, h * d:], keep[:, h * d:])
+
+
+@pytest.mark.parametrize("fault", ["slot", "position", "negative_position"])
+def test_prologue_reports_bad_indices(ctx, fault):
+    t, hk, d = 6, 2, 64
+    k, v = randn(1, t, hk, d), randn(2, t, hk, d)
+    kc, vc = (torch.zeros((2, 16, hk, d), dtype=BF16, device="cuda") for _ in range(2))
+    cos = torch.ones((10, d // 2), device="cuda")
+    sin = torch.zeros_like(cos)
+    pos, slots = ints([0, 1, 2, 3, 4, 5]), ints([0, 1, 2, 3, 4, 5])
+    if fault == "slot":
+        slots[3] = 32
+    elif fault == "position":
+        pos[3] = 10
+    else:
+        pos[3] = -1
+    L.paged_prologue(ctx, None, k, v, None, kc, vc, pos, slots, cos=cos, sin=sin)
+    with pytest.raises(L.LlmrError) as e:
+        ctx.sync()
+    assert e.value.status == L.EINVAL
+    good = [0, 1, 2, 4, 5]
+    assert torch.equal(kc[0, good], k[good]) and (kc[0, 3] == 0).all() and (kc[1] == 0).all()
+
+
+# ------------------------------------------------------------- as they are used
+
+class Server:
+    """Three requests served with the four operators; keeps every token's q, k, v."""
+
+    def __init__(self, ctx, dtype=BF16, room=160):
+        self.ctx, self.dtype, self.room = ctx, dtype, room
+        self.n, self.h, self.hk, self.d, self.page = 3, 8, 2, 128, 16
+        self.pages = 64
+        z = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+        self.lens, self.new, self.cu = z(self.n), z(self.n), z(self.n + 1)
+        self.pos, self.slots = z(room), z(room)
+        self.free = torch.randperm(self.pages, generator=torch.Generator().manual_seed(1)).int().cuda()
+        self.n_free = ints([self.pages])
+        self.table = torch.full((self.n, 20), -1, dtype=torch.int32, device="cuda")
+        shape = (self.pages, self.page, self.hk, self.d)
+        self.kc, self.vc = (torch.full(shape, math.nan, dtype=dtype, device="cuda") for _ in range(2))
+        self.qkv = torch.zeros((room, (self.h + 2 * self.hk) * self.d), dtype=dtype, device="cuda")
+        self.o = torch.zeros((room, self.h, self.d), dtype=dtype, device="cuda")
+        angle = torch.arange(400)[:, None].double() * 10000.0 ** (-torch.arange(0, 128, 2).double() / 128)
+        self.cos, self.sin = angle.cos().float().cuda(), angle.sin().float().cuda()
+        self.gain = torch.rand(self.d, generator=torch.Generator().manual_seed(2)).cuda() + 0.5
+        self.q_rot = torch.zeros((room, self.h, self.d), dtype=dtype, device="cuda")
+        ctx.reserve(L.attention_paged_workspace_bytes(
+            n_seqs=self.n, total_tokens=room, max_q_len=room, n_heads=self.h, n_kv_heads=self.hk,
+            head_dim=self.d))
+
+    def split(self):
+        a, b = self.h * self.d, self.hk * self.d
+        return (x.unflatten(1, (-1, self.d)) for x in self.qkv.split((a, b, b), 1))
+
+    def step(self, max_q):
+        q, k, v = self.split()
+        L.paged_plan(self.ctx, self.lens, self.new, self.free, self.n_free, self.table, self.cu,
+                     self.lens, self.pos, self.slots, self.n_free, page_size=self.page,
+                     num_pages=self.pages)
+        L.paged_prologue(self.ctx, q, k, v, self.q_rot, self.kc, self.vc, self.pos, self.slots,
+                         q_gain=self.gain, k_gain=self.gain, cos=self.cos, sin=self.sin, half=True)
+        L.attention_paged(self.ctx, self.q_rot, self.kc, self.vc, self.o, self.cu, self.lens,
+                          self.table, scale=self.d ** -0.5, max_q_len=max_q)
+
+
+STEPS = [[50, 0, 7], [1, 90, 1], [1, 1, 1], [30, 1, 0], [1, 1, 1], [1, 1, 1]]
+
+
+def feed(server, i):
+    server.new.copy_(torch.tensor(STEPS[i], dtype=torch.int32))
+    server.qkv.copy_(randn(100 + i, *server.qkv.shape, dtype=server.dtype))
+
+
+def whole_prompt(server, steps):
+    """The same tokens as whole prompts through attention_causal, per request and step."""
+    hist = [[[], [], []] for _ in range(server.n)]
+    outs = []
+    done = [0] * server.n
+    for i in range(steps):
+        feed(server, i)
+        q, k, v = (x.clone() for x in server.split())
+        at = 0
+        rows = []
+        for r, n in enumerate(STEPS[i]):
+            pos = torch.arange(done[r], done[r] + n, device="cuda")
+            for part, (x, turn) in enumerate(((q, True), (k, True), (v, False))):
+                y = x[at:at + n]
+                if turn:
+                    y = R.norm(y, server.gain, 1e-6)
+                    y = R.rotate(y, server.cos[pos], server.sin[pos], True).to(server.dtype)
+                hist[r][part].append(y)
+            rows.append((at, n))
+            done[r] += n
+            at += n
+        qs, ks, vs = (torch.cat([torch.cat(hist[r][p]) for r in range(server.n)]) for p in range(3))
+        o = torch.zeros_like(qs)
+        L.attention_causal(server.ctx, qs, ks, vs, o, ints(cumulative(done)), scale=server.d ** -0.5)
+        server.ctx.sync()
+        ends = cumulative(done)
+        outs.append([o[ends[r + 1] - n:ends[r + 1]] for r, (_, n) in enumerate(rows)])
+    return outs
+
+
+def compare_step(server, i, want):
+    at = 0
+    for r, n in enumerate(STEPS[i]):
+        got = server.o[at:at + n].double()
+        # Two kernels' roundings of the numerators (half a step each, beside
+        # values of size ~|v| < 5) and of both outputs, and q or k rounded
+        # the other way where the two norms' fp32 differ in the last place.
+        tol = 4 * R.half_step(server.dtype) * 5
+        assert ((got - want[r].double()).abs() <= tol).all(), (i, r)
+        at += n
+
+
+def test_serving_steps_equal_whole_prompts(ctx):
+    s = Server(ctx)
+    for i in range(len(STEPS)):
+        feed(s, i)
+        s.step(s.room)
+        s.ctx.sync()
+        got = s.o.clone()
+        if i in (0, 1, 3, len(STEPS) - 1):
+            keep = s.new.clone(), s.qkv.clone()
+            want = whole_prompt(s, i + 1)[i]
+            s.new.copy_(keep[0])
+            s.qkv.copy_(keep[1])
+        else:
+            continue
+        s.o.copy_(got)
+        compare_step(s, i, want)
+    used = [int(x) for x in s.lens]
+    assert used == [sum(c) for c in zip(*STEPS)]
+    assert int(s.n_free) == s.pages - sum(-(-u // s.page) for u in used)
+
+
+@pytest.mark.parametrize("max_q", [1, 160])
+def test_captured_step_replays(max_q):
+    """One captured step (plan, prologue, attention) advances by itself and gives the eager bits."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ctx = L.Context(0, stream=stream)
+        eager, graphed = Server(ctx), Server(ctx)
+        first = 0
+        for s in (eager, graphed):
+            feed(s, first)
+            s.step(s.room)
+        ctx.sync()
+        for s in (eager, graphed):
+            feed(s, 2)
+        state = [x.clone() for x in (graphed.lens, graphed.n_free, graphed.table)]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    n0 = ctx.launches
+    with torch.cuda.graph(g, stream=stream):
+        graphed.step(max_q)
+    assert ctx.launches - n0 == 3
+    with torch.cuda.stream(stream):
+        for x, y in zip((graphed.lens, graphed.n_free, graphed.table), state):
+            x.copy_(y)
+        for i in (2, 4, 5):
+            for s in (eager, graphed):
+                feed(s, i)
+            g.replay()
+            eager.step(max_q)
+            ctx.sync()
+            assert torch.equal(eager.o, graphed.o) and torch.equal(eager.lens, graphed.lens)
+            assert torch.equal(eager.table, graphed.table)
+    torch.cuda.synchronize()
+    del g
+    ctx.close()
+
+
+def test_other_stream(ctx):
+    """A context on a stream of its own, inputs made on another and ordered by an event."""
+    s = torch.cuda.Stream()
+    own = L.Context(0, stream=s)
+    q, k, v = randn(1, 300, 8, 64), randn(2, 300, 2, 64), randn(3, 300, 2, 64)
+    o = torch.zeros_like(q)
+    cu = ints([0, 300])
+    s.wait_stream(torch.cuda.current_stream())
+    L.attention_causal(own, q, k, v, o, cu, scale=0.125)
+    own.sync()
+    assert torch.equal(o, run_causal(ctx, [300], 8, 2, 64, BF16, BF16, qkv=(q, k, v)))
+    own.close()
+
+
+def test_refusals_of_the_library(ctx):
+    """What the host can see is refused before anything is launched."""
+    q, k, v = randn(1, 40, 4, 64), randn(2, 40, 2, 64), randn(3, 40, 2, 64)
+    o, cu = torch.zeros_like(q), ints([0, 40])
+    n0 = ctx.launches
+
+    def refused(f, status=L.EINVAL):
+        with pytest.raises(L.LlmrError) as e:
+            f()
+        assert e.value.status == status
+
+    for bad in (0.0, -1.0, math.nan, math.inf):
+        refused(lambda: L.attention_causal(ctx, q, k, v, o, cu, scale=bad))
+    odd = torch.zeros(40 * 4 * 64 + 8, dtype=BF16, device="cuda")[1:-7].view(40, 4, 64)
+    refused(lambda: L.attention_causal(ctx, odd, k, v, o, cu, scale=0.1))
+    refused(lambda: L.attention_causal(ctx, q, k, v, odd, cu, scale=0.1))
+    refused(lambda: L.attention_causal(ctx, q, k.cpu(), v, o, cu, scale=0.1))
+    kc = torch.zeros((4, 24, 2, 64), dtype=BF16, device="cuda")      # page size
+    table = ints([[0, 1]])
+    refused(lambda: L.attention_paged(ctx, q, kc, kc, o, cu, ints([40]), table, scale=0.1, max_q_len=40))
+    fresh = L.Context(0)
+    kc = torch.zeros((4, 16, 2, 64), dtype=BF16, device="cuda")
+    refused(lambda: L.attention_paged(fresh, q, kc, kc, o, cu, ints([32]), table, scale=0.1,
+                                      max_q_len=40), L.ENOMEM)
+    assert ctx.launches == n0 and fresh.launches == 0
+    fresh.close()
+    # Nothing to do is no error and launches nothing.
+    e = lambda *s: torch.zeros(s, dtype=BF16, device="cuda")
+    L.attention_causal(ctx, e(0, 4, 64), e(0, 2, 64), e(0, 2, 64), e(0, 4, 64), ints([0]), scale=0.1)
+    assert ctx.launches == n0
+
+
+def test_the_current_device_stays(ctx):
+    before = torch.cuda.current_device()
+    run_causal(ctx, [10], 4, 2, 64, BF16, BF16)
+    assert torch.cuda.current_device() == before
