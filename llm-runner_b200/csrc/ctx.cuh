@@ -32,7 +32,8 @@ struct llmr_ctx {
   int *d_sync = nullptr;
   unsigned long long *timeline = nullptr;  // LLMR_TIMELINE builds: event buffer
   uint64_t launches = 0;
-  int num_sms = 0;
+  int num_sms = 0;    // SMs the persistent kernels may use (llmr_ctx_set_sm_budget)
+  int total_sms = 0;  // SMs of the device
   bool prof_on = false;
   bool prof_valid = false;
   cudaEvent_t prof_ev[3] = {nullptr, nullptr, nullptr};

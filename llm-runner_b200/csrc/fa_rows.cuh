@@ -1,0 +1,689 @@
+// Causal attention with grouped heads on the 5th-generation tensor cores, for
+// whole packed prompts and for chunks of new tokens over a paged cache.
+//
+// A tile's 128 query rows are the `group` query heads that share one key /
+// value head, for tpt = 128 / group consecutive tokens (row = token * group +
+// head), so K and V are read once for the whole group, a chunk of few
+// tokens still fills a tile, and the triangle wastes little: only blocks that
+// some row of the tile sees are visited.
+//
+// Work unit: (request, key/value head, 2 * tpt tokens[, part of the keys]).
+// Requests' offsets are device data, so units are numbered without knowing
+// them: request i starts at virtual tile cu[i] / (2 tpt) + i, which leaves room
+// for its tiles and at most one empty one behind them, and is found by
+// searching cu. Units are handed out last tokens first (the longest rows of a
+// causal prompt first), by cluster launch control: a CTA takes over units
+// whose CTAs have not started, so no counter in memory is needed and a light
+// unit's CTA goes on at once.
+//
+// CTA: 384 threads, as the non-causal kernel divides them:
+//   warps 0-3 / 4-7  softmax of tile 0 / 1, one query row per thread
+//   warp 8           TMA producer: Q, then K_j, V_j into an NST-slot ring
+//   warp 9           MMA issuer and TMEM owner
+//   warp 10          scheduler: finds the units, one ahead
+//   warp 11          CTA 0: looks through all requests for bad lengths
+// MMA order per key block j: PV0_j, S0_{j+1}, PV1_j, S1_{j+1}, each tile with
+// its own number of blocks. The first blocks need no mask; in those that reach
+// past a row's last key the scores are set to -inf (so P is exactly 0), P V
+// stops at the last key rounded up to 16, and the V rows in between are
+// zeroed in shared memory: what lies behind a request's keys may be NaN.
+//
+// Scores and softmax state are fp32, P is rounded to the inputs' type (half
+// a step, the rounding V's own type has; fp32 P would need a tf32 product at
+// a quarter of the rate), and the row sum takes P before that rounding.
+#pragma once
+#include "fa_tc.cuh"
+#include "paged_kernels.cuh"
+
+namespace llmr {
+
+constexpr int kUnitSlots = 2;  // the unit in work and the next
+// Splitting a unit's keys pays from this many blocks of 128 per part.
+constexpr int kMinSplitBlocks = 8;
+
+struct FaRowsParams {
+  RowsParams rows;
+  int group, tpt, recip;  // recip: r / group = r * recip >> 16 for r < 128
+  int vtiles;             // virtual tiles of all requests
+  int nsplit;             // parts a unit may be cut into
+  int units;              // vtiles * Hk * nsplit
+  int dynamic;            // units are taken over by cluster launch control
+  float scale_log2;
+  float *part_o, *part_lse;  // [unit][part][256 rows]([D])
+};
+
+// One unit, as the scheduler hands it to the other warps.
+struct FaUnit {
+  int kvh;         // -1: no more units
+  int q_row;       // first token's row in q and o
+  int tokens;      // tokens of the unit (tile 0 takes the first tpt)
+  int kv_row;      // packed: the sequence's first row; paged: the request
+  int keys;        // keys the unit's last row sees
+  int pos;         // position of the first token
+  int blk;         // first key block
+  int nb[2];       // key blocks of each tile
+  int part;        // -1, or where the partial result goes
+};
+
+// Blocks of 128 keys that part s of ns takes of n.
+__host__ __device__ __forceinline__ int split_at(int n, int ns, int s) {
+  return (int)((long long)n * s / ns);
+}
+__host__ __device__ __forceinline__ int parts_of(int blocks, int nsplit) {
+  const int most = blocks / kMinSplitBlocks;
+  return most < 1 ? 1 : most < nsplit ? most : nsplit;
+}
+
+// The request that virtual tile vt belongs to: the last with
+// cu[i] / tu + i <= vt. Whole warp, 32 probes at a time.
+__device__ __forceinline__ int find_request(const int *cu, int n, int tu, int vt) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int i = lo + lane * step;
+    const bool le = i < hi && cu[i] / tu + i <= vt;
+    const int c = max(1, __popc(__ballot_sync(0xffffffffu, le)));
+    lo += (c - 1) * step;
+    hi = min(lo + step, hi);
+  }
+  return lo;
+}
+
+// Virtual unit u; false if it is empty. Whole warp.
+template <bool PAGED>
+__device__ __forceinline__ bool fa_unit(const FaRowsParams &p, int u, FaUnit &un) {
+  const int s = u % p.nsplit, vh = u / p.nsplit;
+  const int vt = p.vtiles - 1 - vh / p.rows.Hk;
+  const int tu = 2 * p.tpt;
+  const int r = find_request(p.rows.cu, p.rows.n, tu, vt);
+  int row0, nq, nk;
+  if (!request_rows(p.rows, r, row0, nq, nk)) return false;
+  const int first = (vt - (row0 / tu + r)) * tu;
+  if (first < 0 || first >= nq) return false;
+  un.kvh = vh % p.rows.Hk;
+  un.q_row = row0 + first;
+  un.tokens = min(tu, nq - first);
+  un.kv_row = PAGED ? r : row0;
+  un.pos = nk - nq + first;
+  const int k0 = max(0, un.pos + min(un.tokens, p.tpt));
+  const int k1 = max(0, un.pos + un.tokens);
+  un.keys = k1;
+  const int all = (k1 + 127) / 128;
+  const int parts = parts_of(all, p.nsplit);
+  if (s >= parts) return false;
+  const int end = split_at(all, parts, s + 1);
+  un.blk = split_at(all, parts, s);
+  un.nb[0] = max(0, min((k0 + 127) / 128, end) - un.blk);
+  un.nb[1] = un.tokens > p.tpt ? end - un.blk : 0;
+  un.part = parts > 1 ? u : -1;
+  return true;
+}
+
+template <int D>
+struct FaRowsCfg {
+  static constexpr int BN = 128;
+  static constexpr int CHUNK_BYTES = 128 * 128;
+  static constexpr int NCHUNK = D / 64;
+  static constexpr int TILE_BYTES = 128 * D * 2;
+  static constexpr int NST = D == 128 ? 4 : 8;
+  static constexpr int KV_OFF = 2 * TILE_BYTES;
+  static constexpr int EPI_OFF = KV_OFF + NST * TILE_BYTES;  // 4 KB per softmax warp
+  static constexpr int CTL_OFF = EPI_OFF + 8 * 4096;
+  // q_full, q_empty, kv_full[NST], kv_empty[NST], s_full[2], p_half[4],
+  // o_full[2], o_empty[2], u_full[], u_empty[], clc, drain
+  static constexpr int NBAR = 2 + 2 * NST + 2 + 4 + 2 + 2 + 2 * kUnitSlots + 2;
+  static constexpr int UNIT_OFF = CTL_OFF + (NBAR * 8 + 15) / 16 * 16;
+  static constexpr int CLC_OFF = UNIT_OFF + kUnitSlots * 48;
+  static constexpr int SMEM_BYTES = CLC_OFF + 32 + 1024;
+  static constexpr int THREADS = 384;
+  static constexpr int REG_SOFTMAX = 200, REG_OTHER = 104, REG_LAUNCH = 168;
+  static constexpr int REG_NEED = 2 * 128 * REG_SOFTMAX + 128 * REG_OTHER;
+  static_assert(REG_NEED <= THREADS * REG_LAUNCH, "register split exceeds the launch allocation");
+  static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
+  static_assert(sizeof(FaUnit) <= 48, "unit slot");
+  static constexpr uint32_t O_COL = 256;
+};
+
+template <typename T> __device__ __forceinline__ uint32_t pack16x2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack16x2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack16x2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+
+template <int D, typename T, typename OutT, bool PAGED>
+__global__ void __launch_bounds__(384, 1)
+    fa_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ FaRowsParams p) {
+  using C = FaRowsCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t *smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t *sQ = smem, *sKV = smem + C::KV_OFF;
+  uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + C::CTL_OFF);
+  uint64_t *q_empty = q_full + 1;
+  uint64_t *kv_full = q_full + 2;
+  uint64_t *kv_empty = kv_full + C::NST;
+  uint64_t *s_full = kv_empty + C::NST;
+  uint64_t *p_half = s_full + 2;   // [t * 2 + half]
+  uint64_t *o_full = p_half + 4;   // [t]
+  uint64_t *o_empty = o_full + 2;  // [t]
+  uint64_t *u_full = o_empty + 2;
+  uint64_t *u_empty = u_full + kUnitSlots;
+  uint64_t *clc_bar = u_empty + kUnitSlots;
+  uint64_t *drain = clc_bar + 1;
+  auto unit_slot = [&](int i) {
+    return reinterpret_cast<FaUnit *>(smem + C::UNIT_OFF + (i % kUnitSlots) * 48);
+  };
+  void *clc_resp = smem + C::CLC_OFF;
+  uint32_t *tmem_base_slot = reinterpret_cast<uint32_t *>(smem + C::CLC_OFF + 16);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_base_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < C::NST; i++) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int t = 0; t < 2; t++) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[2 * t], 4);  // one arrival per softmax warp
+      mbar_init(&p_half[2 * t + 1], 4);
+      mbar_init(&o_full[t], 1);
+      mbar_init(&o_empty[t], 4);
+    }
+    for (int i = 0; i < kUnitSlots; i++) {
+      mbar_init(&u_full[i], 1);
+      mbar_init(&u_empty[i], 10);  // producer, MMA issuer, 8 softmax warps
+    }
+    mbar_init(clc_bar, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_base_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_base_slot;
+
+  // A whole warp's wait; all lanes get the same answer, also when it is given up.
+  auto wait = [&](uint64_t *bar, int phase) {
+    return (bool)__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort_flag));
+  };
+  // The next unit of this CTA, for one warp (lane 0's arrival frees the slot).
+  auto next_unit = [&](int i, FaUnit &un) {
+    if (!wait(&u_full[i % kUnitSlots], i / kUnitSlots)) return false;
+    un = *unit_slot(i);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&u_empty[i % kUnitSlots]);
+    return un.kvh >= 0;
+  };
+
+  if (warp >= 8) {
+    reg_dealloc<C::REG_OTHER>();
+    if (warp == 8) {
+      // ---------------------------------------------------------- producer
+      if (lane == 0) {
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+      }
+      const int box_rows = PAGED ? min(p.rows.page, 128) : 128;
+      const int log_box = 31 - __clz(box_rows);
+      const int log_page = PAGED ? 31 - __clz(p.rows.page) : 0;
+      bool ok = true;
+      int issued = 0, kq = 0;
+      FaUnit un;
+      for (int i = 0; next_unit(i, un); i++) {
+        const int nblk = max(un.nb[0], un.nb[1]);
+        if (nblk == 0) continue;
+        if (kq > 0 && !(ok = wait(q_empty, kq - 1))) break;
+        if (lane == 0) {
+          const int tiles = un.tokens > p.tpt ? 2 : 1;
+          const int bytes = p.group * p.tpt * 128;  // per box
+          mbar_arrive_expect_tx(q_full, tiles * C::NCHUNK * bytes);
+          for (int t = 0; t < tiles; t++)
+            for (int c = 0; c < C::NCHUNK; c++)
+              tma_load_4d(sQ + t * C::TILE_BYTES + c * C::CHUNK_BYTES, &tmQ, q_full, c * 64, 0,
+                          un.q_row + t * p.tpt, un.kvh);
+        }
+        kq++;
+        // Lane l loads box l: rows (l / NCHUNK) * box_rows on, columns (l % NCHUNK) * 64 on.
+        const int pc = lane / C::NCHUNK, cc = lane - pc * C::NCHUNK;
+        const int *trow = PAGED ? p.rows.table + (long long)un.kv_row * p.rows.table_stride : nullptr;
+        auto page_at = [&](int j) {  // page of this lane's box in block j, or 0
+          const int key = (un.blk + j) * C::BN + (pc << log_box);
+          return PAGED && j < nblk && (pc << log_box) < C::BN && key < un.keys ? trow[key >> log_page]
+                                                                               : 0;
+        };
+        int page = page_at(0);
+        for (int j = 0; j < nblk && ok; j++) {
+          const int next_page = page_at(j + 1);
+          const int key0 = (un.blk + j) * C::BN;
+          const int valid = min(C::BN, un.keys - key0);
+          const int boxes = PAGED ? ((valid + box_rows - 1) >> log_box) * C::NCHUNK : C::NCHUNK;
+          if (PAGED && lane < boxes && (unsigned)page >= (unsigned)p.rows.num_pages) {
+            atomicOr(p.rows.err, kErrInput);  // the map reads zeros there
+            page = p.rows.num_pages;
+          }
+          for (int kind = 0; kind < 2; kind++) {
+            const int slot = issued % C::NST, round = issued / C::NST;
+            if (round > 0 && !(ok = wait(&kv_empty[slot], round - 1))) break;
+            if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], boxes * box_rows * 128);
+            __syncwarp();
+            if (lane < boxes) {
+              const CUtensorMap *m = kind ? &tmV : &tmK;
+              uint8_t *dst = sKV + slot * C::TILE_BYTES + cc * C::CHUNK_BYTES + (pc << log_box) * 128;
+              if (PAGED)
+                tma_load_4d(dst, m, &kv_full[slot], cc * 64,
+                            (key0 + (pc << log_box)) & (p.rows.page - 1), un.kvh, page);
+              else
+                tma_load_4d(dst, m, &kv_full[slot], cc * 64, un.kv_row + key0, un.kvh, 0);
+            }
+            issued++;
+          }
+          page = next_page;
+        }
+        if (!ok) break;
+      }
+      if (*abort_flag && lane == 0) {
+        // Abort path: let every armed copy land before the CTA exits.
+        if (kq > 0) mbar_wait_raw(q_full, (kq - 1) & 1, 100000000ull);
+        for (int u = issued - C::NST < 0 ? 0 : issued - C::NST; u < issued; u++)
+          mbar_wait_raw(&kv_full[u % C::NST], (u / C::NST) & 1, 100000000ull);
+      }
+    } else if (warp == 9) {
+      // -------------------------------------------------------- MMA issuer
+      constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      constexpr uint32_t IDESC_S = idesc_mma_f32(128, C::BN, FMT, 0);
+      constexpr uint32_t IDESC_O = idesc_mma_f32(128, D, FMT, 1);
+      const uint32_t sQa = smem_u32(sQ), sKVa = smem_u32(sKV);
+      auto issue_s = [&](int t, int slot) {
+        const uint32_t qa = sQa + t * C::TILE_BYTES, ka = sKVa + slot * C::TILE_BYTES;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk++) {
+          const uint32_t off = (kk >> 2) * C::CHUNK_BYTES + (kk & 3) * 32;
+          if (elect_one())
+            mma_ss(tmem + t * 128, sdesc_sw128(qa + off, 16, 1024),
+                   sdesc_sw128(ka + off, 16, 1024), IDESC_S, kk > 0);
+        }
+        if (elect_one()) mma_commit(&s_full[t]);
+      };
+      bool ok = true;
+      int ring = 0;           // K/V tiles of this CTA's earlier units
+      int kq = 0;             // units with a Q load so far
+      int cp[2] = {0, 0};     // key blocks of tile t so far
+      int cu[2] = {0, 0};     // units of tile t so far
+      FaUnit un;
+      for (int i = 0; ok && next_unit(i, un); i++) {
+        const int nblk = max(un.nb[0], un.nb[1]);
+        if (nblk == 0) continue;
+        ok = wait(q_full, kq) && wait(&kv_full[ring % C::NST], ring / C::NST);
+        kq++;
+        if (!ok) break;
+        tc_fence_after();
+        for (int t = 0; t < 2; t++)
+          if (un.nb[t] > 0) issue_s(t, ring % C::NST);
+        if (elect_one()) mma_commit(&kv_empty[ring % C::NST]);
+        if (nblk == 1 && elect_one()) mma_commit(q_empty);
+        for (int j = 0; j < nblk && ok; j++) {
+          const int uV = ring + 2 * j + 1, sV = uV % C::NST;
+          const int uK = uV + 1, sK = uK % C::NST;
+          const bool more = j + 1 < nblk;
+          if (!(ok = wait(&kv_full[sV], uV / C::NST))) break;
+          const uint32_t va = sKVa + sV * C::TILE_BYTES;
+          const int left = un.keys - (un.blk + j) * C::BN;  // keys of this block that any row sees
+          if (left < C::BN && (left & 15)) {
+            // Rows of V up to the next multiple of 16 take part with P = 0.
+            const int n = (16 - (left & 15)) * 8 * C::NCHUNK;
+            for (int x = lane; x < n; x += 32) {
+              const int c = x / (n / C::NCHUNK), y = x - c * (n / C::NCHUNK);
+              *reinterpret_cast<uint4 *>(sKV + sV * C::TILE_BYTES + c * C::CHUNK_BYTES + left * 128 +
+                                         y * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          bool k_ready = false;
+          for (int t = 0; t < 2 && ok; t++) {
+            if (j < un.nb[t]) {
+              // O_t is overwritten by the unit's first product: the previous
+              // epilogue must have read it.
+              if (j == 0 && cu[t] > 0 && !(ok = wait(&o_empty[t], cu[t] - 1))) break;
+              // 16-key steps that some row of this tile sees.
+              const int seen = un.pos + min(un.tokens, (t + 1) * p.tpt) - (un.blk + j) * C::BN;
+              const int steps = min((min(seen, left) + 15) >> 4, C::BN / 16);
+              for (int half = 0; half < 2; half++) {
+                if (!(ok = wait(&p_half[2 * t + half], cp[t]))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < C::BN / 32; kk++) {
+                  const int ks = half * (C::BN / 32) + kk;
+                  if (ks < steps && elect_one())
+                    mma_ts(tmem + C::O_COL + t * D, tmem + t * 128 + ks * 8,
+                           sdesc_sw128(va + ks * 2048, C::CHUNK_BYTES, 1024), IDESC_O,
+                           (j > 0 || ks > 0) ? 1u : 0u);
+                }
+              }
+              if (!ok) break;
+              cp[t]++;
+              if (j + 1 == un.nb[t]) {
+                if (elect_one()) mma_commit(&o_full[t]);
+                cu[t]++;
+              }
+            }
+            if (j + 1 < un.nb[t]) {
+              if (!k_ready) {
+                if (!(ok = wait(&kv_full[sK], uK / C::NST))) break;
+                tc_fence_after();
+                k_ready = true;
+              }
+              issue_s(t, sK);
+            }
+          }
+          if (!ok) break;
+          if (elect_one()) mma_commit(&kv_empty[sV]);
+          if (more) {
+            if (elect_one()) mma_commit(&kv_empty[sK]);
+            // The unit's last S MMAs are issued: Q may be replaced after them.
+            if (j + 2 == nblk && elect_one()) mma_commit(q_empty);
+          }
+        }
+        ring += 2 * nblk;
+      }
+      // Every MMA this warp issued has completed before TMEM is released.
+      if (elect_one()) mma_commit(drain);
+      mbar_wait_raw(drain, 0, 100000000ull);
+    } else if (warp == 10) {
+      // --------------------------------------------------------- scheduler
+      // A unit is asked for when its slot is free, so a CTA holds one unit
+      // ahead of the one it computes and no more.
+      FaUnit un;
+      int u = blockIdx.x, asked = 0;
+      bool ok = true, have = true;
+      for (int i = 0; ok && have; i++) {
+        if (i >= kUnitSlots && !(ok = wait(&u_empty[i % kUnitSlots], i / kUnitSlots - 1))) break;
+        for (bool first = i == 0;; first = false) {
+          if (!first && p.dynamic) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(clc_bar, 16);
+              clc_try_cancel(clc_resp, clc_bar);
+            }
+            __syncwarp();
+            if (!(ok = wait(clc_bar, asked))) {
+              mbar_wait_raw(clc_bar, asked & 1, 100000000ull);
+              break;
+            }
+            asked++;
+            u = clc_answer(clc_resp);
+            fence_proxy_async_smem();
+            __syncwarp();
+          } else if (!first) {
+            u = u < p.units - (int)gridDim.x ? u + (int)gridDim.x : -1;
+          }
+          have = u >= 0;
+          if (!have || fa_unit<PAGED>(p, u, un)) break;
+        }
+        if (ok && lane == 0) {
+          if (!have) un.kvh = -1;
+          *unit_slot(i) = un;
+          mbar_arrive(&u_full[i % kUnitSlots]);
+        }
+      }
+    } else if (blockIdx.x == 0) {
+      check_requests(p.rows, lane, 32);
+    }
+  } else {
+    reg_alloc<C::REG_SOFTMAX>();
+    // ------------------------------------------------------------- softmax
+    const int t = warp >> 2;           // tile 0 or 1
+    const int row = threadIdx.x & 127;  // row within the tile = TMEM lane
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lane_off + t * 128;
+    const uint32_t tO = tmem + lane_off + C::O_COL + t * D;
+    const float sl2 = p.scale_log2;
+    bool ok = true;
+    int cs = 0, cu = 0;  // key blocks and units of this tile so far
+    for (int i = 0; ok; i++) {
+      // The unit's slot is kept until its epilogue is done, which reads it
+      // again: a row of scores leaves few registers.
+      if (!wait(&u_full[i % kUnitSlots], i / kUnitSlots)) break;
+      const FaUnit &un = *unit_slot(i);
+      if (un.kvh < 0) break;
+      const int nblk = un.nb[t];
+      // Keys of the unit's next block that this row sees; rows that hold no
+      // query are not masked.
+      int valid = 0x3fffffff;
+      {
+        const int tok = row * p.recip >> 16;
+        if (tok < min(un.tokens - t * p.tpt, p.tpt)) valid = un.pos + t * p.tpt + tok + 1 - un.blk * C::BN;
+      }
+      float m_used = -INFINITY;  // log2-domain max the P values are relative to
+      float l = 0.0f;
+      for (int j = 0; j < nblk; j++) {
+        ok = wait(&s_full[t], cs);
+        if (!ok) break;
+        cs++;
+        tc_fence_after();
+        uint32_t sbuf[128];
+#pragma unroll
+        for (int c = 0; c < 4; c++) tmem_ld32(tS + c * 32, sbuf + c * 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; c++) reg_fence32(sbuf + c * 32);
+        const bool masked = __any_sync(0xffffffffu, valid < C::BN);
+        if (masked) {
+#pragma unroll
+          for (int x = 0; x < 128; x++)
+            if (x >= valid) sbuf[x] = 0xff800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 128; x += 2)
+          mx[(x >> 1) & 3] = max3f(mx[(x >> 1) & 3], __uint_as_float(sbuf[x]), __uint_as_float(sbuf[x + 1]));
+        // The max moves only when this block passes it by more than kMaxExp.
+        const float m_new = max3f(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl2;
+        const bool need = m_new > m_used + kMaxExp;
+        if (__any_sync(0xffffffffu, need)) {
+          const float m_tgt = need ? m_new : m_used;
+          const float factor = need ? ex2_approx(m_used - m_tgt) : 1.0f;
+          l *= factor;
+          if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; c++) {
+              uint32_t o[32];
+              tmem_ld32(tO + c * 32, o);
+              tmem_wait_ld();
+              reg_fence32(o);
+#pragma unroll
+              for (int x = 0; x < 32; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
+              tmem_st32(tO + c * 32, o);
+            }
+          }
+          m_used = m_tgt;
+        }
+        // P = 2^(s*scale*log2e - m). A quarter of the pairs of a block without
+        // a mask runs on the FMA pipe; that routine does not reach 0.
+        uint64_t part2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+        const uint64_t sl2x2 = f2_pack(sl2, sl2);
+        const float m_sub = m_used == -INFINITY ? 0.0f : m_used;  // no key so far: all P are 0
+        const uint64_t neg_mx2 = f2_pack(-m_sub, -m_sub);
+        auto write_p = [&](auto poly) {
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const float *v = reinterpret_cast<const float *>(sbuf + c * 32);
+            uint32_t pk[16];
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+              const float2 e = f2_unpack(f2_fma(f2_pack(v[2 * x], v[2 * x + 1]), sl2x2, neg_mx2));
+              uint64_t pp;
+              if (decltype(poly)::value && ((kExp2EmuMask >> x) & 1u))
+                pp = exp2_poly_x2(f2_pack(fmaxf(e.x, -125.0f), fmaxf(e.y, -125.0f)));
+              else
+                pp = f2_pack(ex2_approx(e.x), ex2_approx(e.y));
+              part2[x & 1] = f2_add(part2[x & 1], pp);
+              const float2 pf = f2_unpack(pp);
+              pk[x] = pack16x2<T>(pf.x, pf.y);
+            }
+            tmem_st16(tS + c * 16, pk);
+            if (c == 1 || c == 3) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_half[2 * t + (c == 3 ? 1 : 0)]);
+            }
+          }
+        };
+        if (masked)
+          write_p(std::false_type{});
+        else
+          write_p(std::true_type{});
+        const float2 s0 = f2_unpack(part2[0]), s1 = f2_unpack(part2[1]);
+        l += (s0.x + s0.y) + (s1.x + s1.y);
+        valid -= C::BN;
+      }
+      if (!ok) break;
+      // ------------------------------------------------------- epilogue
+      if (nblk > 0) {
+        ok = wait(&o_full[t], cu);
+        if (!ok) break;
+        cu++;
+        tc_fence_after();
+      }
+      const bool none = m_used == -INFINITY;  // no key
+      const float inv = none ? 0.0f : 1.0f / l;
+      const float lse = none ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
+      const int tok = row * p.recip >> 16, head = row - tok * p.group;
+      const int ntok = min(un.tokens - t * p.tpt, p.tpt);  // tokens of this tile (<= 0: none)
+      const bool live = tok < ntok;
+      const int kvh = un.kvh, q_row = un.q_row + t * p.tpt;  // the tile's first token
+      const int part_at = un.part;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&u_empty[i % kUnitSlots]);
+      if (ntok <= 0) continue;
+      // Column chunk c of this row, normalised; rows without a key are 0
+      // whatever the accumulator holds.
+      auto chunk = [&](int c, float *v) {
+        uint32_t o[32] = {};
+        if (nblk > 0) {
+          tmem_ld32(tO + c * 32, o);
+          tmem_wait_ld();
+          reg_fence32(o);
+          if (c == D / 32 - 1) {
+            // O_t is read out: the next unit's first product may overwrite it.
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty[t]);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 32; x++)
+          v[x] = none ? 0.0f : __uint_as_float(o[x]) * inv;
+      };
+      if (part_at >= 0) {
+        const long long r = (long long)part_at * 256 + t * 128 + row;
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) {
+          float v[32];
+          chunk(c, v);
+          if (live) store_row_chunk<float>(p.part_o + r * D + c * 32, v);
+        }
+        if (live) p.part_lse[r] = lse;
+        continue;
+      }
+      // Stores of whole 128-byte row segments through the warp's staging
+      // block (16-byte pieces XOR-swizzled by row).
+      constexpr int CPR = 128 / (int)sizeof(OutT);  // columns per round
+      uint8_t *stg = smem + C::EPI_OFF + warp * 4096;
+#pragma unroll
+      for (int rnd = 0; rnd < D / CPR; rnd++) {
+#pragma unroll
+        for (int cc = 0; cc < CPR / 32; cc++) {
+          float v[32];
+          chunk(rnd * (CPR / 32) + cc, v);
+          constexpr int PIECES = 32 * (int)sizeof(OutT) / 16;
+          alignas(16) OutT pk[32];
+#pragma unroll
+          for (int x = 0; x < 32; x++) pk[x] = from_f32<OutT>(v[x]);
+#pragma unroll
+          for (int pc = 0; pc < PIECES; pc++)
+            *reinterpret_cast<uint4 *>(stg + lane * 128 + (((cc * PIECES + pc) ^ (lane & 7)) << 4)) =
+                reinterpret_cast<const uint4 *>(pk)[pc];
+        }
+        __syncwarp();
+#pragma unroll
+        for (int it = 0; it < 8; it++) {
+          const int pid = it * 32 + lane, r = pid >> 3, part = pid & 7;
+          const uint4 val = *reinterpret_cast<const uint4 *>(stg + r * 128 + ((part ^ (r & 7)) << 4));
+          const int tr = (warp & 3) * 32 + r;  // row within the tile
+          const int rt = tr * p.recip >> 16;
+          if (rt < ntok)
+            *reinterpret_cast<uint4 *>(static_cast<OutT *>(p.rows.o) +
+                                       (long long)(q_row + rt) * p.rows.os[0] +
+                                       (long long)(kvh * p.group + tr - rt * p.group) * p.rows.os[1] +
+                                       rnd * CPR + part * (16 / (int)sizeof(OutT))) = val;
+        }
+        __syncwarp();
+      }
+      if (p.rows.lse && live)
+        p.rows.lse[(long long)(kvh * p.group + head) * p.rows.tokens + q_row + tok] = lse;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.rows.err, kErrTimeout);
+}
+
+// Joins the parts of units whose keys were split: one warp per (unit, row),
+// o = sum_s w_s o_s with w_s = exp(lse_s) / sum exp(lse), parts in order.
+template <int D, typename OutT, bool PAGED>
+__global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant__ FaRowsParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int first = (int)(w >> 8) * p.nsplit, row = (int)(w & 255);
+  FaUnit un;
+  if (first >= p.units || !fa_unit<PAGED>(p, first, un) || un.part < 0) return;
+  const int t = row >> 7, tr = row & 127;
+  const int rt = tr * p.recip >> 16, tok = t * p.tpt + rt;
+  if (rt >= p.tpt || tok >= un.tokens) return;
+  const int parts = parts_of((un.keys + 127) / 128, p.nsplit);
+  const long long base = (long long)first * 256 + row;
+  float mx = -INFINITY;
+  for (int s = lane; s < parts; s += 32) mx = fmaxf(mx, p.part_lse[base + s * 256]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  constexpr int E = D / 32;
+  float acc[E] = {}, sum = 0.0f;
+  for (int s = 0; s < parts; s++) {
+    const float ls = p.part_lse[base + s * 256];
+    if (ls == -INFINITY) continue;  // saw no key; nothing was written
+    const float wt = expf(ls - mx);
+    sum += wt;
+    const Pack<float, E> v = *reinterpret_cast<const Pack<float, E> *>(
+        p.part_o + (base + s * 256) * D + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[e] = fmaf(wt, v.v[e], acc[e]);
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const int h = un.kvh * p.group + tr - rt * p.group;
+  const int q_row = un.q_row + tok;
+  Pack<OutT, E> out;
+#pragma unroll
+  for (int e = 0; e < E; e++) out.v[e] = from_f32<OutT>(acc[e] * inv);
+  *reinterpret_cast<Pack<OutT, E> *>(static_cast<OutT *>(p.rows.o) + (long long)q_row * p.rows.os[0] +
+                                     (long long)h * p.rows.os[1] + lane * E) = out;
+  if (p.rows.lse && lane == 0)
+    p.rows.lse[(long long)h * p.rows.tokens + q_row] = sum > 0.0f ? mx + logf(sum) : -INFINITY;
+}
+
+}  // namespace llmr

@@ -547,7 +547,7 @@ int llmr_ctx_create(int device, size_t workspace_bytes, void *stream, llmr_ctx *
   if (prop.major != 10) return LLMR_ENODEV;  // sm_100a code only
   llmr_ctx *c = new llmr_ctx();
   c->device = device;
-  c->num_sms = prop.multiProcessorCount;
+  c->num_sms = c->total_sms = prop.multiProcessorCount;
   if (cudaSetDevice(device) != cudaSuccess) { delete c; return LLMR_ECUDA; }
   if (stream) {
     c->stream = static_cast<cudaStream_t>(stream);

@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include "ctx.cuh"
+#include "fa_rows.cuh"
 #include "kattr.cuh"
 #include "paged_kernels.cuh"
 
@@ -80,26 +81,101 @@ const char *bad_paged(const llmr_paged_desc *d) {
   return nullptr;
 }
 
-template <int D, typename T, typename OutT>
-int launch_rows(llmr_ctx *ctx, const RowsParams &p) {
-  const long long warps = (long long)p.tokens * p.H;
-  rows_attention_kernel<D, T, OutT><<<(unsigned)((warps + 7) / 8), 256, 0, ctx->stream>>>(p);
-  return after_launch(ctx, "rows_attention");
+// 16-bit tensor map with 128-byte swizzle; strides in elements, box[0] = 64.
+// The element type only names the zeros outside.
+int make_map16(llmr_ctx *ctx, CUtensorMap *map, const void *base, const long long (&dims)[4],
+               const long long (&strides)[3], int box1, int box2) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return fail(ctx, LLMR_ECUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t d[4], st[3];
+  for (int i = 0; i < 4; i++) d[i] = (cuuint64_t)dims[i];
+  for (int i = 0; i < 3; i++) st[i] = (cuuint64_t)strides[i] * 2;
+  cuuint32_t box[4] = {64, (cuuint32_t)box1, (cuuint32_t)box2, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(base), d, st, box,
+                   estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ctx, LLMR_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return LLMR_OK;
 }
 
-template <int D, typename T>
-int launch_rows_o(llmr_ctx *ctx, llmr_dtype od, const RowsParams &p) {
-  if (od == LLMR_F32) return launch_rows<D, T, float>(ctx, p);
-  if (od == LLMR_F16) return launch_rows<D, T, __half>(ctx, p);
-  return launch_rows<D, T, __nv_bfloat16>(ctx, p);
+// Virtual tiles of a call: every request's tiles and one place over
+// (fa_rows.cuh).
+long long virtual_tiles(long long tokens, long long n, int tu) { return tokens / tu + n; }
+
+// Parts a unit's keys may be cut into: so many that one wave of CTAs covers
+// 148 SMs when there are few units (a long context and few rows).
+int split_parts(long long units) { return units >= 148 ? 1 : (int)(148 / units); }
+
+template <int D, typename T, typename OutT, bool PAGED>
+int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r, int nsplit, float *part) {
+  using C = FaRowsCfg<D>;
+  FaRowsParams p;
+  p.rows = r;
+  p.group = r.H / r.Hk;
+  p.tpt = 128 / p.group;
+  p.recip = (65536 + p.group - 1) / p.group;
+  const long long vt = virtual_tiles(r.tokens, r.n, 2 * p.tpt);
+  const long long units = vt * r.Hk * nsplit;
+  if (units > 0x7fffffffLL) return fail(ctx, LLMR_EINVAL, "problem too large");
+  p.vtiles = (int)vt;
+  p.nsplit = nsplit;
+  p.units = (int)units;
+  // With an SM budget the grid is that small and strides over the units.
+  p.dynamic = units > ctx->num_sms && ctx->num_sms == ctx->total_sms;
+  p.scale_log2 = r.scale * 1.4426950408889634f;
+  p.part_o = part;
+  p.part_lse = part ? part + units * 256 * D : nullptr;
+  CUtensorMap mq, mk, mv;
+  int rc;
+  if ((rc = make_map16(ctx, &mq, r.q, {D, p.group, r.tokens, r.Hk},
+                       {r.qs[1], r.qs[0], r.qs[1] * p.group}, p.group, p.tpt)))
+    return rc;
+  auto kv_map = [&](CUtensorMap *m, const void *base, const long long *st) {
+    if (PAGED)
+      return make_map16(ctx, m, base, {D, r.page, r.Hk, r.num_pages}, {st[1], st[2], st[0]},
+                        r.page < 128 ? r.page : 128, 1);
+    return make_map16(ctx, m, base, {D, r.tokens, r.Hk, 1}, {st[1], st[2], st[1]}, 128, 1);
+  };
+  if ((rc = kv_map(&mk, r.k, r.ks)) || (rc = kv_map(&mv, r.v, r.vs))) return rc;
+  auto kern = fa_rows_kernel<D, T, OutT, PAGED>;
+  CUDA_TRY(ctx, set_smem_once(kern, C::SMEM_BYTES));
+  // setmaxnreg.inc waits until the registers it asks for are free within
+  // the block's launch allocation: never launch a split that cannot fit.
+  int regs = 0;
+  CUDA_TRY(ctx, launch_regs(kern, &regs));
+  if (regs * C::THREADS < C::REG_NEED)
+    return fail(ctx, LLMR_ECUDA, "fa_rows: %d launch registers per thread are too few for the "
+                "register split", regs);
+  const unsigned grid = p.dynamic || units < ctx->num_sms ? (unsigned)units : (unsigned)ctx->num_sms;
+  kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mq, mk, mv, p);
+  if ((rc = after_launch(ctx, "fa_rows"))) return rc;
+  if (nsplit == 1) return LLMR_OK;
+  fa_rows_join_kernel<D, OutT, PAGED><<<(unsigned)(units / nsplit * 32), 256, 0, ctx->stream>>>(p);
+  return after_launch(ctx, "fa_rows_join");
 }
 
-int launch_rows_any(llmr_ctx *ctx, int D, llmr_dtype dt, llmr_dtype od, const RowsParams &p) {
+template <int D, typename T, bool PAGED>
+int launch_fa_rows_o(llmr_ctx *ctx, llmr_dtype od, const RowsParams &r, int nsplit, float *part) {
+  if (od == LLMR_F32) return launch_fa_rows<D, T, float, PAGED>(ctx, r, nsplit, part);
+  if (od == LLMR_F16) return launch_fa_rows<D, T, __half, PAGED>(ctx, r, nsplit, part);
+  return launch_fa_rows<D, T, __nv_bfloat16, PAGED>(ctx, r, nsplit, part);
+}
+
+template <bool PAGED>
+int launch_fa_rows_any(llmr_ctx *ctx, int D, llmr_dtype dt, llmr_dtype od, const RowsParams &r,
+                       int nsplit, float *part) {
   if (D == 128)
-    return dt == LLMR_F16 ? launch_rows_o<128, __half>(ctx, od, p)
-                          : launch_rows_o<128, __nv_bfloat16>(ctx, od, p);
-  return dt == LLMR_F16 ? launch_rows_o<64, __half>(ctx, od, p)
-                        : launch_rows_o<64, __nv_bfloat16>(ctx, od, p);
+    return dt == LLMR_F16 ? launch_fa_rows_o<128, __half, PAGED>(ctx, od, r, nsplit, part)
+                          : launch_fa_rows_o<128, __nv_bfloat16, PAGED>(ctx, od, r, nsplit, part);
+  return dt == LLMR_F16 ? launch_fa_rows_o<64, __half, PAGED>(ctx, od, r, nsplit, part)
+                        : launch_fa_rows_o<64, __nv_bfloat16, PAGED>(ctx, od, r, nsplit, part);
+}
+
+// Key parts of a paged call, from its bounds alone.
+int paged_parts(const llmr_paged_desc *d) {
+  const int tu = 2 * (128 / (int)(d->n_heads / d->n_kv_heads));
+  return split_parts(virtual_tiles(d->total_tokens, d->n_seqs, tu) * d->n_kv_heads);
 }
 
 template <int D, typename InT, typename OutT>
@@ -169,12 +245,15 @@ int llmr_attention_causal(llmr_ctx *ctx, const llmr_causal_desc *d, const int32_
       !strides16({p.os[0], p.os[1]}, size_of(d->out_dtype)))
     return fail(ctx, LLMR_EINVAL, "q, k, v, o and their strides must be 16-byte aligned");
   if (!a4(cu_seqlens) || !a4(lse)) return fail(ctx, LLMR_EINVAL, "cu_seqlens or lse is misaligned");
-  return launch_rows_any(ctx, (int)D, d->dtype, d->out_dtype, p);
+  return launch_fa_rows_any<false>(ctx, (int)D, d->dtype, d->out_dtype, p, 1, nullptr);
 }
 
 size_t llmr_attention_paged_workspace_bytes(const llmr_paged_desc *d) {
   if (!d || bad_paged(d)) return 0;
-  return 16;
+  const int parts = paged_parts(d);
+  const int tu = 2 * (128 / (int)(d->n_heads / d->n_kv_heads));
+  const size_t units = (size_t)virtual_tiles(d->total_tokens, d->n_seqs, tu) * d->n_kv_heads * parts;
+  return parts == 1 ? 16 : units * 256 * (d->head_dim + 1) * sizeof(float);
 }
 
 int llmr_attention_paged(llmr_ctx *ctx, const llmr_paged_desc *d, const int32_t *cu_q,
@@ -229,7 +308,8 @@ int llmr_attention_paged(llmr_ctx *ctx, const llmr_paged_desc *d, const int32_t 
     return fail(ctx, LLMR_EINVAL, "q, the caches, o and their strides must be 16-byte aligned");
   if (!a4(cu_q) || !a4(kv_lens) || !a4(block_table) || !a4(lse))
     return fail(ctx, LLMR_EINVAL, "cu_q, kv_lens, block_table or lse is misaligned");
-  return launch_rows_any(ctx, (int)D, d->dtype, d->out_dtype, p);
+  return launch_fa_rows_any<true>(ctx, (int)D, d->dtype, d->out_dtype, p, paged_parts(d),
+                                  static_cast<float *>(ctx->ws));
 }
 
 int llmr_paged_plan(llmr_ctx *ctx, const llmr_plan_desc *d, const int32_t *ctx_lens,

@@ -342,59 +342,4 @@ __device__ __forceinline__ void check_requests(const RowsParams &p, int first, i
   for (int r = first; r < p.n; r += count) request_rows(p, r, row0, nq, nk);
 }
 
-// One warp per (row, head), keys one after another with the running maximum
-// and sum: right for every shape and slow.
-template <int D, typename T, typename OutT>
-__global__ void __launch_bounds__(256) rows_attention_kernel(const RowsParams p) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  if (blockIdx.x == 0) check_requests(p, threadIdx.x, 256);
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int t = (int)(item / p.H), h = (int)(item - (long long)t * p.H);
-  if (t >= p.tokens || t >= p.cu[p.n] || t < 0) return;
-  int row0, nq, nk;
-  const int r = last_at_most(p.cu, p.n, t);
-  if (!request_rows(p, r, row0, nq, nk) || t < row0 || t >= row0 + nq) return;
-  const int hk = h / (p.H / p.Hk);
-  const int keys = min(nk, nk - nq + t - row0 + 1);
-  float q[E], acc[E];
-  const T *qp = static_cast<const T *>(p.q) + t * p.qs[0] + h * p.qs[1] + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    q[e] = to_f32<T>(qp[e]);
-    acc[e] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (int j = 0; j < keys; j++) {
-    long long pg = 0, row = row0 + j;
-    if (p.paged) {
-      pg = p.table[r * p.table_stride + j / p.page];
-      row = j % p.page;
-      if (pg < 0 || pg >= p.num_pages) {
-        atomicOr(p.err, kErrInput);
-        return;
-      }
-    }
-    const T *kp = static_cast<const T *>(p.k) + pg * p.ks[0] + row * p.ks[1] + hk * p.ks[2] + lane * E;
-    const T *vp = static_cast<const T *>(p.v) + pg * p.vs[0] + row * p.vs[1] + hk * p.vs[2] + lane * E;
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) s = fmaf(q[e], to_f32<T>(kp[e]), s);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= p.scale;
-    const float mn = fmaxf(m, s), f = m == -INFINITY ? 0.0f : expf(m - mn);
-    const float w = mn == -INFINITY ? 0.0f : expf(s - mn);
-    l = l * f + w;
-#pragma unroll
-    for (int e = 0; e < E; e++) acc[e] = acc[e] * f + w * to_f32<T>(vp[e]);
-    m = mn;
-  }
-  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
-  OutT *op = static_cast<OutT *>(p.o) + t * p.os[0] + h * p.os[1] + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e++) op[e] = from_f32<OutT>(acc[e] * inv);
-  if (p.lse && lane == 0) p.lse[(long long)h * p.tokens + t] = m == -INFINITY ? m : m + logf(l);
-}
-
 }  // namespace llmr

@@ -419,10 +419,12 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(uint32_t M, uint32_t N,
                                                      uint32_t b_mn_major) {
   return (1u << 4) | (b_mn_major << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
-// kind::f16 with fp32 accumulation, both operands K-major, A and B of the
-// same format: 0 = fp16, 1 = bf16 (bits 7-9 and 10-12).
-__host__ __device__ constexpr uint32_t idesc_mma_f32(uint32_t M, uint32_t N, uint32_t ab_fmt) {
-  return (1u << 4) | (ab_fmt << 7) | (ab_fmt << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
+// kind::f16 with fp32 accumulation, A and B of the same format: 0 = fp16,
+// 1 = bf16 (bits 7-9 and 10-12); A K-major, B K-major or (bit 16) MN-major.
+__host__ __device__ constexpr uint32_t idesc_mma_f32(uint32_t M, uint32_t N, uint32_t ab_fmt,
+                                                     uint32_t b_mn_major = 0) {
+  return (1u << 4) | (ab_fmt << 7) | (ab_fmt << 10) | (b_mn_major << 16) | ((N >> 3) << 17) |
+         ((M >> 4) << 24);
 }
 
 // ------------------------------------------------------------------ math
@@ -499,6 +501,42 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// The same for bf16.
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// ------------------------------------------------- cluster launch control
+// Asks the hardware for one CTA of this grid that has not started yet, to be
+// run by this CTA instead (clusters of one CTA). The 16-byte answer lands at
+// `resp` and completes 16 transaction bytes on `bar`. Not to be asked again
+// after an answer that cancelled nothing.
+__device__ __forceinline__ void clc_try_cancel(void *resp, uint64_t *bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
+      "[%0], [%1];" ::"r"(smem_u32(resp)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// The answer: the x index of the CTA taken over, or -1 if none was left.
+__device__ __forceinline__ int clc_answer(const void *resp) {
+  uint32_t x = 0, ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t.reg .b32 a, b, c, d;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %1, 1, 0, p;\n\t"
+      "mov.b32 %0, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {a, b, c, d}, r;\n\t"
+      "@p mov.b32 %0, a;\n\t}\n"
+      : "=r"(x), "=r"(ok)
+      : "r"(smem_u32(resp))
+      : "memory");
+  return ok ? (int)x : -1;
 }
 
 }  // namespace llmr

@@ -651,7 +651,7 @@ def test_captured_step_replays(max_q):
     n0 = ctx.launches
     with torch.cuda.graph(g, stream=stream):
         graphed.step(max_q)
-    assert ctx.launches - n0 == 3
+    assert ctx.launches - n0 in (3, 4)   # attention joins its parts in a launch of its own
     with torch.cuda.stream(stream):
         for x, y in zip((graphed.lens, graphed.n_free, graphed.table), state):
             x.copy_(y)
