@@ -145,10 +145,6 @@ struct FaRowsCfg {
   static constexpr uint32_t O_COL = 256;
 };
 
-template <typename T> __device__ __forceinline__ uint32_t pack16x2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack16x2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
-template <> __device__ __forceinline__ uint32_t pack16x2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
-
 template <int D, typename T, typename OutT, bool PAGED>
 __global__ void __launch_bounds__(384, 1)
     fa_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,

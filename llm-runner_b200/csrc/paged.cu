@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include "ctx.cuh"
+#include "fa_decode.cuh"
 #include "fa_rows.cuh"
 #include "kattr.cuh"
 #include "paged_kernels.cuh"
@@ -172,6 +173,55 @@ int launch_fa_rows_any(llmr_ctx *ctx, int D, llmr_dtype dt, llmr_dtype od, const
                         : launch_fa_rows_o<64, __nv_bfloat16, PAGED>(ctx, od, r, nsplit, part);
 }
 
+// Query rows per (request, key/value head) up to which the decode kernel runs.
+constexpr uint32_t kDecodeRows = 32;
+
+uint32_t rows_per_head(const llmr_paged_desc *d) {
+  const uint64_t q = d->max_q_len < d->total_tokens ? d->max_q_len : d->total_tokens;
+  const uint64_t rows = q * (d->n_heads / d->n_kv_heads);
+  return rows > 0xffffffffull ? 0xffffffffu : (uint32_t)rows;
+}
+
+template <int D, int MT, typename T, typename OutT>
+int launch_decode(llmr_ctx *ctx, const RowsParams &r, float *parts) {
+  using C = DecodeCfg<D, MT>;
+  DecodeParams p;
+  p.rows = r;
+  p.group = r.H / r.Hk;
+  p.scale_log2 = r.scale * 1.4426950408889634f;
+  p.parts = parts;
+  p.counters = ctx->d_sync;
+  CUtensorMap mk, mv;
+  int rc;
+  if ((rc = make_map16(ctx, &mk, r.k, {D, r.page, r.Hk, r.num_pages}, {r.ks[1], r.ks[2], r.ks[0]},
+                       r.page < 128 ? r.page : 128, 1)) ||
+      (rc = make_map16(ctx, &mv, r.v, {D, r.page, r.Hk, r.num_pages}, {r.vs[1], r.vs[2], r.vs[0]},
+                       r.page < 128 ? r.page : 128, 1)))
+    return rc;
+  auto kern = fa_decode_kernel<D, MT, T, OutT>;
+  CUDA_TRY(ctx, set_smem_once(kern, C::SMEM_BYTES));
+  int regs = 0;  // as for fa_rows: never launch a split that cannot fit
+  CUDA_TRY(ctx, launch_regs(kern, &regs));
+  if (MT > 1 && regs * C::THREADS < C::REG_NEED)
+    return fail(ctx, LLMR_ECUDA, "fa_decode: %d launch registers per thread are too few for the "
+                "register split", regs);
+  const int grid = ctx->num_sms < kDecodeCtas ? ctx->num_sms : kDecodeCtas;
+  kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mk, mv, p);
+  return after_launch(ctx, "fa_decode");
+}
+
+template <int D, int MT>
+int launch_decode_any(llmr_ctx *ctx, llmr_dtype dt, llmr_dtype od, const RowsParams &r, float *parts) {
+  if (dt == LLMR_F16) {
+    if (od == LLMR_F32) return launch_decode<D, MT, __half, float>(ctx, r, parts);
+    if (od == LLMR_F16) return launch_decode<D, MT, __half, __half>(ctx, r, parts);
+    return launch_decode<D, MT, __half, __nv_bfloat16>(ctx, r, parts);
+  }
+  if (od == LLMR_F32) return launch_decode<D, MT, __nv_bfloat16, float>(ctx, r, parts);
+  if (od == LLMR_F16) return launch_decode<D, MT, __nv_bfloat16, __half>(ctx, r, parts);
+  return launch_decode<D, MT, __nv_bfloat16, __nv_bfloat16>(ctx, r, parts);
+}
+
 // Key parts of a paged call, from its bounds alone.
 int paged_parts(const llmr_paged_desc *d) {
   const int tu = 2 * (128 / (int)(d->n_heads / d->n_kv_heads));
@@ -250,6 +300,10 @@ int llmr_attention_causal(llmr_ctx *ctx, const llmr_causal_desc *d, const int32_
 
 size_t llmr_attention_paged_workspace_bytes(const llmr_paged_desc *d) {
   if (!d || bad_paged(d)) return 0;
+  if (rows_per_head(d) <= kDecodeRows) {
+    const size_t rows = rows_per_head(d) <= 16 ? 16 : 32;
+    return (size_t)kDecodeCtas * 2 * rows * (d->head_dim + 2) * sizeof(float);
+  }
   const int parts = paged_parts(d);
   const int tu = 2 * (128 / (int)(d->n_heads / d->n_kv_heads));
   const size_t units = (size_t)virtual_tiles(d->total_tokens, d->n_seqs, tu) * d->n_kv_heads * parts;
@@ -308,6 +362,14 @@ int llmr_attention_paged(llmr_ctx *ctx, const llmr_paged_desc *d, const int32_t 
     return fail(ctx, LLMR_EINVAL, "q, the caches, o and their strides must be 16-byte aligned");
   if (!a4(cu_q) || !a4(kv_lens) || !a4(block_table) || !a4(lse))
     return fail(ctx, LLMR_EINVAL, "cu_q, kv_lens, block_table or lse is misaligned");
+  if (rows_per_head(d) <= kDecodeRows) {
+    float *parts = static_cast<float *>(ctx->ws);
+    if (rows_per_head(d) <= 16)
+      return D == 128 ? launch_decode_any<128, 1>(ctx, d->dtype, d->out_dtype, p, parts)
+                      : launch_decode_any<64, 1>(ctx, d->dtype, d->out_dtype, p, parts);
+    return D == 128 ? launch_decode_any<128, 2>(ctx, d->dtype, d->out_dtype, p, parts)
+                    : launch_decode_any<64, 2>(ctx, d->dtype, d->out_dtype, p, parts);
+  }
   return launch_fa_rows_any<true>(ctx, (int)D, d->dtype, d->out_dtype, p, paged_parts(d),
                                   static_cast<float *>(ctx->ws));
 }

@@ -304,6 +304,11 @@ __global__ void __launch_bounds__(256) paged_prologue_kernel(const PagedRopePara
 }
 
 // ---------------------------------------------------------------- attention
+// Two fp32 values rounded to a word of T; lo lands in the low half.
+template <typename T> __device__ __forceinline__ uint32_t pack16x2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack16x2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack16x2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+
 // What both attention operators are given. paged: K and V rows are found
 // through the block table; otherwise they are packed like the queries.
 struct RowsParams {

@@ -562,56 +562,125 @@ def out_project(ctx: Context, o, hidden, w0, w1=None, *, batch: int, seq_len: in
 
 # ------------------------------------------------- causal prompts and a paged cache
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise LlmrError(EINVAL, what)
+# The checks below run before every call of a serving step: messages are built
+# only for a refusal, and a tensor's shape, strides and type are read once.
+
+def _refuse(what: str):
+    raise LlmrError(EINVAL, what)
 
 
-def _stride(t, dim: int) -> int:
-    """The element stride of a dimension; 0 (the dense default) where it is never stepped."""
-    if t.shape[dim] <= 1:
+def _step(size: int, stride: int) -> int:
+    """An element stride; 0 (the dense default) for a dimension that is never stepped."""
+    if size <= 1:
         return 0
-    _need(t.stride(dim) > 0, "a broadcast (stride 0) dimension is not supported")
-    return t.stride(dim)
+    if stride <= 0:
+        _refuse("a broadcast (stride 0) dimension is not supported")
+    return stride
 
 
-def _rows(t, name: str, dtypes, tokens: int, heads: int, dim: int):
-    """`t` as [tokens, heads, dim] with dense elements (an output may be [tokens, heads*dim])."""
-    _need(t.dim() in (2, 3), f"{name} must be [tokens, heads, head_dim]")
+class _Types(dict):
+    """torch dtype -> LLMR_F32 / F16 / BF16 / "int32"; torch is imported on the first use."""
+
+    def __missing__(self, dtype):
+        import torch
+        self.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16,
+                     torch.int32: "int32"})
+        return self.setdefault(dtype, None)
+
+
+_TYPES = _Types()
+
+
+def _code(t, name: str) -> int:
+    """LLMR_F32 / F16 / BF16 of a tensor."""
+    code = _TYPES[t.dtype]
+    if code is None or code == "int32":
+        _refuse(f"{name}: unsupported dtype {t.dtype}")
+    return code
+
+
+def _rows(t, name: str, code, tokens: int, heads: int, dim: int, device: int):
+    """(row stride, head stride) of a [tokens, heads, dim] tensor with dense elements."""
+    if t.shape != (tokens, heads, dim):
+        _refuse(f"{name} is {tuple(t.shape)}, not {(tokens, heads, dim)}")
+    st = t.stride()
+    if st[2] != 1 and tokens:
+        _refuse(f"{name}: elements of a row must be dense")
+    if code is not None and _code(t, name) != code:
+        _refuse(f"{name}: dtype {t.dtype} differs")
+    _place(t, name, device)
+    return _step(tokens, st[0]), _step(heads, st[1])
+
+
+def _out_rows(t, name: str, tokens: int, heads: int, dim: int, device: int):
+    """_rows for an output, which may also be [tokens, heads * dim]."""
     if t.dim() == 2:
-        _need(t.shape[1] == heads * dim and (t.shape[0] == 0 or t.stride(1) == 1),
-              f"{name} must be [{tokens}, {heads * dim}]")
-        t = t.unflatten(1, (heads, dim))
-    _need(tuple(t.shape) == (tokens, heads, dim),
-          f"{name} is {tuple(t.shape)}, not {(tokens, heads, dim)}")
-    _need(t.numel() == 0 or t.stride(2) == 1, f"{name}: elements of a row must be dense")
-    _need(_dtype_code(t) in dtypes, f"{name}: unsupported dtype {t.dtype}")
-    return t
+        if t.shape != (tokens, heads * dim) or (tokens and t.stride(1) != 1):
+            _refuse(f"{name} must be [{tokens}, {heads * dim}] or [{tokens}, {heads}, {dim}], dense rows")
+        _place(t, name, device)
+        return _step(tokens, t.stride(0)), 0
+    return _rows(t, name, None, tokens, heads, dim, device)
 
 
-def _vector(t, name: str, length: int, dtype: str = "int32") -> None:
-    _need(t.dim() == 1 and t.shape[0] == length and (length <= 1 or t.stride(0) == 1),
-          f"{name} must be a dense vector of {length}")
-    _need(str(t.dtype) == f"torch.{dtype}", f"{name} must be {dtype}")
+def _place(t, name: str, device: int) -> None:
+    if t.get_device() != device:  # -1 on the host
+        _refuse(f"{name} must be on cuda:{device}")
 
 
-def _on_device(ctx: "Context", **tensors) -> None:
-    for name, t in tensors.items():
-        _need(t is None or (t.device.type == "cuda" and t.device.index == ctx.device),
-              f"{name} must be on cuda:{ctx.device}")
+def _vector(t, name: str, length: int, device: int, kind="int32") -> None:
+    if t.shape != (length,) or (length > 1 and t.stride(0) != 1):
+        _refuse(f"{name} must be a dense vector of {length}")
+    if _TYPES[t.dtype] != kind:
+        _refuse(f"{name} must be {'fp32' if kind == F32 else kind}, not {t.dtype}")
+    _place(t, name, device)
 
 
-def _lse(lse, heads: int, tokens: int) -> None:
-    if lse is not None:
-        _need(tuple(lse.shape) == (heads, tokens) and lse.is_contiguous()
-              and str(lse.dtype) == "torch.float32", f"lse must be fp32 [{heads}, {tokens}], dense")
+def _lse(lse, heads: int, tokens: int, device: int) -> None:
+    if lse is None:
+        return
+    if lse.shape != (heads, tokens) or not lse.is_contiguous() or _TYPES[lse.dtype] != F32:
+        _refuse(f"lse must be fp32 [{heads}, {tokens}], dense")
+    _place(lse, "lse", device)
 
 
-def _heads(q, name_k: str, kv_heads: int) -> None:
-    _need(q.dim() == 3, "q must be [tokens, heads, head_dim]")
-    _need(q.shape[2] in (64, 128), "head_dim must be 64 or 128")
-    _need(kv_heads > 0 and q.shape[1] > 0 and q.shape[1] % kv_heads == 0,
-          f"q's {q.shape[1]} heads are no multiple of {name_k}'s {kv_heads}")
+def _query(q, name_k: str, kv_heads: int):
+    """(tokens, heads, head_dim, dtype code) of q."""
+    if q.dim() != 3:
+        _refuse("q must be [tokens, heads, head_dim]")
+    t, h, dim = q.shape
+    if dim not in (64, 128):
+        _refuse("head_dim must be 64 or 128")
+    if kv_heads < 1 or h < 1 or h % kv_heads:
+        _refuse(f"q's {h} heads are no multiple of {name_k}'s {kv_heads}")
+    code = _code(q, "q")
+    if code == F32:
+        _refuse(f"q: unsupported dtype {q.dtype}")
+    return t, h, dim, code
+
+
+def _cache(t, name: str, code: int, shape, device: int):
+    """(page, row, head) strides of a cache."""
+    if t.shape != shape or not t.numel():
+        _refuse(f"{name} is {tuple(t.shape)}, not {tuple(shape)}")
+    st = t.stride()
+    if st[3] != 1:
+        _refuse(f"{name}: elements of a row must be dense")
+    if _code(t, name) != code:
+        _refuse(f"{name}: dtype {t.dtype} differs")
+    _place(t, name, device)
+    return _step(shape[0], st[0]), _step(shape[1], st[1]), _step(shape[2], st[2])
+
+
+def _table(block_table, n: int, device: int):
+    """(columns, row stride) of a block table."""
+    if block_table.dim() != 2 or _TYPES[block_table.dtype] != "int32":
+        _refuse("block_table must be int32 [n_seqs, max_pages]")
+    rows, cols = block_table.shape
+    st = block_table.stride()
+    if rows != n or cols < 1 or (cols > 1 and st[1] != 1):
+        _refuse(f"block_table must be [{n}, max_pages] with dense rows")
+    _place(block_table, "block_table", device)
+    return cols, _step(rows, st[0])
 
 
 def attention_causal(ctx: Context, q, k, v, o, cu_seqlens, *, scale: float, lse=None) -> None:
@@ -622,43 +691,33 @@ def attention_causal(ctx: Context, q, k, v, o, cu_seqlens, *, scale: float, lse=
     fp32). Sequence i is rows cu_seqlens[i]:cu_seqlens[i+1] (int32, on the
     device); rows behind the last keep what o and lse hold. lse: fp32
     [heads, tokens]."""
-    _need(k.dim() == 3, "k must be [tokens, kv_heads, head_dim]")
-    _heads(q, "k", k.shape[1])
-    t, h, dim = q.shape
-    hk = k.shape[1]
-    q = _rows(q, "q", (F16, BF16), t, h, dim)
-    k = _rows(k, "k", (_dtype_code(q),), t, hk, dim)
-    v = _rows(v, "v", (_dtype_code(q),), t, hk, dim)
-    o = _rows(o, "o", (F32, F16, BF16), t, h, dim)
-    _need(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "cu_seqlens must be [n_seqs + 1]")
-    _vector(cu_seqlens, "cu_seqlens", cu_seqlens.shape[0])
-    _lse(lse, h, t)
-    _on_device(ctx, q=q, k=k, v=v, o=o, cu_seqlens=cu_seqlens, lse=lse)
-    d = CausalDesc(n_seqs=cu_seqlens.shape[0] - 1, total_tokens=t, n_heads=h, n_kv_heads=hk,
-                   head_dim=dim, dtype=_dtype_code(q), out_dtype=_dtype_code(o), scale=scale,
-                   q_row_stride=_stride(q, 0), q_head_stride=_stride(q, 1),
-                   k_row_stride=_stride(k, 0), k_head_stride=_stride(k, 1),
-                   v_row_stride=_stride(v, 0), v_head_stride=_stride(v, 1),
-                   o_row_stride=_stride(o, 0), o_head_stride=_stride(o, 1))
-    ctx.check(lib.llmr_attention_causal(ctx.handle, ctypes.byref(d), _ptr(cu_seqlens), _ptr(q),
-                                        _ptr(k), _ptr(v), _ptr(o), _ptr(lse)))
-
-
-def _cache(t, name: str, dtype: int, shape=None):
-    _need(t.dim() == 4, f"{name} must be [pages, page_size, kv_heads, head_dim]")
-    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name} is {tuple(t.shape)}, not {shape}")
-    _need(t.numel() > 0 and t.stride(3) == 1, f"{name}: elements of a row must be dense")
-    _need(_dtype_code(t) == dtype, f"{name}: dtype {t.dtype} differs")
+    if k.dim() != 3:
+        _refuse("k must be [tokens, kv_heads, head_dim]")
+    hk, dev = k.shape[1], ctx.device
+    t, h, dim, code = _query(q, "k", hk)
+    qr, qh = _rows(q, "q", None, t, h, dim, dev)
+    kr, kh = _rows(k, "k", code, t, hk, dim, dev)
+    vr, vh = _rows(v, "v", code, t, hk, dim, dev)
+    orow, oh = _out_rows(o, "o", t, h, dim, dev)
+    n = cu_seqlens.numel() - 1
+    if n < 0:
+        _refuse("cu_seqlens must be [n_seqs + 1]")
+    _vector(cu_seqlens, "cu_seqlens", n + 1, dev)
+    _lse(lse, h, t, dev)
+    d = CausalDesc(n, t, h, hk, dim, code, _code(o, "o"), scale, qr, kr, vr, orow, qh, kh, vh, oh)
+    ctx.check(lib.llmr_attention_causal(ctx.handle, ctypes.byref(d), cu_seqlens.data_ptr(),
+                                        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                        _ptr(lse)))
 
 
 def attention_paged_workspace_bytes(*, n_seqs: int, total_tokens: int, max_q_len: int,
                                     n_heads: int, n_kv_heads: int, head_dim: int) -> int:
     """Workspace of attention_paged for these bounds (ctx.reserve)."""
-    d = PagedDesc(n_seqs=n_seqs, total_tokens=total_tokens, max_q_len=max_q_len, n_heads=n_heads,
-                  n_kv_heads=n_kv_heads, head_dim=head_dim, dtype=F16, out_dtype=F16, scale=1.0,
-                  page_size=16, num_pages=1, max_pages=1)
+    d = PagedDesc(n_seqs, total_tokens, max_q_len, n_heads, n_kv_heads, head_dim, F16, F16, 1.0,
+                  16, 1, 1)
     n = int(lib.llmr_attention_paged_workspace_bytes(ctypes.byref(d)))
-    _need(n > 0, "head_dim must be 64 or 128 and n_heads a multiple of n_kv_heads")
+    if n == 0:
+        _refuse("head_dim must be 64 or 128 and n_heads a multiple of n_kv_heads")
     return n
 
 
@@ -672,42 +731,28 @@ def attention_paged(ctx: Context, q, k_cache, v_cache, o, cu_q, kv_lens, block_t
     block_table[i, :]. cu_q, kv_lens, block_table are int32 on the device.
     max_q_len: at least the new tokens of any one request. Needs
     attention_paged_workspace_bytes of workspace."""
-    _need(k_cache.dim() == 4, "k_cache must be [pages, page_size, kv_heads, head_dim]")
-    _heads(q, "k_cache", k_cache.shape[2])
-    t, h, dim = q.shape
-    q = _rows(q, "q", (F16, BF16), t, h, dim)
+    if k_cache.dim() != 4:
+        _refuse("k_cache must be [pages, page_size, kv_heads, head_dim]")
     pages, page, hk, _ = k_cache.shape
-    _cache(k_cache, "k_cache", _dtype_code(q), (pages, page, hk, dim))
-    _cache(v_cache, "v_cache", _dtype_code(q), (pages, page, hk, dim))
-    o = _rows(o, "o", (F32, F16, BF16), t, h, dim)
-    _need(kv_lens.dim() == 1, "kv_lens must be [n_seqs]")
-    n = kv_lens.shape[0]
-    _vector(kv_lens, "kv_lens", n)
-    _vector(cu_q, "cu_q", n + 1)
-    _table(block_table, n)
-    _lse(lse, h, t)
-    _need(max_q_len >= 0, "max_q_len must not be negative")
-    _on_device(ctx, q=q, k_cache=k_cache, v_cache=v_cache, o=o, cu_q=cu_q, kv_lens=kv_lens,
-               block_table=block_table, lse=lse)
-    d = PagedDesc(n_seqs=n, total_tokens=t, max_q_len=min(max_q_len, t), n_heads=h, n_kv_heads=hk,
-                  head_dim=dim, dtype=_dtype_code(q), out_dtype=_dtype_code(o), scale=scale,
-                  page_size=page, num_pages=pages, max_pages=block_table.shape[1],
-                  table_stride=_stride(block_table, 0),
-                  q_row_stride=_stride(q, 0), q_head_stride=_stride(q, 1),
-                  o_row_stride=_stride(o, 0), o_head_stride=_stride(o, 1),
-                  k_page_stride=_stride(k_cache, 0), k_row_stride=_stride(k_cache, 1),
-                  k_head_stride=_stride(k_cache, 2), v_page_stride=_stride(v_cache, 0),
-                  v_row_stride=_stride(v_cache, 1), v_head_stride=_stride(v_cache, 2))
-    ctx.check(lib.llmr_attention_paged(ctx.handle, ctypes.byref(d), _ptr(cu_q), _ptr(kv_lens),
-                                       _ptr(block_table), _ptr(q), _ptr(k_cache), _ptr(v_cache),
-                                       _ptr(o), _ptr(lse)))
-
-
-def _table(block_table, n: int) -> None:
-    _need(block_table.dim() == 2 and block_table.shape[0] == n and block_table.shape[1] >= 1
-          and (block_table.shape[1] == 1 or block_table.stride(1) == 1)
-          and str(block_table.dtype) == "torch.int32",
-          f"block_table must be int32 [{n}, max_pages] with dense rows")
+    dev = ctx.device
+    t, h, dim, code = _query(q, "k_cache", hk)
+    qr, qh = _rows(q, "q", None, t, h, dim, dev)
+    kc = _cache(k_cache, "k_cache", code, (pages, page, hk, dim), dev)
+    vc = _cache(v_cache, "v_cache", code, (pages, page, hk, dim), dev)
+    orow, oh = _out_rows(o, "o", t, h, dim, dev)
+    n = kv_lens.numel()
+    _vector(kv_lens, "kv_lens", n, dev)
+    _vector(cu_q, "cu_q", n + 1, dev)
+    cols, table_step = _table(block_table, n, dev)
+    _lse(lse, h, t, dev)
+    if max_q_len < 0:
+        _refuse("max_q_len must not be negative")
+    d = PagedDesc(n, t, min(max_q_len, t), h, hk, dim, code, _code(o, "o"), scale, page, pages, cols,
+                  table_step, qr, orow, qh, oh, *kc, *vc)
+    ctx.check(lib.llmr_attention_paged(ctx.handle, ctypes.byref(d), cu_q.data_ptr(),
+                                       kv_lens.data_ptr(), block_table.data_ptr(), q.data_ptr(),
+                                       k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
+                                       _ptr(lse)))
 
 
 def paged_plan(ctx: Context, ctx_lens, new_lens, free_pages, n_free, block_table, cu_q, kv_lens,
@@ -720,27 +765,25 @@ def paged_plan(ctx: Context, ctx_lens, new_lens, free_pages, n_free, block_table
     (0 and -1 behind the last token), and n_free_out [1]. kv_lens may be
     ctx_lens and n_free_out may be n_free. All tensors int32 on the device.
     num_pages: pages of the cache, against which page numbers are checked."""
-    _need(ctx_lens.dim() == 1 and free_pages.dim() == 1 and positions.dim() == 1,
-          "ctx_lens, free_pages and positions must be vectors")
-    n = ctx_lens.shape[0]
-    for name, t, length in (("ctx_lens", ctx_lens, n), ("new_lens", new_lens, n),
-                            ("free_pages", free_pages, free_pages.shape[0]),
-                            ("n_free", n_free, 1), ("cu_q", cu_q, n + 1), ("kv_lens", kv_lens, n),
-                            ("positions", positions, positions.shape[0]),
-                            ("slots", slots, positions.shape[0]), ("n_free_out", n_free_out, 1)):
-        _vector(t, name, length)
-    _table(block_table, n)
-    _need(page_size > 0, "page_size must be positive")
-    _on_device(ctx, ctx_lens=ctx_lens, new_lens=new_lens, free_pages=free_pages, n_free=n_free,
-               block_table=block_table, cu_q=cu_q, kv_lens=kv_lens, positions=positions,
-               slots=slots, n_free_out=n_free_out)
-    d = PlanDesc(n_seqs=n, max_tokens=positions.shape[0], page_size=page_size,
-                 num_pages=0x7fffffff // page_size if num_pages is None else num_pages,
-                 free_capacity=free_pages.shape[0], max_pages=block_table.shape[1],
-                 table_stride=_stride(block_table, 0))
-    ctx.check(lib.llmr_paged_plan(ctx.handle, ctypes.byref(d), _ptr(ctx_lens), _ptr(new_lens),
-                                  _ptr(free_pages), _ptr(n_free), _ptr(block_table), _ptr(cu_q),
-                                  _ptr(kv_lens), _ptr(positions), _ptr(slots), _ptr(n_free_out)))
+    n, room, cap, dev = ctx_lens.numel(), positions.numel(), free_pages.numel(), ctx.device
+    _vector(ctx_lens, "ctx_lens", n, dev)
+    _vector(new_lens, "new_lens", n, dev)
+    _vector(free_pages, "free_pages", cap, dev)
+    _vector(n_free, "n_free", 1, dev)
+    _vector(cu_q, "cu_q", n + 1, dev)
+    _vector(kv_lens, "kv_lens", n, dev)
+    _vector(positions, "positions", room, dev)
+    _vector(slots, "slots", room, dev)
+    _vector(n_free_out, "n_free_out", 1, dev)
+    cols, table_step = _table(block_table, n, dev)
+    if page_size < 1:
+        _refuse("page_size must be positive")
+    d = PlanDesc(n, room, page_size, 0x7fffffff // page_size if num_pages is None else num_pages,
+                 cap, cols, table_step)
+    ctx.check(lib.llmr_paged_plan(ctx.handle, ctypes.byref(d), ctx_lens.data_ptr(),
+                                  new_lens.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(),
+                                  block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(),
+                                  positions.data_ptr(), slots.data_ptr(), n_free_out.data_ptr()))
 
 
 def paged_prologue(ctx: Context, q, k, v, q_out, k_cache, v_cache, positions, slots, *,
@@ -754,57 +797,57 @@ def paged_prologue(ctx: Context, q, k, v, q_out, k_cache, v_cache, positions, sl
     None = no norm of that tensor. cos / sin: fp32 [rows, D/2], indexed by
     positions [tokens]; None = no rotation. half: pairs (i, i + D/2) instead
     of (2i, 2i+1). q and q_out may both be None (K and V alone)."""
-    _need(k.dim() == 3 and k_cache.dim() == 4, "k must be [tokens, kv_heads, head_dim]")
+    if k.dim() != 3 or k_cache.dim() != 4:
+        _refuse("k must be [tokens, kv_heads, head_dim] and k_cache [pages, page_size, kv_heads, head_dim]")
     t, hk, dim = k.shape
-    code = _dtype_code(k_cache)
-    _need(code in (F16, BF16), "the caches must be fp16 or bf16")
+    dev, code, code_in = ctx.device, _code(k_cache, "k_cache"), _code(k, "k")
+    if code == F32:
+        _refuse("the caches must be fp16 or bf16")
     pages, page = k_cache.shape[:2]
-    _cache(k_cache, "k_cache", code, (pages, page, hk, dim))
-    _cache(v_cache, "v_cache", code, (pages, page, hk, dim))
-    k = _rows(k, "k", (F32, F16, BF16), t, hk, dim)
-    v = _rows(v, "v", (_dtype_code(k),), t, hk, dim)
-    _need((q is None) == (q_out is None), "q and q_out go together")
-    h = hk
+    kc = _cache(k_cache, "k_cache", code, (pages, page, hk, dim), dev)
+    vc = _cache(v_cache, "v_cache", code, (pages, page, hk, dim), dev)
+    kr, kh = _rows(k, "k", None, t, hk, dim, dev)
+    vr, vh = _rows(v, "v", code_in, t, hk, dim, dev)
+    if (q is None) != (q_out is None):
+        _refuse("q and q_out go together")
+    h, qr, qh, orow, oh = hk, 0, 0, 0, 0
     if q is not None:
-        _heads(q, "k", hk)
+        if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % hk:
+            _refuse(f"q must be [tokens, heads, head_dim], its heads a multiple of k's {hk}")
         h = q.shape[1]
-        q = _rows(q, "q", (_dtype_code(k),), t, h, dim)
-        q_out = _rows(q_out, "q_out", (code,), t, h, dim)
-    _vector(slots, "slots", t)
-    _need((cos is None) == (sin is None), "cos and sin go together")
-    rows = 0
+        qr, qh = _rows(q, "q", code_in, t, h, dim, dev)
+        orow, oh = _rows(q_out, "q_out", code, t, h, dim, dev)
+    elif q_gain is not None:
+        _refuse("q_gain needs q")
+    _vector(slots, "slots", t, dev)
+    if (cos is None) != (sin is None):
+        _refuse("cos and sin go together")
+    rows = flags = 0
     if cos is not None:
         rows = cos.shape[0]
-        for name, x in (("cos", cos), ("sin", sin)):
-            _need(tuple(x.shape) == (rows, dim // 2) and x.is_contiguous()
-                  and str(x.dtype) == "torch.float32", f"{name} must be fp32 [rows, {dim // 2}]")
-        _need(positions is not None, "cos and sin need positions")
-    _need(cos is not None or not half, "half needs cos and sin")
+        for x in (cos, sin):
+            if x.shape != (rows, dim // 2) or not x.is_contiguous() or _TYPES[x.dtype] != F32:
+                _refuse(f"cos and sin must be fp32 [rows, {dim // 2}]")
+            _place(x, "cos and sin", dev)
+        if positions is None:
+            _refuse("cos and sin need positions")
+        flags = (ROPE | ROPE_HALF) if half else ROPE
+    elif half:
+        _refuse("half needs cos and sin")
     if positions is not None:
-        _vector(positions, "positions", t)
-    for name, g in (("q_gain", q_gain), ("k_gain", k_gain)):
-        if g is not None:
-            _vector(g, name, dim, "float32")
-    _need(q is not None or q_gain is None, "q_gain needs q")
-    _on_device(ctx, q=q, k=k, v=v, q_out=q_out, k_cache=k_cache, v_cache=v_cache,
-               positions=positions, slots=slots, q_gain=q_gain, k_gain=k_gain, cos=cos, sin=sin)
-    d = PagedPrologueDesc(
-        total_tokens=t, n_heads=h, n_kv_heads=hk, head_dim=dim, in_dtype=_dtype_code(k), dtype=code,
-        flags=((NORM_Q if q_gain is not None else 0) | (NORM_K if k_gain is not None else 0)
-               | (ROPE if cos is not None else 0) | (ROPE_HALF if half else 0)),
-        eps=eps, page_size=page, num_pages=pages, rope_rows=rows,
-        k_row_stride=_stride(k, 0), k_head_stride=_stride(k, 1), v_row_stride=_stride(v, 0),
-        v_head_stride=_stride(v, 1), k_page_stride=_stride(k_cache, 0),
-        k_cache_row_stride=_stride(k_cache, 1), k_cache_head_stride=_stride(k_cache, 2),
-        v_page_stride=_stride(v_cache, 0), v_cache_row_stride=_stride(v_cache, 1),
-        v_cache_head_stride=_stride(v_cache, 2))
-    if q is not None:
-        d.q_row_stride, d.q_head_stride = _stride(q, 0), _stride(q, 1)
-        d.q_out_row_stride, d.q_out_head_stride = _stride(q_out, 0), _stride(q_out, 1)
-    ctx.check(lib.llmr_paged_prologue(ctx.handle, ctypes.byref(d), _ptr(positions), _ptr(slots),
-                                      _ptr(q), _ptr(k), _ptr(v), _ptr(q_gain), _ptr(k_gain),
-                                      _ptr(cos), _ptr(sin), _ptr(q_out), _ptr(k_cache),
-                                      _ptr(v_cache)))
+        _vector(positions, "positions", t, dev)
+    if q_gain is not None:
+        _vector(q_gain, "q_gain", dim, dev, F32)
+        flags |= NORM_Q
+    if k_gain is not None:
+        _vector(k_gain, "k_gain", dim, dev, F32)
+        flags |= NORM_K
+    d = PagedPrologueDesc(t, h, hk, dim, code_in, code, flags, eps, page, pages, rows, qr, kr, vr,
+                          orow, qh, kh, vh, oh, *kc, *vc)
+    ctx.check(lib.llmr_paged_prologue(ctx.handle, ctypes.byref(d), _ptr(positions),
+                                      slots.data_ptr(), _ptr(q), k.data_ptr(), v.data_ptr(),
+                                      _ptr(q_gain), _ptr(k_gain), _ptr(cos), _ptr(sin),
+                                      _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr()))
 
 
 # --------------------------------------------------------------------- peer buffers

@@ -58,8 +58,12 @@ def test_null_context_is_refused():
 
 
 class NoDevice:
-    """Stands for a context; the library must not be reached with it."""
-    device, handle = 0, None
+    """Stands for a context; the library must not be reached with it. -1 is
+    where torch says that host tensors are."""
+    handle = None
+
+    def __init__(self, device=-1):
+        self.device = device
 
     def check(self, rc):
         raise AssertionError("a refused call reached the library")
@@ -93,19 +97,19 @@ def refused(f, word=""):
 ])
 def test_causal_refuses(change, word):
     a = {**dict(q=z(5, 4, 64), k=z(5, 2, 64), v=z(5, 2, 64), o=z(5, 4, 64), cu=i32(2), lse=None), **change}
-    refused(lambda: L.attention_causal(NoDevice(), a["q"], a["k"], a["v"], a["o"], a["cu"], scale=0.1,
+    refused(lambda: L.attention_causal(NoDevice(0 if not change else -1), a["q"], a["k"], a["v"], a["o"], a["cu"], scale=0.1,
                                        lse=a["lse"]), word)
 
 
 def test_broadcast_inputs_are_refused():
-    k = z(5, 1, 64).expand(5, 2, 64)
-    refused(lambda: L._stride(k, 1), "broadcast")
-    assert L._stride(z(5, 1, 64), 1) == 0 and L._stride(z(5, 2, 64), 0) == 128
+    refused(lambda: L._step(2, z(5, 1, 64).expand(5, 2, 64).stride(1)), "broadcast")
+    assert L._step(1, 0) == 0 and L._step(5, 128) == 128
 
 
 @pytest.mark.parametrize("change,word", [
     (dict(kc=z(3, 16, 64)), "k_cache"), (dict(vc=z(3, 32, 2, 64)), "v_cache"),
     (dict(kc=z(3, 16, 2, 64, dtype=torch.float16)), "dtype"), (dict(kc=z(3, 16, 3, 64)), "multiple"),
+    (dict(vc=z(3, 16, 2, 64, dtype=torch.float16)), "dtype"),
     (dict(cu=i32(4)), "cu_q"), (dict(kv=torch.zeros(2, dtype=torch.int64)), "kv_lens"),
     (dict(table=i32(3, 4)), "block_table"), (dict(table=i32(2, 0)), "block_table"),
     (dict(table=i32(2, 8)[:, ::2]), "block_table"), (dict(max_q=-1), "max_q_len"), (dict(), "cuda:0"),
@@ -113,7 +117,7 @@ def test_broadcast_inputs_are_refused():
 def test_paged_refuses(change, word):
     a = {**dict(q=z(5, 4, 64), kc=z(3, 16, 2, 64), vc=z(3, 16, 2, 64), o=z(5, 4, 64), cu=i32(3), kv=i32(2),
                 table=i32(2, 4), max_q=5), **change}
-    refused(lambda: L.attention_paged(NoDevice(), a["q"], a["kc"], a["vc"], a["o"], a["cu"], a["kv"],
+    refused(lambda: L.attention_paged(NoDevice(0 if not change else -1), a["q"], a["kc"], a["vc"], a["o"], a["cu"], a["kv"],
                                       a["table"], scale=0.1, max_q_len=a["max_q"]), word)
 
 
@@ -126,7 +130,7 @@ def test_paged_refuses(change, word):
 def test_plan_refuses(change, word):
     a = {**dict(ctx=i32(3), new=i32(3), free=i32(5), n_free=i32(1), table=i32(3, 4), cu=i32(4), kv=i32(3),
                 pos=i32(9), slots=i32(9), out=i32(1), page=16), **change}
-    refused(lambda: L.paged_plan(NoDevice(), a["ctx"], a["new"], a["free"], a["n_free"], a["table"], a["cu"],
+    refused(lambda: L.paged_plan(NoDevice(0 if not change else -1), a["ctx"], a["new"], a["free"], a["n_free"], a["table"], a["cu"],
                                  a["kv"], a["pos"], a["slots"], a["out"], page_size=a["page"]), word)
 
 
@@ -145,6 +149,6 @@ def test_prologue_refuses(change, word):
     a = {**dict(q=z(5, 4, 64), k=z(5, 2, 64), v=z(5, 2, 64), q_out=z(5, 4, 64), kc=z(3, 16, 2, 64),
                 vc=z(3, 16, 2, 64), pos=i32(5), slots=i32(5), cos=z(9, 32, dtype=F), sin=z(9, 32, dtype=F),
                 q_gain=z(64, dtype=F), k_gain=None), **change}
-    refused(lambda: L.paged_prologue(NoDevice(), a["q"], a["k"], a["v"], a["q_out"], a["kc"], a["vc"], a["pos"],
+    refused(lambda: L.paged_prologue(NoDevice(0 if not change else -1), a["q"], a["k"], a["v"], a["q_out"], a["kc"], a["vc"], a["pos"],
                                      a["slots"], q_gain=a["q_gain"], k_gain=a["k_gain"], cos=a["cos"],
                                      sin=a["sin"], half=True), word)
