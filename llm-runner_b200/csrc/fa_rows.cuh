@@ -33,7 +33,7 @@
 // a quarter of the rate), and the row sum takes P before that rounding.
 #pragma once
 #include "fa_tc.cuh"
-#include "paged_kernels.cuh"
+#include "paged_rows.cuh"
 
 namespace llmr {
 

@@ -8,7 +8,6 @@
 #include <string.h>
 
 #include "ctx.cuh"
-#include "fa_decode.cuh"
 #include "fa_rows.cuh"
 #include "kattr.cuh"
 #include "paged_kernels.cuh"
@@ -80,24 +79,6 @@ const char *bad_paged(const llmr_paged_desc *d) {
     return "max_pages must be at least 1 and max_pages * page_size below 2^31";
   if (d->table_stride && d->table_stride < d->max_pages) return "table_stride is below max_pages";
   return nullptr;
-}
-
-// 16-bit tensor map with 128-byte swizzle; strides in elements, box[0] = 64.
-// The element type only names the zeros outside.
-int make_map16(llmr_ctx *ctx, CUtensorMap *map, const void *base, const long long (&dims)[4],
-               const long long (&strides)[3], int box1, int box2) {
-  EncodeTiledFn enc = get_encode_fn();
-  if (!enc) return fail(ctx, LLMR_ECUDA, "cuTensorMapEncodeTiled unavailable");
-  cuuint64_t d[4], st[3];
-  for (int i = 0; i < 4; i++) d[i] = (cuuint64_t)dims[i];
-  for (int i = 0; i < 3; i++) st[i] = (cuuint64_t)strides[i] * 2;
-  cuuint32_t box[4] = {64, (cuuint32_t)box1, (cuuint32_t)box2, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(base), d, st, box,
-                   estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(ctx, LLMR_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return LLMR_OK;
 }
 
 // Virtual tiles of a call: every request's tiles and one place over
@@ -174,52 +155,12 @@ int launch_fa_rows_any(llmr_ctx *ctx, int D, llmr_dtype dt, llmr_dtype od, const
 }
 
 // Query rows per (request, key/value head) up to which the decode kernel runs.
-constexpr uint32_t kDecodeRows = 32;
+constexpr uint32_t kDecodeRows = 64;
 
 uint32_t rows_per_head(const llmr_paged_desc *d) {
   const uint64_t q = d->max_q_len < d->total_tokens ? d->max_q_len : d->total_tokens;
   const uint64_t rows = q * (d->n_heads / d->n_kv_heads);
   return rows > 0xffffffffull ? 0xffffffffu : (uint32_t)rows;
-}
-
-template <int D, int MT, typename T, typename OutT>
-int launch_decode(llmr_ctx *ctx, const RowsParams &r, float *parts) {
-  using C = DecodeCfg<D, MT>;
-  DecodeParams p;
-  p.rows = r;
-  p.group = r.H / r.Hk;
-  p.scale_log2 = r.scale * 1.4426950408889634f;
-  p.parts = parts;
-  p.counters = ctx->d_sync;
-  CUtensorMap mk, mv;
-  int rc;
-  if ((rc = make_map16(ctx, &mk, r.k, {D, r.page, r.Hk, r.num_pages}, {r.ks[1], r.ks[2], r.ks[0]},
-                       r.page < 128 ? r.page : 128, 1)) ||
-      (rc = make_map16(ctx, &mv, r.v, {D, r.page, r.Hk, r.num_pages}, {r.vs[1], r.vs[2], r.vs[0]},
-                       r.page < 128 ? r.page : 128, 1)))
-    return rc;
-  auto kern = fa_decode_kernel<D, MT, T, OutT>;
-  CUDA_TRY(ctx, set_smem_once(kern, C::SMEM_BYTES));
-  int regs = 0;  // as for fa_rows: never launch a split that cannot fit
-  CUDA_TRY(ctx, launch_regs(kern, &regs));
-  if (MT > 1 && regs * C::THREADS < C::REG_NEED)
-    return fail(ctx, LLMR_ECUDA, "fa_decode: %d launch registers per thread are too few for the "
-                "register split", regs);
-  const int grid = ctx->num_sms < kDecodeCtas ? ctx->num_sms : kDecodeCtas;
-  kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mk, mv, p);
-  return after_launch(ctx, "fa_decode");
-}
-
-template <int D, int MT>
-int launch_decode_any(llmr_ctx *ctx, llmr_dtype dt, llmr_dtype od, const RowsParams &r, float *parts) {
-  if (dt == LLMR_F16) {
-    if (od == LLMR_F32) return launch_decode<D, MT, __half, float>(ctx, r, parts);
-    if (od == LLMR_F16) return launch_decode<D, MT, __half, __half>(ctx, r, parts);
-    return launch_decode<D, MT, __half, __nv_bfloat16>(ctx, r, parts);
-  }
-  if (od == LLMR_F32) return launch_decode<D, MT, __nv_bfloat16, float>(ctx, r, parts);
-  if (od == LLMR_F16) return launch_decode<D, MT, __nv_bfloat16, __half>(ctx, r, parts);
-  return launch_decode<D, MT, __nv_bfloat16, __nv_bfloat16>(ctx, r, parts);
 }
 
 // Key parts of a paged call, from its bounds alone.
@@ -300,10 +241,7 @@ int llmr_attention_causal(llmr_ctx *ctx, const llmr_causal_desc *d, const int32_
 
 size_t llmr_attention_paged_workspace_bytes(const llmr_paged_desc *d) {
   if (!d || bad_paged(d)) return 0;
-  if (rows_per_head(d) <= kDecodeRows) {
-    const size_t rows = rows_per_head(d) <= 16 ? 16 : 32;
-    return (size_t)kDecodeCtas * 2 * rows * (d->head_dim + 2) * sizeof(float);
-  }
+  if (rows_per_head(d) <= kDecodeRows) return decode_parts_bytes((int)rows_per_head(d), (int)d->head_dim);
   const int parts = paged_parts(d);
   const int tu = 2 * (128 / (int)(d->n_heads / d->n_kv_heads));
   const size_t units = (size_t)virtual_tiles(d->total_tokens, d->n_seqs, tu) * d->n_kv_heads * parts;
@@ -363,12 +301,8 @@ int llmr_attention_paged(llmr_ctx *ctx, const llmr_paged_desc *d, const int32_t 
   if (!a4(cu_q) || !a4(kv_lens) || !a4(block_table) || !a4(lse))
     return fail(ctx, LLMR_EINVAL, "cu_q, kv_lens, block_table or lse is misaligned");
   if (rows_per_head(d) <= kDecodeRows) {
-    float *parts = static_cast<float *>(ctx->ws);
-    if (rows_per_head(d) <= 16)
-      return D == 128 ? launch_decode_any<128, 1>(ctx, d->dtype, d->out_dtype, p, parts)
-                      : launch_decode_any<64, 1>(ctx, d->dtype, d->out_dtype, p, parts);
-    return D == 128 ? launch_decode_any<128, 2>(ctx, d->dtype, d->out_dtype, p, parts)
-                    : launch_decode_any<64, 2>(ctx, d->dtype, d->out_dtype, p, parts);
+    return launch_decode_any(ctx, (int)D, (int)rows_per_head(d), d->dtype, d->out_dtype, p,
+                             static_cast<float *>(ctx->ws));
   }
   return launch_fa_rows_any<true>(ctx, (int)D, d->dtype, d->out_dtype, p, paged_parts(d),
                                   static_cast<float *>(ctx->ws));

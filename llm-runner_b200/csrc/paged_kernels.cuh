@@ -1,5 +1,5 @@
 // The page planner and the norm + RoPE + cache-write prologue of the paged
-// operators, and what the paged kernels share: where a request's rows are.
+// operators.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -301,50 +301,6 @@ __global__ void __launch_bounds__(256) paged_prologue_kernel(const PagedRopePara
     store8<OutT>(dst + sub * 8, y);
     store8<OutT>(dst + D / 2 + sub * 8, y + 8);
   }
-}
-
-// ---------------------------------------------------------------- attention
-// Two fp32 values rounded to a word of T; lo lands in the low half.
-template <typename T> __device__ __forceinline__ uint32_t pack16x2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack16x2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
-template <> __device__ __forceinline__ uint32_t pack16x2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
-
-// What both attention operators are given. paged: K and V rows are found
-// through the block table; otherwise they are packed like the queries.
-struct RowsParams {
-  int n, tokens, H, Hk, page, num_pages, max_pages, max_q;
-  bool paged;
-  const int *cu, *kv_lens, *table;
-  long long table_stride;
-  const void *q, *k, *v;
-  void *o;
-  float *lse;
-  long long qs[2], os[2];        // {row, head}
-  long long ks[3], vs[3];        // {page, row, head}
-  float scale;
-  int *err;
-};
-
-// Request r's rows, checked; false (and the error bit) if its offsets or
-// lengths are out of range.
-__device__ __forceinline__ bool request_rows(const RowsParams &p, int r, int &row0, int &nq,
-                                             int &nk) {
-  const int end = p.cu[r + 1];
-  row0 = p.cu[r];
-  const bool in = 0 <= row0 && row0 <= end && end <= p.tokens;
-  nq = in ? end - row0 : 0;
-  nk = p.paged ? p.kv_lens[r] : nq;
-  const bool ok = in && nk >= 0 &&
-                  (!p.paged || (nk <= (long long)p.max_pages * p.page && nq <= p.max_q));
-  if (!ok) atomicOr(p.err, kErrInput);
-  return ok;
-}
-
-// Reports requests that no row would lead to: one CTA's `count` threads look
-// at all of them.
-__device__ __forceinline__ void check_requests(const RowsParams &p, int first, int count) {
-  int row0, nq, nk;
-  for (int r = first; r < p.n; r += count) request_rows(p, r, row0, nq, nk);
 }
 
 }  // namespace llmr
