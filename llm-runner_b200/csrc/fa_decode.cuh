@@ -147,6 +147,75 @@ __device__ __forceinline__ void finish_row(const DecodeParams &p, const DecodeSe
         none ? -INFINITY : (top + log2f(l)) * 0.69314718055994531f;
 }
 
+// Joins the parts of a pair that CTAs first .. last have left: rows warp,
+// warp + 4, .. for one warp, B of them together, U parts at a time.
+template <int D, int RW, typename OutT, int B, int U>
+__device__ __forceinline__ void join_rows(const DecodeParams &p, const DecodeSeg &sg, int nrows, int first,
+                                          int last, int warp, int lane) {
+  using C = DecodeCfg<D, RW>;
+  constexpr int E = D / 32;
+  typedef typename std::conditional<E == 4, float4, float2>::type Vec;
+  // Part x of the pair: O [ROWS][D], then (max, sum) [ROWS].
+  auto part = [&](int x) {
+    return p.parts + (long long)(2 * (first + x) + (x == 0 ? 1 : 0)) * C::PART;
+  };
+  auto part_ml = [&](int x, int r) {
+    return __ldcg(reinterpret_cast<const float2 *>(part(x) + C::ROWS * D) + r);
+  };
+  const int parts = last - first + 1;
+  for (int r0 = warp; r0 < nrows; r0 += B * C::WARPS) {
+    float top[B], l[B];
+    float acc[B][E] = {};
+#pragma unroll
+    for (int i = 0; i < B; i++) {
+      const int r = min(r0 + i * C::WARPS, nrows - 1);
+      top[i] = -INFINITY;
+      for (int x = lane; x < parts; x += 32) top[i] = fmaxf(top[i], part_ml(x, r).x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+      l[i] = 0.0f;
+    }
+    for (int x0 = 0; x0 < parts; x0 += 32) {
+      // This lane's part's weight, for all lanes.
+      float w[B];
+#pragma unroll
+      for (int i = 0; i < B; i++) {
+        const int r = min(r0 + i * C::WARPS, nrows - 1);
+        const float2 e = x0 + lane < parts ? part_ml(x0 + lane, r) : make_float2(-INFINITY, 0.0f);
+        w[i] = e.x == -INFINITY ? 0.0f : ex2_approx(e.x - top[i]);
+        l[i] += w[i] * e.y;
+      }
+      const int n = min(32, parts - x0);
+      for (int x = 0; x < n; x += U) {
+        Vec v[U][B];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int i = 0; i < B; i++)
+            v[u][i] = __ldcg(reinterpret_cast<const Vec *>(
+                          part(x0 + min(x + u, n - 1)) + min(r0 + i * C::WARPS, nrows - 1) * D) + lane);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int i = 0; i < B; i++) {
+            const float f = x + u < n ? __shfl_sync(0xffffffffu, w[i], (x + u) & 31) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++)
+              if (f != 0.0f) acc[i][e] = fmaf(elem(v[u][i], e), f, acc[i][e]);
+          }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < B; i++) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+      const int r = r0 + i * C::WARPS;
+      if (r < nrows)
+        finish_row<D, OutT>(p, sg, r, lane * E, *reinterpret_cast<const Vec *>(acc[i]), top[i], l[i]);
+    }
+  }
+}
+
 template <int D, int RW, typename T, typename OutT>
 __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
     fa_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -519,27 +588,12 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
       named_barrier(1, 32 * C::WARPS);
       if (*last_flag) {
         __threadfence();
-        for (int x = tid; x < nrows * (D / 4); x += 32 * C::WARPS) {
-          const int r = x / (D / 4), col = (x - r * (D / 4)) * 4;
-          auto at_part = [&](int c) { return p.parts + (long long)(2 * c + (c == first ? 1 : 0)) * C::PART; };
-          float top = -INFINITY, l = 0.0f;
-#pragma unroll 4
-          for (int c = first; c <= last; c++)
-            top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(at_part(c) + C::ROWS * D) + r).x);
-          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-          for (int c = first; c <= last; c++) {
-            const float2 e = __ldcg(reinterpret_cast<const float2 *>(at_part(c) + C::ROWS * D) + r);
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(at_part(c) + r * D + col));
-            const float f = e.x == -INFINITY ? 0.0f : ex2_approx(e.x - top);
-            l = fmaf(e.y, f, l);
-            acc.x = fmaf(v.x, f, acc.x);
-            acc.y = fmaf(v.y, f, acc.y);
-            acc.z = fmaf(v.z, f, acc.z);
-            acc.w = fmaf(v.w, f, acc.w);
-          }
-          finish_row<D, OutT>(p, sg, r, col, acc, top, l);
-        }
+        // A warp takes a row (two of many rows) at a time, its lanes the row's
+        // columns; eight parts are asked for before any is used.
+        if (nrows <= C::WARPS)
+          join_rows<D, RW, OutT, 1, 8>(p, sg, nrows, first, last, warp, lane);
+        else
+          join_rows<D, RW, OutT, 2, 4>(p, sg, nrows, first, last, warp, lane);
         if (tid == 0) p.counters[first] = 0;
       }
       named_barrier(1, 32 * C::WARPS);  // last_flag may be written again

@@ -8,13 +8,18 @@
 // some row of the tile sees are visited.
 //
 // Work unit: (request, key/value head, 2 * tpt tokens[, part of the keys]).
-// Requests' offsets are device data, so units are numbered without knowing
-// them: request i starts at virtual tile cu[i] / (2 tpt) + i, which leaves room
-// for its tiles and at most one empty one behind them, and is found by
-// searching cu. Units are handed out last tokens first (the longest rows of a
-// causal prompt first), by cluster launch control: a CTA takes over units
-// whose CTAs have not started, so no counter in memory is needed and a light
-// unit's CTA goes on at once.
+// Requests' offsets are device data, so each CTA finds its units itself.
+//  * Prompts: units are numbered without knowing the offsets. Request i
+//    starts at virtual tile cu[i] / (2 tpt) + i, which leaves room for its tiles
+//    and at most one empty one behind them, and is found by searching cu. Units
+//    are handed out last tokens first (the longest rows first), by cluster
+//    launch control: a CTA takes over units whose CTAs have not started, so no
+//    counter in memory is needed. It asks when the last loads of its unit are
+//    under way and no sooner: a unit held early is one that an idle CTA lacks.
+//  * Paged chunks: few units of very different lengths, so all units' keys
+//    (and kUnitKeys more for each unit's ends) are laid end to end and cut into one
+//    range per CTA. A unit that a cut falls into leaves parts in the
+//    workspace, joined by a second launch; cuts near a unit's ends move there.
 //
 // CTA: 384 threads, as the non-causal kernel divides them:
 //   warps 0-3 / 4-7  softmax of tile 0 / 1, one query row per thread
@@ -38,18 +43,29 @@
 namespace llmr {
 
 constexpr int kUnitSlots = 2;  // the unit in work and the next
-// Splitting a unit's keys pays from this many blocks of 128 per part.
-constexpr int kMinSplitBlocks = 8;
+constexpr int kMaxRanges = 160;  // CTAs of a paged call (workspace)
+// What a unit costs besides its keys, in keys; blocks of 128 that a cut keeps
+// away from a unit's ends; least keys of a range.
+constexpr int kUnitKeys = 128;
+constexpr int kCutBlocks = 3;
+constexpr int kRangeKeys = 1024;
+
+// A unit that a cut falls into, entered by the CTA that begins it: its parts
+// are that CTA's second part and the first parts of the CTAs up to `last`.
+struct FaJoin {
+  int last;  // -1: the CTA begins no such unit
+  int q_row, tokens, kvh;
+};
 
 struct FaRowsParams {
   RowsParams rows;
   int group, tpt, recip;  // recip: r / group = r * recip >> 16 for r < 128
-  int vtiles;             // virtual tiles of all requests
-  int nsplit;             // parts a unit may be cut into
-  int units;              // vtiles * Hk * nsplit
-  int dynamic;            // units are taken over by cluster launch control
+  int vtiles;             // prompts: virtual tiles of all requests
+  int units;              // prompts: vtiles * Hk
+  int dynamic;            // prompts: units are taken over by cluster launch control
   float scale_log2;
-  float *part_o, *part_lse;  // [unit][part][256 rows]([D])
+  float *part_o, *part_lse;  // paged: [2 * CTA + 0 / 1][256 rows]([D])
+  FaJoin *joins;             // paged: [CTA]
 };
 
 // One unit, as the scheduler hands it to the other warps.
@@ -64,15 +80,6 @@ struct FaUnit {
   int nb[2];       // key blocks of each tile
   int part;        // -1, or where the partial result goes
 };
-
-// Blocks of 128 keys that part s of ns takes of n.
-__host__ __device__ __forceinline__ int split_at(int n, int ns, int s) {
-  return (int)((long long)n * s / ns);
-}
-__host__ __device__ __forceinline__ int parts_of(int blocks, int nsplit) {
-  const int most = blocks / kMinSplitBlocks;
-  return most < 1 ? 1 : most < nsplit ? most : nsplit;
-}
 
 // The request that virtual tile vt belongs to: the last with
 // cu[i] / tu + i <= vt. Whole warp, 32 probes at a time.
@@ -90,35 +97,61 @@ __device__ __forceinline__ int find_request(const int *cu, int n, int tu, int vt
   return lo;
 }
 
-// Virtual unit u; false if it is empty. Whole warp.
-template <bool PAGED>
-__device__ __forceinline__ bool fa_unit(const FaRowsParams &p, int u, FaUnit &un) {
-  const int s = u % p.nsplit, vh = u / p.nsplit;
-  const int vt = p.vtiles - 1 - vh / p.rows.Hk;
-  const int tu = 2 * p.tpt;
+// Tile `tile` of a request: all of a unit but its range of key blocks.
+__device__ __forceinline__ void unit_rows(FaUnit &un, int tu, int kvh, int row0, int nq, int nk, int tile) {
+  const int first = tile * tu;
+  un.kvh = kvh;
+  un.q_row = row0 + first;
+  un.tokens = min(tu, nq - first);
+  un.pos = nk - nq + first;
+  un.keys = max(0, un.pos + un.tokens);
+  un.part = -1;
+}
+// Key blocks [b0, b1) of the unit, of which tile 0 sees those with its keys.
+__device__ __forceinline__ void unit_blocks(FaUnit &un, int tpt, int b0, int b1) {
+  const int k0 = max(0, un.pos + min(un.tokens, tpt));
+  un.blk = b0;
+  un.nb[0] = max(0, min((k0 + 127) / 128, b1) - b0);
+  un.nb[1] = un.tokens > tpt ? b1 - b0 : 0;
+}
+
+// Prompts: virtual unit u; false if it is empty. Whole warp.
+__device__ __forceinline__ bool prompt_unit(const FaRowsParams &p, int u, FaUnit &un) {
+  const int vt = p.vtiles - 1 - u / p.rows.Hk, tu = 2 * p.tpt;
   const int r = find_request(p.rows.cu, p.rows.n, tu, vt);
   int row0, nq, nk;
   if (!request_rows(p.rows, r, row0, nq, nk)) return false;
-  const int first = (vt - (row0 / tu + r)) * tu;
-  if (first < 0 || first >= nq) return false;
-  un.kvh = vh % p.rows.Hk;
-  un.q_row = row0 + first;
-  un.tokens = min(tu, nq - first);
-  un.kv_row = PAGED ? r : row0;
-  un.pos = nk - nq + first;
-  const int k0 = max(0, un.pos + min(un.tokens, p.tpt));
-  const int k1 = max(0, un.pos + un.tokens);
-  un.keys = k1;
-  const int all = (k1 + 127) / 128;
-  const int parts = parts_of(all, p.nsplit);
-  if (s >= parts) return false;
-  const int end = split_at(all, parts, s + 1);
-  un.blk = split_at(all, parts, s);
-  un.nb[0] = max(0, min((k0 + 127) / 128, end) - un.blk);
-  un.nb[1] = un.tokens > p.tpt ? end - un.blk : 0;
-  un.part = parts > 1 ? u : -1;
+  const int tile = vt - (row0 / tu + r);
+  if (tile < 0 || tile >= (nq + tu - 1) / tu) return false;
+  unit_rows(un, tu, u % p.rows.Hk, row0, nq, nk, tile);
+  un.kv_row = row0;
+  unit_blocks(un, p.tpt, 0, (un.keys + 127) / 128);
   return true;
 }
+
+// Paged: where tile i of a request begins, in keys from the request's first:
+// tile j counts its last token's position (as if it were full) and kUnitKeys.
+__host__ __device__ __forceinline__ long long tile_begin(long long ctx, long long tu, long long i) {
+  return i * (ctx + kUnitKeys) + tu * (i * (i + 1) / 2);
+}
+// Paged: the block that a cut `y` keys into a unit of `blocks` blocks falls
+// on; a few blocks at either end belong to the neighbour.
+__host__ __device__ __forceinline__ int cut_block(long long y, int blocks) {
+  const long long b = y <= kUnitKeys ? 0 : (y - kUnitKeys) / 128;
+  if (b < kCutBlocks) return 0;
+  return b > blocks - kCutBlocks ? blocks : (int)b;
+}
+// Beginning of range c of `ranges`.
+__host__ __device__ __forceinline__ long long cut_at(long long line, int ranges, int c) {
+  return line / ranges * c + line % ranges * c / ranges;
+}
+
+// A cut of the line: request, head, tile, key block, and where that tile's unit
+// begins in the line; r = n behind the last.
+struct FaCut {
+  int r, kvh, tile, blk;
+  long long begin;
+};
 
 template <int D>
 struct FaRowsCfg {
@@ -131,8 +164,8 @@ struct FaRowsCfg {
   static constexpr int EPI_OFF = KV_OFF + NST * TILE_BYTES;  // 4 KB per softmax warp
   static constexpr int CTL_OFF = EPI_OFF + 8 * 4096;
   // q_full, q_empty, kv_full[NST], kv_empty[NST], s_full[2], p_half[4],
-  // o_full[2], o_empty[2], u_full[], u_empty[], clc, drain
-  static constexpr int NBAR = 2 + 2 * NST + 2 + 4 + 2 + 2 + 2 * kUnitSlots + 2;
+  // o_full[2], o_empty[2], u_full[], u_empty[], u_ask, clc, drain
+  static constexpr int NBAR = 2 + 2 * NST + 2 + 4 + 2 + 2 + 2 * kUnitSlots + 3;
   static constexpr int UNIT_OFF = CTL_OFF + (NBAR * 8 + 15) / 16 * 16;
   static constexpr int CLC_OFF = UNIT_OFF + kUnitSlots * 48;
   static constexpr int SMEM_BYTES = CLC_OFF + 32 + 1024;
@@ -144,6 +177,137 @@ struct FaRowsCfg {
   static_assert(sizeof(FaUnit) <= 48, "unit slot");
   static constexpr uint32_t O_COL = 256;
 };
+
+// Paged: a request's length in the line, per key/value head.
+__device__ __forceinline__ long long request_line(const RowsParams &p, int tu, int r, int &row0, int &nq,
+                                                  int &nk) {
+  if (!request_rows(p, r, row0, nq, nk) || nq == 0) return 0;
+  return tile_begin(max(0, nk - nq), tu, (nq + tu - 1) / tu);
+}
+
+// Paged, all 384 threads: the cuts before and behind this CTA's range.
+__device__ __forceinline__ void find_range(const FaRowsParams &p, uint8_t *smem, FaCut &lo, FaCut &hi,
+                                           long long &line, int &ranges) {
+  constexpr int THREADS = 384, WARPS = THREADS / 32;
+  const RowsParams &rp = p.rows;
+  long long *sums = reinterpret_cast<long long *>(smem);  // [WARPS]
+  FaCut *cuts = reinterpret_cast<FaCut *>(smem + 128);     // [2]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tu = 2 * p.tpt;
+  int row0 = 0, nq = 0, nk = 0;
+  long long mine = 0, incl = 0, total = 0;
+  auto block_scan = [&](int i0) {
+    const int r = i0 + tid;
+    mine = r < rp.n ? request_line(rp, tu, r, row0, nq, nk) : 0;
+    incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    long long sum = 0;
+    for (int w = 0; w < WARPS; w++) {
+      if (w == warp) incl += sum;
+      sum += sums[w];
+    }
+    return sum;
+  };
+  for (int i0 = 0; i0 < rp.n; i0 += THREADS) total += block_scan(i0);
+  line = total * rp.Hk;
+  const long long most = max(1ll, line / kRangeKeys);
+  ranges = most < (long long)gridDim.x ? (int)most : (int)gridDim.x;
+  const int c = blockIdx.x;
+  if (tid < 2) cuts[tid] = FaCut{rp.n, 0, 0, 0, 0};
+  __syncthreads();
+  if (c < ranges && line > 0) {
+    const long long at[2] = {cut_at(line, ranges, c), cut_at(line, ranges, c + 1)};
+    long long before = 0;
+    for (int i0 = 0; i0 < rp.n; i0 += THREADS) {
+      long long sum = total;
+      if (rp.n > THREADS) sum = block_scan(i0);
+      const long long b = (before + incl - mine) * rp.Hk;
+      for (int e = 0; e < 2; e++)
+        if (mine > 0 && b <= at[e] && at[e] < b + mine * rp.Hk) {
+          const long long y = at[e] - b, ctx = max(0, nk - nq);
+          const int kvh = (int)(y / mine);
+          const long long z = y - kvh * mine;
+          int t0 = 0, t1 = (nq + tu - 1) / tu;  // the last tile that begins at or before z
+          while (t1 - t0 > 1) {
+            const int mid = (t0 + t1) >> 1;
+            if (tile_begin(ctx, tu, mid) <= z) t0 = mid;
+            else t1 = mid;
+          }
+          FaUnit un;
+          unit_rows(un, tu, kvh, row0, nq, nk, t0);
+          const long long into = z - tile_begin(ctx, tu, t0);
+          cuts[e] = FaCut{i0 + tid, kvh, t0, cut_block(into, (un.keys + 127) / 128), at[e] - into};
+        }
+      before += sum;
+    }
+  }
+  __syncthreads();
+  lo = cuts[0];
+  hi = cuts[1];
+  __syncthreads();  // smem is free again
+}
+
+// Paged, the scheduler warp: hands the units between the cuts to
+// give(i, unit), the end among them, and enters the unit that the next CTA goes
+// on with.
+template <typename Give>
+__device__ __forceinline__ void walk_range(const FaRowsParams &p, const FaCut &lo, const FaCut &hi,
+                                           long long line, int ranges, Give give) {
+  const RowsParams &rp = p.rows;
+  const int tu = 2 * p.tpt, c = blockIdx.x;
+  FaJoin join{-1, 0, 0, 0};
+  FaUnit un;
+  int i = 0, row0 = 0, nq = 0, nk = 0;
+  bool ok = true;
+  FaCut at = lo;
+  if (at.r < rp.n) request_rows(rp, at.r, row0, nq, nk);
+  while (ok && at.r < rp.n) {
+    const bool last = at.r == hi.r && at.kvh == hi.kvh && at.tile == hi.tile;
+    unit_rows(un, tu, at.kvh, row0, nq, nk, at.tile);
+    un.kv_row = at.r;
+    const int blocks = (un.keys + 127) / 128;
+    const int end = last ? hi.blk : blocks;
+    // Rows without a key are written by every CTA that comes by.
+    if (at.blk < end || blocks == 0) {
+      unit_blocks(un, p.tpt, at.blk, end);
+      if (at.blk > 0 || end < blocks) un.part = 2 * c + (at.blk > 0 ? 0 : 1);
+      if (at.blk == 0 && end < blocks) join = FaJoin{c, un.q_row, un.tokens, un.kvh};
+      ok = give(i++, un);
+    }
+    if (last) break;
+    at.blk = 0;
+    if (++at.tile * tu < nq) continue;
+    at.tile = 0;
+    if (++at.kvh < rp.Hk) continue;
+    at.kvh = 0;
+    do {
+      at.r++;
+    } while (at.r < rp.n && request_line(rp, tu, at.r, row0, nq, nk) == 0);
+  }
+  un.kvh = -1;
+  if (ok) give(i, un);
+  if (join.last >= 0) {
+    // The unit (hi's, of the request last looked at) ends in the first later
+    // range whose end is at or behind the unit's. 32 ranges at a time.
+    const long long ctx = max(0, nk - nq);
+    const long long length = tile_begin(ctx, tu, hi.tile + 1) - tile_begin(ctx, tu, hi.tile);
+    unit_rows(un, tu, hi.kvh, row0, nq, nk, hi.tile);
+    const int blocks = (un.keys + 127) / 128, lane = threadIdx.x & 31;
+    for (int x = c + 1; join.last == c; x += 32) {
+      const int end = x + lane + 1;  // the range x + lane ends at this cut
+      const long long e = end >= ranges ? length : cut_at(line, ranges, end) - hi.begin;
+      const unsigned m = __ballot_sync(0xffffffffu, e >= length || cut_block(e, blocks) == blocks);
+      if (m) join.last = x + __ffs(m) - 1;
+    }
+  }
+  if ((threadIdx.x & 31) == 0) p.joins[c] = join;
+}
 
 template <int D, typename T, typename OutT, bool PAGED>
 __global__ void __launch_bounds__(384, 1)
@@ -164,7 +328,8 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t *o_empty = o_full + 2;  // [t]
   uint64_t *u_full = o_empty + 2;
   uint64_t *u_empty = u_full + kUnitSlots;
-  uint64_t *clc_bar = u_empty + kUnitSlots;
+  uint64_t *u_ask = u_empty + kUnitSlots;
+  uint64_t *clc_bar = u_ask + 1;
   uint64_t *drain = clc_bar + 1;
   auto unit_slot = [&](int i) {
     return reinterpret_cast<FaUnit *>(smem + C::UNIT_OFF + (i % kUnitSlots) * 48);
@@ -192,6 +357,7 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(&u_full[i], 1);
       mbar_init(&u_empty[i], 10);  // producer, MMA issuer, 8 softmax warps
     }
+    mbar_init(u_ask, 1);
     mbar_init(clc_bar, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -205,6 +371,10 @@ __global__ void __launch_bounds__(384, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_base_slot;
+  FaCut lo, hi;
+  long long line = 0;
+  int ranges = 1;
+  if constexpr (PAGED) find_range(p, smem + C::EPI_OFF, lo, hi, line, ranges);
 
   // A whole warp's wait; all lanes get the same answer, also when it is given up.
   auto wait = [&](uint64_t *bar, int phase) {
@@ -236,7 +406,10 @@ __global__ void __launch_bounds__(384, 1)
       FaUnit un;
       for (int i = 0; next_unit(i, un); i++) {
         const int nblk = max(un.nb[0], un.nb[1]);
-        if (nblk == 0) continue;
+        if (nblk == 0) {
+          if (lane == 0) mbar_arrive(u_ask);
+          continue;
+        }
         if (kq > 0 && !(ok = wait(q_empty, kq - 1))) break;
         if (lane == 0) {
           const int tiles = un.tokens > p.tpt ? 2 : 1;
@@ -285,6 +458,7 @@ __global__ void __launch_bounds__(384, 1)
           page = next_page;
         }
         if (!ok) break;
+        if (lane == 0) mbar_arrive(u_ask);  // the unit's loads are under way
       }
       if (*abort_flag && lane == 0) {
         // Abort path: let every armed copy land before the CTA exits.
@@ -396,38 +570,50 @@ __global__ void __launch_bounds__(384, 1)
       mbar_wait_raw(drain, 0, 100000000ull);
     } else if (warp == 10) {
       // --------------------------------------------------------- scheduler
-      // A unit is asked for when its slot is free, so a CTA holds one unit
-      // ahead of the one it computes and no more.
       FaUnit un;
-      int u = blockIdx.x, asked = 0;
-      bool ok = true, have = true;
-      for (int i = 0; ok && have; i++) {
-        if (i >= kUnitSlots && !(ok = wait(&u_empty[i % kUnitSlots], i / kUnitSlots - 1))) break;
-        for (bool first = i == 0;; first = false) {
-          if (!first && p.dynamic) {
-            if (lane == 0) {
-              mbar_arrive_expect_tx(clc_bar, 16);
-              clc_try_cancel(clc_resp, clc_bar);
-            }
-            __syncwarp();
-            if (!(ok = wait(clc_bar, asked))) {
-              mbar_wait_raw(clc_bar, asked & 1, 100000000ull);
-              break;
-            }
-            asked++;
-            u = clc_answer(clc_resp);
-            fence_proxy_async_smem();
-            __syncwarp();
-          } else if (!first) {
-            u = u < p.units - (int)gridDim.x ? u + (int)gridDim.x : -1;
-          }
-          have = u >= 0;
-          if (!have || fa_unit<PAGED>(p, u, un)) break;
-        }
-        if (ok && lane == 0) {
-          if (!have) un.kvh = -1;
+      auto hand_out = [&](int i) {  // un as the CTA's i-th
+        if (lane == 0) {
           *unit_slot(i) = un;
           mbar_arrive(&u_full[i % kUnitSlots]);
+        }
+      };
+      if constexpr (PAGED) {
+        walk_range(p, lo, hi, line, ranges, [&](int i, const FaUnit &next) {
+          if (i >= kUnitSlots && !wait(&u_empty[i % kUnitSlots], i / kUnitSlots - 1)) return false;
+          un = next;
+          hand_out(i);
+          return true;
+        });
+      } else {
+        int u = blockIdx.x, asked = 0;
+        bool ok = true, have = true;
+        for (int i = 0; ok && have; i++) {
+          if (i > 0 && !(ok = wait(u_ask, i - 1))) break;
+          if (i >= kUnitSlots && !(ok = wait(&u_empty[i % kUnitSlots], i / kUnitSlots - 1))) break;
+          for (bool first = i == 0;; first = false) {
+            if (!first && p.dynamic) {
+              if (lane == 0) {
+                mbar_arrive_expect_tx(clc_bar, 16);
+                clc_try_cancel(clc_resp, clc_bar);
+              }
+              __syncwarp();
+              if (!(ok = wait(clc_bar, asked))) {
+                mbar_wait_raw(clc_bar, asked & 1, 100000000ull);
+                break;
+              }
+              asked++;
+              u = clc_answer(clc_resp);
+              fence_proxy_async_smem();
+              __syncwarp();
+            } else if (!first) {
+              u = u < p.units - (int)gridDim.x ? u + (int)gridDim.x : -1;
+            }
+            have = u >= 0;
+            if (!have || prompt_unit(p, u, un)) break;
+          }
+          if (!ok) break;
+          if (!have) un.kvh = -1;
+          hand_out(i);
         }
       }
     } else if (blockIdx.x == 0) {
@@ -640,46 +826,80 @@ __global__ void __launch_bounds__(384, 1)
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.rows.err, kErrTimeout);
 }
 
-// Joins the parts of units whose keys were split: one warp per (unit, row),
-// o = sum_s w_s o_s with w_s = exp(lse_s) / sum exp(lse), parts in order.
-template <int D, typename OutT, bool PAGED>
+// Joins the parts of the units that cuts fell into (paged): o = sum_s w_s o_s
+// with w_s = exp(lse_s) / sum exp(lse), parts in the order of the keys. One
+// CTA per (range, 32 of its unit's rows), a warp for 4 rows, 4 parts at a time
+// so that their loads overlap; lane x first finds the weight of part x.
+template <int D, typename OutT>
 __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant__ FaRowsParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int first = (int)(w >> 8) * p.nsplit, row = (int)(w & 255);
-  FaUnit un;
-  if (first >= p.units || !fa_unit<PAGED>(p, first, un) || un.part < 0) return;
-  const int t = row >> 7, tr = row & 127;
-  const int rt = tr * p.recip >> 16, tok = t * p.tpt + rt;
-  if (rt >= p.tpt || tok >= un.tokens) return;
-  const int parts = parts_of((un.keys + 127) / 128, p.nsplit);
-  const long long base = (long long)first * 256 + row;
-  float mx = -INFINITY;
-  for (int s = lane; s < parts; s += 32) mx = fmaxf(mx, p.part_lse[base + s * 256]);
+  griddep_wait();
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int E = D / 32, ROWS = 4, U = 4;
+  const int row0 = blockIdx.y * 32 + warp * ROWS;
+  const FaJoin join = p.joins[c];
+  if (join.last < 0) return;
+  // A warp's four rows lie in one tile; it may be empty, or behind the tokens.
+  const int tok0 = (row0 >> 7) * p.tpt + ((row0 & 127) * p.recip >> 16);
+  if (tok0 >= join.tokens) return;
+  const int parts = join.last - c + 1;
+  auto part_row = [&](int x, int i) { return (long long)(2 * (c + x) + (x == 0 ? 1 : 0)) * 256 + row0 + i; };
+  float mx[ROWS], acc[ROWS][E] = {}, sum[ROWS] = {};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  constexpr int E = D / 32;
-  float acc[E] = {}, sum = 0.0f;
-  for (int s = 0; s < parts; s++) {
-    const float ls = p.part_lse[base + s * 256];
-    if (ls == -INFINITY) continue;  // saw no key; nothing was written
-    const float wt = expf(ls - mx);
-    sum += wt;
-    const Pack<float, E> v = *reinterpret_cast<const Pack<float, E> *>(
-        p.part_o + (base + s * 256) * D + lane * E);
+  for (int i = 0; i < ROWS; i++) mx[i] = -INFINITY;
+  for (int x = lane; x < parts; x += 32)
 #pragma unroll
-    for (int e = 0; e < E; e++) acc[e] = fmaf(wt, v.v[e], acc[e]);
+    for (int i = 0; i < ROWS; i++) mx[i] = fmaxf(mx[i], p.part_lse[part_row(x, i)]);
+#pragma unroll
+  for (int i = 0; i < ROWS; i++)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+  for (int x0 = 0; x0 < parts; x0 += 32) {
+    float w[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+      const float ls = x0 + lane < parts ? p.part_lse[part_row(x0 + lane, i)] : -INFINITY;
+      w[i] = ls == -INFINITY ? 0.0f : expf(ls - mx[i]);  // 0: saw no key
+      sum[i] += w[i];
+    }
+    const int n = min(32, parts - x0);
+    for (int x = 0; x < n; x += U) {
+      Pack<float, E> v[U][ROWS];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int i = 0; i < ROWS; i++)
+          v[u][i] = *reinterpret_cast<const Pack<float, E> *>(
+              p.part_o + part_row(x0 + min(x + u, n - 1), i) * D + lane * E);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+          const float f = x + u < n ? __shfl_sync(0xffffffffu, w[i], (x + u) & 31) : 0.0f;
+          if (f != 0.0f)
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[i][e] = fmaf(f, v[u][i].v[e], acc[i][e]);
+        }
+    }
   }
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  const int h = un.kvh * p.group + tr - rt * p.group;
-  const int q_row = un.q_row + tok;
-  Pack<OutT, E> out;
 #pragma unroll
-  for (int e = 0; e < E; e++) out.v[e] = from_f32<OutT>(acc[e] * inv);
-  *reinterpret_cast<Pack<OutT, E> *>(static_cast<OutT *>(p.rows.o) + (long long)q_row * p.rows.os[0] +
-                                     (long long)h * p.rows.os[1] + lane * E) = out;
-  if (p.rows.lse && lane == 0)
-    p.rows.lse[(long long)h * p.rows.tokens + q_row] = sum > 0.0f ? mx + logf(sum) : -INFINITY;
+  for (int i = 0; i < ROWS; i++)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+    const int row = row0 + i, t = row >> 7, tr = row & 127;
+    const int rt = tr * p.recip >> 16, tok = t * p.tpt + rt;
+    if (rt >= p.tpt || tok >= join.tokens) continue;
+    const float inv = sum[i] > 0.0f ? 1.0f / sum[i] : 0.0f;
+    const int h = join.kvh * p.group + tr - rt * p.group, q_row = join.q_row + tok;
+    Pack<OutT, E> out;
+#pragma unroll
+    for (int e = 0; e < E; e++) out.v[e] = from_f32<OutT>(acc[i][e] * inv);
+    *reinterpret_cast<Pack<OutT, E> *>(static_cast<OutT *>(p.rows.o) + (long long)q_row * p.rows.os[0] +
+                                       (long long)h * p.rows.os[1] + lane * E) = out;
+    if (p.rows.lse && lane == 0)
+      p.rows.lse[(long long)h * p.rows.tokens + q_row] = sum[i] > 0.0f ? mx[i] + logf(sum[i]) : -INFINITY;
+  }
 }
 
 }  // namespace llmr

@@ -81,33 +81,36 @@ const char *bad_paged(const llmr_paged_desc *d) {
   return nullptr;
 }
 
-// Virtual tiles of a call: every request's tiles and one place over
-// (fa_rows.cuh).
-long long virtual_tiles(long long tokens, long long n, int tu) { return tokens / tu + n; }
-
-// Parts a unit's keys may be cut into: so many that one wave of CTAs covers
-// 148 SMs when there are few units (a long context and few rows).
-int split_parts(long long units) { return units >= 148 ? 1 : (int)(148 / units); }
+// Workspace of the paged chunk kernel: two parts per CTA (O and log-sum-exp of
+// 256 rows) and its unit to join.
+size_t chunk_parts_bytes(int D) {
+  return (size_t)kMaxRanges * (2 * 256 * (D + 1) * sizeof(float) + sizeof(FaJoin));
+}
 
 template <int D, typename T, typename OutT, bool PAGED>
-int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r, int nsplit, float *part) {
+int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r) {
   using C = FaRowsCfg<D>;
-  FaRowsParams p;
+  FaRowsParams p = {};
   p.rows = r;
   p.group = r.H / r.Hk;
   p.tpt = 128 / p.group;
   p.recip = (65536 + p.group - 1) / p.group;
-  const long long vt = virtual_tiles(r.tokens, r.n, 2 * p.tpt);
-  const long long units = vt * r.Hk * nsplit;
-  if (units > 0x7fffffffLL) return fail(ctx, LLMR_EINVAL, "problem too large");
-  p.vtiles = (int)vt;
-  p.nsplit = nsplit;
-  p.units = (int)units;
-  // With an SM budget the grid is that small and strides over the units.
-  p.dynamic = units > ctx->num_sms && ctx->num_sms == ctx->total_sms;
   p.scale_log2 = r.scale * 1.4426950408889634f;
-  p.part_o = part;
-  p.part_lse = part ? part + units * 256 * D : nullptr;
+  int grid;
+  if (PAGED) {
+    grid = ctx->num_sms < kMaxRanges ? ctx->num_sms : kMaxRanges;
+    p.part_o = static_cast<float *>(ctx->ws);
+    p.part_lse = p.part_o + (size_t)2 * kMaxRanges * 256 * D;
+    p.joins = reinterpret_cast<FaJoin *>(p.part_lse + (size_t)2 * kMaxRanges * 256);
+  } else {
+    const long long vt = (long long)r.tokens / (2 * p.tpt) + r.n, units = vt * r.Hk;
+    if (units > 0x7fffffffLL) return fail(ctx, LLMR_EINVAL, "problem too large");
+    p.vtiles = (int)vt;
+    p.units = (int)units;
+    // With an SM budget the grid is that small and strides over the units.
+    p.dynamic = units > ctx->num_sms && ctx->num_sms == ctx->total_sms;
+    grid = p.dynamic || units < ctx->num_sms ? (int)units : ctx->num_sms;
+  }
   CUtensorMap mq, mk, mv;
   int rc;
   if ((rc = make_map16(ctx, &mq, r.q, {D, p.group, r.tokens, r.Hk},
@@ -129,44 +132,48 @@ int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r, int nsplit, float *part) 
   if (regs * C::THREADS < C::REG_NEED)
     return fail(ctx, LLMR_ECUDA, "fa_rows: %d launch registers per thread are too few for the "
                 "register split", regs);
-  const unsigned grid = p.dynamic || units < ctx->num_sms ? (unsigned)units : (unsigned)ctx->num_sms;
   kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mq, mk, mv, p);
-  if ((rc = after_launch(ctx, "fa_rows"))) return rc;
-  if (nsplit == 1) return LLMR_OK;
-  fa_rows_join_kernel<D, OutT, PAGED><<<(unsigned)(units / nsplit * 32), 256, 0, ctx->stream>>>(p);
+  if ((rc = after_launch(ctx, "fa_rows")) || !PAGED) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto join = fa_rows_join_kernel<D, OutT>;
+  CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, join, p));
   return after_launch(ctx, "fa_rows_join");
 }
 
 template <int D, typename T, bool PAGED>
-int launch_fa_rows_o(llmr_ctx *ctx, llmr_dtype od, const RowsParams &r, int nsplit, float *part) {
-  if (od == LLMR_F32) return launch_fa_rows<D, T, float, PAGED>(ctx, r, nsplit, part);
-  if (od == LLMR_F16) return launch_fa_rows<D, T, __half, PAGED>(ctx, r, nsplit, part);
-  return launch_fa_rows<D, T, __nv_bfloat16, PAGED>(ctx, r, nsplit, part);
+int launch_fa_rows_o(llmr_ctx *ctx, llmr_dtype od, const RowsParams &r) {
+  if (od == LLMR_F32) return launch_fa_rows<D, T, float, PAGED>(ctx, r);
+  if (od == LLMR_F16) return launch_fa_rows<D, T, __half, PAGED>(ctx, r);
+  return launch_fa_rows<D, T, __nv_bfloat16, PAGED>(ctx, r);
 }
 
 template <bool PAGED>
-int launch_fa_rows_any(llmr_ctx *ctx, int D, llmr_dtype dt, llmr_dtype od, const RowsParams &r,
-                       int nsplit, float *part) {
+int launch_fa_rows_any(llmr_ctx *ctx, int D, llmr_dtype dt, llmr_dtype od, const RowsParams &r) {
   if (D == 128)
-    return dt == LLMR_F16 ? launch_fa_rows_o<128, __half, PAGED>(ctx, od, r, nsplit, part)
-                          : launch_fa_rows_o<128, __nv_bfloat16, PAGED>(ctx, od, r, nsplit, part);
-  return dt == LLMR_F16 ? launch_fa_rows_o<64, __half, PAGED>(ctx, od, r, nsplit, part)
-                        : launch_fa_rows_o<64, __nv_bfloat16, PAGED>(ctx, od, r, nsplit, part);
+    return dt == LLMR_F16 ? launch_fa_rows_o<128, __half, PAGED>(ctx, od, r)
+                          : launch_fa_rows_o<128, __nv_bfloat16, PAGED>(ctx, od, r);
+  return dt == LLMR_F16 ? launch_fa_rows_o<64, __half, PAGED>(ctx, od, r)
+                        : launch_fa_rows_o<64, __nv_bfloat16, PAGED>(ctx, od, r);
 }
 
 // Query rows per (request, key/value head) up to which the decode kernel runs.
-constexpr uint32_t kDecodeRows = 64;
+#ifndef DROWS
+#define DROWS 64
+#endif
+constexpr uint32_t kDecodeRows = DROWS;
 
 uint32_t rows_per_head(const llmr_paged_desc *d) {
   const uint64_t q = d->max_q_len < d->total_tokens ? d->max_q_len : d->total_tokens;
   const uint64_t rows = q * (d->n_heads / d->n_kv_heads);
   return rows > 0xffffffffull ? 0xffffffffu : (uint32_t)rows;
-}
-
-// Key parts of a paged call, from its bounds alone.
-int paged_parts(const llmr_paged_desc *d) {
-  const int tu = 2 * (128 / (int)(d->n_heads / d->n_kv_heads));
-  return split_parts(virtual_tiles(d->total_tokens, d->n_seqs, tu) * d->n_kv_heads);
 }
 
 template <int D, typename InT, typename OutT>
@@ -236,16 +243,13 @@ int llmr_attention_causal(llmr_ctx *ctx, const llmr_causal_desc *d, const int32_
       !strides16({p.os[0], p.os[1]}, size_of(d->out_dtype)))
     return fail(ctx, LLMR_EINVAL, "q, k, v, o and their strides must be 16-byte aligned");
   if (!a4(cu_seqlens) || !a4(lse)) return fail(ctx, LLMR_EINVAL, "cu_seqlens or lse is misaligned");
-  return launch_fa_rows_any<false>(ctx, (int)D, d->dtype, d->out_dtype, p, 1, nullptr);
+  return launch_fa_rows_any<false>(ctx, (int)D, d->dtype, d->out_dtype, p);
 }
 
 size_t llmr_attention_paged_workspace_bytes(const llmr_paged_desc *d) {
   if (!d || bad_paged(d)) return 0;
   if (rows_per_head(d) <= kDecodeRows) return decode_parts_bytes((int)rows_per_head(d), (int)d->head_dim);
-  const int parts = paged_parts(d);
-  const int tu = 2 * (128 / (int)(d->n_heads / d->n_kv_heads));
-  const size_t units = (size_t)virtual_tiles(d->total_tokens, d->n_seqs, tu) * d->n_kv_heads * parts;
-  return parts == 1 ? 16 : units * 256 * (d->head_dim + 1) * sizeof(float);
+  return chunk_parts_bytes((int)d->head_dim);
 }
 
 int llmr_attention_paged(llmr_ctx *ctx, const llmr_paged_desc *d, const int32_t *cu_q,
@@ -304,8 +308,7 @@ int llmr_attention_paged(llmr_ctx *ctx, const llmr_paged_desc *d, const int32_t 
     return launch_decode_any(ctx, (int)D, (int)rows_per_head(d), d->dtype, d->out_dtype, p,
                              static_cast<float *>(ctx->ws));
   }
-  return launch_fa_rows_any<true>(ctx, (int)D, d->dtype, d->out_dtype, p, paged_parts(d),
-                                  static_cast<float *>(ctx->ws));
+  return launch_fa_rows_any<true>(ctx, (int)D, d->dtype, d->out_dtype, p);
 }
 
 int llmr_paged_plan(llmr_ctx *ctx, const llmr_plan_desc *d, const int32_t *ctx_lens,

@@ -176,7 +176,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_plan_kernel(const PlanP
 // that both pairings of the rotation, (2i, 2i+1) and (i, i + D/2), stay inside
 // a lane and every access is 16 bytes. A warp takes kRopeSteps rows per
 // group of ONE token, all loads issued before the first use.
-constexpr int kRopeSteps = 4;
+#ifndef ROPE_STEPS
+#define ROPE_STEPS 4
+#endif
+constexpr int kRopeSteps = ROPE_STEPS;
 
 struct PagedRopeParams {
   int tokens, hq, hk, page, num_pages, rope_rows, chunks;  // chunks: warps per token
@@ -210,7 +213,10 @@ __device__ __forceinline__ void store8(T *dst, const float *x) {
 }
 
 template <int D, typename InT, typename OutT, bool HALF>
-__global__ void __launch_bounds__(256) paged_prologue_kernel(const PagedRopeParams p) {
+#ifndef ROPE_MINB
+#define ROPE_MINB 2
+#endif
+__global__ void __launch_bounds__(256, ROPE_MINB) paged_prologue_kernel(const PagedRopeParams p) {
   constexpr int LANES = D / 16, GROUPS = 32 / LANES;
   const int lane = threadIdx.x & 31;
   const int sub = lane % LANES, grp = lane / LANES;
@@ -218,14 +224,10 @@ __global__ void __launch_bounds__(256) paged_prologue_kernel(const PagedRopePara
   const int t = (int)(item / p.chunks);
   if (t >= p.tokens) return;
   const int h0 = (int)(item - (long long)t * p.chunks) * (GROUPS * kRopeSteps);
+  // The slot, the position and the rows are asked for together: a token's
+  // chain is two loads long (its table row comes second).
   const int slot = p.slots[t];
-  if (slot < 0) return;  // padding
   const int pos = p.cos_t ? p.positions[t] : 0;
-  const int pg = slot / p.page, prow = slot - pg * p.page;
-  if (pg >= p.num_pages || pos < 0 || (p.cos_t && pos >= p.rope_rows)) {
-    if (lane == 0) atomicOr(p.err, kErrInput);
-    return;
-  }
   const int first = p.q ? 0 : p.hq;  // rows: hq of Q, hk of K, hk of V
   const int rows = p.hq + 2 * p.hk;
   float x[kRopeSteps][16] = {};
@@ -243,6 +245,12 @@ __global__ void __launch_bounds__(256) paged_prologue_kernel(const PagedRopePara
       load8<InT>(x[s], src + sub * 8);
       load8<InT>(x[s] + 8, src + D / 2 + sub * 8);
     }
+  }
+  if (slot < 0) return;  // padding
+  const int pg = slot / p.page, prow = slot - pg * p.page;
+  if (pg >= p.num_pages || pos < 0 || (p.cos_t && pos >= p.rope_rows)) {
+    if (lane == 0) atomicOr(p.err, kErrInput);
+    return;
   }
   // The token's table row, in the order this lane's elements use it: pair
   // (i, i + D/2) is element i of both halves; pairs (2i, 2i+1) are 4 of the
