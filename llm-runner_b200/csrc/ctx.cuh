@@ -27,9 +27,7 @@ struct llmr_ctx {
   void *ws = nullptr;
   size_t ws_bytes = 0;
   int *d_err = nullptr;
-  // Self-resetting counters: the fused prologue's pieces, or the parts of a
-  // paged-attention row block that have been written.
-  int *d_sync = nullptr;
+  int *d_sync = nullptr;  // fused-prologue piece counters (self-resetting)
   unsigned long long *timeline = nullptr;  // LLMR_TIMELINE builds: event buffer
   uint64_t launches = 0;
   int num_sms = 0;    // SMs the persistent kernels may use (llmr_ctx_set_sm_budget)

@@ -1,5 +1,5 @@
 // Attention of few new tokens per request over a paged cache (one token each
-// when decoding): at most 64 query rows per request and key/value head,
+// when decoding): at most 32 query rows per request and key/value head,
 // row = token * group + head.
 //
 // Bound by HBM: every key and value is read once and meets few rows, so what
@@ -17,11 +17,11 @@
 // 16 rows fill the M of mma.sync (m16n8k16), so the products take that and not
 // tcgen05, whose M = 128 would be spent on a few of its rows. The four warps
 // are RW row tiles of 16 times KW shares of a block's keys: (1, 4) up to 16
-// rows, (2, 2) up to 32, (4, 1) up to 64. Every warp has its own running
+// rows, (2, 2) up to 32. Every warp has its own running
 // maximum and sum and its own O, so none waits for another until a pair's
 // range ends; then the KW shares are joined through shared memory. A pair
-// that the cuts split leaves parts in the workspace, and the CTA that finishes
-// last joins them, in the order of the keys whoever that is.
+// that the cuts split leaves parts in the workspace, which a second launch
+// joins in the order of the keys.
 #pragma once
 #include <type_traits>
 
@@ -29,8 +29,9 @@
 
 namespace llmr {
 
-constexpr int kDecodeCtas = 320;  // upper bound of the grid (workspace, counters)
+constexpr int kDecodeCtas = 320;  // upper bound of the grid (workspace)
 constexpr int kPairBlocks = 2;    // what a pair costs besides its blocks, in blocks
+constexpr int kRangeBlocks = 2;  // least length of a CTA's range
 constexpr int kDecodeBN = 64;     // keys per block
 
 template <int D, int RW>
@@ -53,12 +54,18 @@ struct DecodeCfg {
   static constexpr int PART = ROWS * (D + 2);
 };
 
+// A pair that a cut falls into, entered by the CTA that begins it.
+struct DecodeJoin {
+  int last;  // CTA of its last part; -1: this CTA begins no such pair
+  int row0, nq, kvh;
+};
+
 struct DecodeParams {
   RowsParams rows;
   int group;
   float scale_log2;
-  float *parts;   // [CTA][2][PART]
-  int *counters;  // [CTA], 0 between launches
+  float *parts;       // [CTA][2][PART]
+  DecodeJoin *joins;  // [CTA]
 };
 
 template <typename T>
@@ -147,75 +154,6 @@ __device__ __forceinline__ void finish_row(const DecodeParams &p, const DecodeSe
         none ? -INFINITY : (top + log2f(l)) * 0.69314718055994531f;
 }
 
-// Joins the parts of a pair that CTAs first .. last have left: rows warp,
-// warp + 4, .. for one warp, B of them together, U parts at a time.
-template <int D, int RW, typename OutT, int B, int U>
-__device__ __forceinline__ void join_rows(const DecodeParams &p, const DecodeSeg &sg, int nrows, int first,
-                                          int last, int warp, int lane) {
-  using C = DecodeCfg<D, RW>;
-  constexpr int E = D / 32;
-  typedef typename std::conditional<E == 4, float4, float2>::type Vec;
-  // Part x of the pair: O [ROWS][D], then (max, sum) [ROWS].
-  auto part = [&](int x) {
-    return p.parts + (long long)(2 * (first + x) + (x == 0 ? 1 : 0)) * C::PART;
-  };
-  auto part_ml = [&](int x, int r) {
-    return __ldcg(reinterpret_cast<const float2 *>(part(x) + C::ROWS * D) + r);
-  };
-  const int parts = last - first + 1;
-  for (int r0 = warp; r0 < nrows; r0 += B * C::WARPS) {
-    float top[B], l[B];
-    float acc[B][E] = {};
-#pragma unroll
-    for (int i = 0; i < B; i++) {
-      const int r = min(r0 + i * C::WARPS, nrows - 1);
-      top[i] = -INFINITY;
-      for (int x = lane; x < parts; x += 32) top[i] = fmaxf(top[i], part_ml(x, r).x);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-      l[i] = 0.0f;
-    }
-    for (int x0 = 0; x0 < parts; x0 += 32) {
-      // This lane's part's weight, for all lanes.
-      float w[B];
-#pragma unroll
-      for (int i = 0; i < B; i++) {
-        const int r = min(r0 + i * C::WARPS, nrows - 1);
-        const float2 e = x0 + lane < parts ? part_ml(x0 + lane, r) : make_float2(-INFINITY, 0.0f);
-        w[i] = e.x == -INFINITY ? 0.0f : ex2_approx(e.x - top[i]);
-        l[i] += w[i] * e.y;
-      }
-      const int n = min(32, parts - x0);
-      for (int x = 0; x < n; x += U) {
-        Vec v[U][B];
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-          for (int i = 0; i < B; i++)
-            v[u][i] = __ldcg(reinterpret_cast<const Vec *>(
-                          part(x0 + min(x + u, n - 1)) + min(r0 + i * C::WARPS, nrows - 1) * D) + lane);
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-          for (int i = 0; i < B; i++) {
-            const float f = x + u < n ? __shfl_sync(0xffffffffu, w[i], (x + u) & 31) : 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; e++)
-              if (f != 0.0f) acc[i][e] = fmaf(elem(v[u][i], e), f, acc[i][e]);
-          }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < B; i++) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
-      const int r = r0 + i * C::WARPS;
-      if (r < nrows)
-        finish_row<D, OutT>(p, sg, r, lane * E, *reinterpret_cast<const Vec *>(acc[i]), top[i], l[i]);
-    }
-  }
-}
-
 template <int D, int RW, typename T, typename OutT>
 __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
     fa_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -229,7 +167,6 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::CTL_OFF);
   uint64_t *empty = full + C::NST;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(empty + C::NST);
-  volatile int *last_flag = abort_flag + 1;
   __shared__ long long scan[C::WARPS + 1];
   __shared__ DecodeSeg start;
 
@@ -270,8 +207,11 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
   int mine, row0, nq, nk;
   for (int i0 = 0; i0 < rp.n; i0 += C::THREADS) total += block_scan(i0, incl, mine, row0, nq, nk);
   const long long line = total * rp.Hk;
-  const int ctas = line < (long long)gridDim.x ? (int)line : (int)gridDim.x;
+  const long long most = max(1ll, line / kRangeBlocks);
+  const int ctas = line == 0 ? 0 : most < (long long)gridDim.x ? (int)most : (int)gridDim.x;
   const int cta = blockIdx.x;
+  pdl_launch_dependents();  // the join's CTAs fit beside this kernel's and wait there
+  if (tid == 0) p.joins[cta].last = -1;
   if (cta >= ctas) return;
   const long long lo = range_begin(line, ctas, cta), hi = range_begin(line, ctas, cta + 1);
   {
@@ -519,8 +459,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
       if (whole) {
         finish_row<D, OutT>(p, sg, r, col, acc, top, l);
       } else {
-        __stcg(reinterpret_cast<std::decay_t<decltype(acc)> *>(part + r * D + col), acc);
-        if (col == 0) __stcg(reinterpret_cast<float2 *>(part + C::ROWS * D) + r, make_float2(top, l));
+        *reinterpret_cast<std::decay_t<decltype(acc)> *>(part + r * D + col) = acc;
+        if (col == 0) reinterpret_cast<float2 *>(part + C::ROWS * D)[r] = make_float2(top, l);
       }
     };
     if constexpr (C::KW == 1) {
@@ -577,29 +517,64 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
       }
       named_barrier(1, 32 * C::WARPS);  // merge and ml may be written again
     }
-    if (!whole) {
-      // The pair's parts: CTAs first .. last of the line.
-      const long long b = range_begin(line, ctas, cta) + sg.at + kPairBlocks;
-      const int first = range_owner(line, ctas, b);
-      const int last = range_owner(line, ctas, b + sg.blocks - 1);
-      __threadfence();
-      named_barrier(1, 32 * C::WARPS);
-      if (tid == 0) *last_flag = atomicAdd(p.counters + first, 1) == last - first;
-      named_barrier(1, 32 * C::WARPS);
-      if (*last_flag) {
-        __threadfence();
-        // A warp takes a row (two of many rows) at a time, its lanes the row's
-        // columns; eight parts are asked for before any is used.
-        if (nrows <= C::WARPS)
-          join_rows<D, RW, OutT, 1, 8>(p, sg, nrows, first, last, warp, lane);
-        else
-          join_rows<D, RW, OutT, 2, 4>(p, sg, nrows, first, last, warp, lane);
-        if (tid == 0) p.counters[first] = 0;
-      }
-      named_barrier(1, 32 * C::WARPS);  // last_flag may be written again
+    if (b0 == 0 && !whole && tid == 0) {
+      const long long end = range_begin(line, ctas, cta) + sg.at + kPairBlocks + sg.blocks - 1;
+      p.joins[cta] = DecodeJoin{range_owner(line, ctas, end), sg.row0, sg.nq, sg.kvh};
     }
   } while (advance());
   if (tid == 0 && *abort_flag) atomicOr(rp.err, kErrTimeout);
+}
+
+// Joins the parts of the pairs that cuts fell into: a warp per row, its lanes
+// the row's columns, eight parts asked for before any is used. (Joined by the
+// CTA that finishes last instead, 32 rows of one request over 32768 keys took
+// 62 us, with this launch 37; 64 decodes 88.3 us and 87.2.)
+template <int D, int RW, typename OutT>
+__global__ void __launch_bounds__(128) fa_decode_join_kernel(const __grid_constant__ DecodeParams p) {
+  using C = DecodeCfg<D, RW>;
+  constexpr int E = D / 32, U = 8;
+  typedef typename std::conditional<E == 4, float4, float2>::type Vec;
+  griddep_wait();
+  const int first = blockIdx.x, r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const DecodeJoin join = p.joins[first];
+  if (join.last < 0 || r >= join.nq * p.group) return;
+  // Part x of the pair: O [ROWS][D], then (max, sum) [ROWS].
+  auto part = [&](int x) {
+    return p.parts + (long long)(2 * (first + x) + (x == 0 ? 1 : 0)) * C::PART;
+  };
+  auto part_ml = [&](int x) { return reinterpret_cast<const float2 *>(part(x) + C::ROWS * D)[r]; };
+  const int parts = join.last - first + 1;
+  float top = -INFINITY, l = 0.0f;
+  float acc[E] = {};
+  for (int x = lane; x < parts; x += 32) top = fmaxf(top, part_ml(x).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int x0 = 0; x0 < parts; x0 += 32) {
+    // This lane's part's weight, for all lanes.
+    const float2 e = x0 + lane < parts ? part_ml(x0 + lane) : make_float2(-INFINITY, 0.0f);
+    const float w = e.x == -INFINITY ? 0.0f : ex2_approx(e.x - top);
+    l += w * e.y;
+    const int n = min(32, parts - x0);
+    for (int x = 0; x < n; x += U) {
+      Vec v[U];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        v[u] = *(reinterpret_cast<const Vec *>(part(x0 + min(x + u, n - 1)) + r * D) + lane);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const float f = x + u < n ? __shfl_sync(0xffffffffu, w, (x + u) & 31) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; i++)
+          if (f != 0.0f) acc[i] = fmaf(elem(v[u], i), f, acc[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  DecodeSeg sg = {};
+  sg.row0 = join.row0;
+  sg.kvh = join.kvh;
+  finish_row<D, OutT>(p, sg, r, lane * E, *reinterpret_cast<const Vec *>(acc), top, l);
 }
 
 }  // namespace llmr

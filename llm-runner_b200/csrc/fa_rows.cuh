@@ -48,7 +48,7 @@ constexpr int kMaxRanges = 160;  // CTAs of a paged call (workspace)
 // away from a unit's ends; least keys of a range.
 constexpr int kUnitKeys = 128;
 constexpr int kCutBlocks = 3;
-constexpr int kRangeKeys = 1024;
+constexpr int kRangeKeys = 256;
 
 // A unit that a cut falls into, entered by the CTA that begins it: its parts
 // are that CTA's second part and the first parts of the CTAs up to `last`.
@@ -60,6 +60,7 @@ struct FaJoin {
 struct FaRowsParams {
   RowsParams rows;
   int group, tpt, recip;  // recip: r / group = r * recip >> 16 for r < 128
+  int tu;                 // tokens per unit: tpt or 2 * tpt
   int vtiles;             // prompts: virtual tiles of all requests
   int units;              // prompts: vtiles * Hk
   int dynamic;            // prompts: units are taken over by cluster launch control
@@ -78,6 +79,7 @@ struct FaUnit {
   int pos;         // position of the first token
   int blk;         // first key block
   int nb[2];       // key blocks of each tile
+  int dual;        // the tiles are the same rows, tile 1 with the blocks behind tile 0's
   int part;        // -1, or where the partial result goes
 };
 
@@ -107,17 +109,19 @@ __device__ __forceinline__ void unit_rows(FaUnit &un, int tu, int kvh, int row0,
   un.keys = max(0, un.pos + un.tokens);
   un.part = -1;
 }
-// Key blocks [b0, b1) of the unit, of which tile 0 sees those with its keys.
+// Key blocks [b0, b1) of the unit. Two tiles of tokens see what their last
+// token sees; one tile's rows go to both, each with half of the blocks.
 __device__ __forceinline__ void unit_blocks(FaUnit &un, int tpt, int b0, int b1) {
   const int k0 = max(0, un.pos + min(un.tokens, tpt));
   un.blk = b0;
-  un.nb[0] = max(0, min((k0 + 127) / 128, b1) - b0);
-  un.nb[1] = un.tokens > tpt ? b1 - b0 : 0;
+  un.dual = un.tokens <= tpt;
+  un.nb[0] = un.dual ? (b1 - b0 + 1) / 2 : max(0, min((k0 + 127) / 128, b1) - b0);
+  un.nb[1] = un.dual ? (b1 - b0) / 2 : b1 - b0;
 }
 
 // Prompts: virtual unit u; false if it is empty. Whole warp.
 __device__ __forceinline__ bool prompt_unit(const FaRowsParams &p, int u, FaUnit &un) {
-  const int vt = p.vtiles - 1 - u / p.rows.Hk, tu = 2 * p.tpt;
+  const int vt = p.vtiles - 1 - u / p.rows.Hk, tu = p.tu;
   const int r = find_request(p.rows.cu, p.rows.n, tu, vt);
   int row0, nq, nk;
   if (!request_rows(p.rows, r, row0, nq, nk)) return false;
@@ -164,11 +168,13 @@ struct FaRowsCfg {
   static constexpr int EPI_OFF = KV_OFF + NST * TILE_BYTES;  // 4 KB per softmax warp
   static constexpr int CTL_OFF = EPI_OFF + 8 * 4096;
   // q_full, q_empty, kv_full[NST], kv_empty[NST], s_full[2], p_half[4],
-  // o_full[2], o_empty[2], u_full[], u_empty[], u_ask, clc, drain
-  static constexpr int NBAR = 2 + 2 * NST + 2 + 4 + 2 + 2 + 2 * kUnitSlots + 3;
+  // o_full[2], o_empty[2], u_full[], u_empty[], u_ask, x_full, x_empty, clc,
+  // drain
+  static constexpr int NBAR = 2 + 2 * NST + 2 + 4 + 2 + 2 + 2 * kUnitSlots + 5;
   static constexpr int UNIT_OFF = CTL_OFF + (NBAR * 8 + 15) / 16 * 16;
   static constexpr int CLC_OFF = UNIT_OFF + kUnitSlots * 48;
-  static constexpr int SMEM_BYTES = CLC_OFF + 32 + 1024;
+  static constexpr int X_OFF = CLC_OFF + 32;  // tile 1's (max, sum) of 128 rows for tile 0
+  static constexpr int SMEM_BYTES = X_OFF + 1024 + 1024;
   static constexpr int THREADS = 384;
   static constexpr int REG_SOFTMAX = 200, REG_OTHER = 104, REG_LAUNCH = 168;
   static constexpr int REG_NEED = 2 * 128 * REG_SOFTMAX + 128 * REG_OTHER;
@@ -192,7 +198,7 @@ __device__ __forceinline__ void find_range(const FaRowsParams &p, uint8_t *smem,
   const RowsParams &rp = p.rows;
   long long *sums = reinterpret_cast<long long *>(smem);  // [WARPS]
   FaCut *cuts = reinterpret_cast<FaCut *>(smem + 128);     // [2]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tu = 2 * p.tpt;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tu = p.tu;
   int row0 = 0, nq = 0, nk = 0;
   long long mine = 0, incl = 0, total = 0;
   auto block_scan = [&](int i0) {
@@ -260,7 +266,7 @@ template <typename Give>
 __device__ __forceinline__ void walk_range(const FaRowsParams &p, const FaCut &lo, const FaCut &hi,
                                            long long line, int ranges, Give give) {
   const RowsParams &rp = p.rows;
-  const int tu = 2 * p.tpt, c = blockIdx.x;
+  const int tu = p.tu, c = blockIdx.x;
   FaJoin join{-1, 0, 0, 0};
   FaUnit un;
   int i = 0, row0 = 0, nq = 0, nk = 0;
@@ -329,11 +335,14 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t *u_full = o_empty + 2;
   uint64_t *u_empty = u_full + kUnitSlots;
   uint64_t *u_ask = u_empty + kUnitSlots;
-  uint64_t *clc_bar = u_ask + 1;
+  uint64_t *x_full = u_ask + 1;
+  uint64_t *x_empty = x_full + 1;
+  uint64_t *clc_bar = x_empty + 1;
   uint64_t *drain = clc_bar + 1;
   auto unit_slot = [&](int i) {
     return reinterpret_cast<FaUnit *>(smem + C::UNIT_OFF + (i % kUnitSlots) * 48);
   };
+  float2 *exchange = reinterpret_cast<float2 *>(smem + C::X_OFF);
   void *clc_resp = smem + C::CLC_OFF;
   uint32_t *tmem_base_slot = reinterpret_cast<uint32_t *>(smem + C::CLC_OFF + 16);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_base_slot + 1);
@@ -358,6 +367,8 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(&u_empty[i], 10);  // producer, MMA issuer, 8 softmax warps
     }
     mbar_init(u_ask, 1);
+    mbar_init(x_full, 4);
+    mbar_init(x_empty, 4);
     mbar_init(clc_bar, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -374,6 +385,7 @@ __global__ void __launch_bounds__(384, 1)
   FaCut lo, hi;
   long long line = 0;
   int ranges = 1;
+  if constexpr (PAGED) pdl_launch_dependents();  // the join comes as soon as an SM is free
   if constexpr (PAGED) find_range(p, smem + C::EPI_OFF, lo, hi, line, ranges);
 
   // A whole warp's wait; all lanes get the same answer, also when it is given up.
@@ -424,22 +436,28 @@ __global__ void __launch_bounds__(384, 1)
         // Lane l loads box l: rows (l / NCHUNK) * box_rows on, columns (l % NCHUNK) * 64 on.
         const int pc = lane / C::NCHUNK, cc = lane - pc * C::NCHUNK;
         const int *trow = PAGED ? p.rows.table + (long long)un.kv_row * p.rows.table_stride : nullptr;
-        auto page_at = [&](int j) {  // page of this lane's box in block j, or 0
-          const int key = (un.blk + j) * C::BN + (pc << log_box);
-          return PAGED && j < nblk && (pc << log_box) < C::BN && key < un.keys ? trow[key >> log_page]
-                                                                               : 0;
+        auto page_at = [&](int b, bool on) {  // page of this lane's box in key block b, or 0
+          const int key = b * C::BN + (pc << log_box);
+          return PAGED && on && (pc << log_box) < C::BN && key < un.keys ? trow[key >> log_page] : 0;
         };
-        int page = page_at(0);
+        // Step j loads K then V of block blk + j, and, if the tiles have blocks
+        // of their own, of tile 1's block with either.
+        const int ways = un.dual ? 2 : 1, blk1 = un.blk + un.nb[0];
+        int page[2] = {page_at(un.blk, true), page_at(blk1, un.dual && un.nb[1] > 0)};
         for (int j = 0; j < nblk && ok; j++) {
-          const int next_page = page_at(j + 1);
-          const int key0 = (un.blk + j) * C::BN;
-          const int valid = min(C::BN, un.keys - key0);
-          const int boxes = PAGED ? ((valid + box_rows - 1) >> log_box) * C::NCHUNK : C::NCHUNK;
-          if (PAGED && lane < boxes && (unsigned)page >= (unsigned)p.rows.num_pages) {
-            atomicOr(p.rows.err, kErrInput);  // the map reads zeros there
-            page = p.rows.num_pages;
-          }
-          for (int kind = 0; kind < 2; kind++) {
+          const int next[2] = {page_at(un.blk + j + 1, j + 1 < nblk),
+                               page_at(blk1 + j + 1, un.dual && j + 1 < un.nb[1])};
+          for (int load = 0; load < 2 * ways; load++) {
+            const int kind = load / ways, way = load - kind * ways;
+            if (way == 1 && j >= un.nb[1]) continue;
+            const int key0 = ((way ? blk1 : un.blk) + j) * C::BN;
+            const int valid = min(C::BN, un.keys - key0);
+            const int boxes = PAGED ? ((valid + box_rows - 1) >> log_box) * C::NCHUNK : C::NCHUNK;
+            int pg = way ? page[1] : page[0];
+            if (PAGED && lane < boxes && (unsigned)pg >= (unsigned)p.rows.num_pages) {
+              atomicOr(p.rows.err, kErrInput);  // the map reads zeros there
+              pg = p.rows.num_pages;
+            }
             const int slot = issued % C::NST, round = issued / C::NST;
             if (round > 0 && !(ok = wait(&kv_empty[slot], round - 1))) break;
             if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], boxes * box_rows * 128);
@@ -449,13 +467,14 @@ __global__ void __launch_bounds__(384, 1)
               uint8_t *dst = sKV + slot * C::TILE_BYTES + cc * C::CHUNK_BYTES + (pc << log_box) * 128;
               if (PAGED)
                 tma_load_4d(dst, m, &kv_full[slot], cc * 64,
-                            (key0 + (pc << log_box)) & (p.rows.page - 1), un.kvh, page);
+                            (key0 + (pc << log_box)) & (p.rows.page - 1), un.kvh, pg);
               else
                 tma_load_4d(dst, m, &kv_full[slot], cc * 64, un.kv_row + key0, un.kvh, 0);
             }
             issued++;
           }
-          page = next_page;
+          page[0] = next[0];
+          page[1] = next[1];
         }
         if (!ok) break;
         if (lane == 0) mbar_arrive(u_ask);  // the unit's loads are under way
@@ -472,8 +491,8 @@ __global__ void __launch_bounds__(384, 1)
       constexpr uint32_t IDESC_S = idesc_mma_f32(128, C::BN, FMT, 0);
       constexpr uint32_t IDESC_O = idesc_mma_f32(128, D, FMT, 1);
       const uint32_t sQa = smem_u32(sQ), sKVa = smem_u32(sKV);
-      auto issue_s = [&](int t, int slot) {
-        const uint32_t qa = sQa + t * C::TILE_BYTES, ka = sKVa + slot * C::TILE_BYTES;
+      auto issue_s = [&](int t, int qt, int slot) {
+        const uint32_t qa = sQa + qt * C::TILE_BYTES, ka = sKVa + slot * C::TILE_BYTES;
 #pragma unroll
         for (int kk = 0; kk < D / 16; kk++) {
           const uint32_t off = (kk >> 2) * C::CHUNK_BYTES + (kk & 3) * 32;
@@ -492,78 +511,117 @@ __global__ void __launch_bounds__(384, 1)
       for (int i = 0; ok && next_unit(i, un); i++) {
         const int nblk = max(un.nb[0], un.nb[1]);
         if (nblk == 0) continue;
-        ok = wait(q_full, kq) && wait(&kv_full[ring % C::NST], ring / C::NST);
+        if (!(ok = wait(q_full, kq))) break;
         kq++;
-        if (!ok) break;
-        tc_fence_after();
-        for (int t = 0; t < 2; t++)
-          if (un.nb[t] > 0) issue_s(t, ring % C::NST);
-        if (elect_one()) mma_commit(&kv_empty[ring % C::NST]);
-        if (nblk == 1 && elect_one()) mma_commit(q_empty);
-        for (int j = 0; j < nblk && ok; j++) {
-          const int uV = ring + 2 * j + 1, sV = uV % C::NST;
-          const int uK = uV + 1, sK = uK % C::NST;
-          const bool more = j + 1 < nblk;
-          if (!(ok = wait(&kv_full[sV], uV / C::NST))) break;
-          const uint32_t va = sKVa + sV * C::TILE_BYTES;
-          const int left = un.keys - (un.blk + j) * C::BN;  // keys of this block that any row sees
-          if (left < C::BN && (left & 15)) {
-            // Rows of V up to the next multiple of 16 take part with P = 0.
-            const int n = (16 - (left & 15)) * 8 * C::NCHUNK;
-            for (int x = lane; x < n; x += 32) {
-              const int c = x / (n / C::NCHUNK), y = x - c * (n / C::NCHUNK);
-              *reinterpret_cast<uint4 *>(sKV + sV * C::TILE_BYTES + c * C::CHUNK_BYTES + left * 128 +
-                                         y * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
+        // Rows of V behind the last key, up to the next multiple of 16, take
+        // part with P = 0 and may hold anything: they are zeroed.
+        auto zero_tail = [&](int slot, int left) {
+          if (left >= C::BN || !(left & 15)) return;
+          const int n = (16 - (left & 15)) * 8 * C::NCHUNK;
+          for (int x = lane; x < n; x += 32) {
+            const int c = x / (n / C::NCHUNK), y = x - c * (n / C::NCHUNK);
+            *reinterpret_cast<uint4 *>(sKV + slot * C::TILE_BYTES + c * C::CHUNK_BYTES + left * 128 +
+                                       y * 16) = make_uint4(0, 0, 0, 0);
           }
-          bool k_ready = false;
-          for (int t = 0; t < 2 && ok; t++) {
-            if (j < un.nb[t]) {
-              // O_t is overwritten by the unit's first product: the previous
-              // epilogue must have read it.
-              if (j == 0 && cu[t] > 0 && !(ok = wait(&o_empty[t], cu[t] - 1))) break;
-              // 16-key steps that some row of this tile sees.
-              const int seen = un.pos + min(un.tokens, (t + 1) * p.tpt) - (un.blk + j) * C::BN;
-              const int steps = min((min(seen, left) + 15) >> 4, C::BN / 16);
-              for (int half = 0; half < 2; half++) {
-                if (!(ok = wait(&p_half[2 * t + half], cp[t]))) break;
-                tc_fence_after();
+          fence_proxy_async_smem();
+          __syncwarp();
+        };
+        // O_t (+)= P_t V of step j, its first `steps` groups of 16 keys.
+        auto issue_o = [&](int t, int slot, int j, int steps) {
+          const uint32_t va = sKVa + slot * C::TILE_BYTES;
+          for (int half = 0; half < 2; half++) {
+            if (!wait(&p_half[2 * t + half], cp[t])) return false;
+            tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < C::BN / 32; kk++) {
-                  const int ks = half * (C::BN / 32) + kk;
-                  if (ks < steps && elect_one())
-                    mma_ts(tmem + C::O_COL + t * D, tmem + t * 128 + ks * 8,
-                           sdesc_sw128(va + ks * 2048, C::CHUNK_BYTES, 1024), IDESC_O,
-                           (j > 0 || ks > 0) ? 1u : 0u);
+            for (int kk = 0; kk < C::BN / 32; kk++) {
+              const int ks = half * (C::BN / 32) + kk;
+              if (ks < steps && elect_one())
+                mma_ts(tmem + C::O_COL + t * D, tmem + t * 128 + ks * 8,
+                       sdesc_sw128(va + ks * 2048, C::CHUNK_BYTES, 1024), IDESC_O,
+                       (j > 0 || ks > 0) ? 1u : 0u);
+            }
+          }
+          cp[t]++;
+          return true;
+        };
+        auto last_o = [&](int t) {
+          if (elect_one()) mma_commit(&o_full[t]);
+          cu[t]++;
+        };
+        if (!un.dual) {
+          // Step j reads K_j, V_j for both tiles; tile 0 may end before tile 1.
+          if (!(ok = wait(&kv_full[ring % C::NST], ring / C::NST))) break;
+          tc_fence_after();
+          for (int t = 0; t < 2; t++)
+            if (un.nb[t] > 0) issue_s(t, t, ring % C::NST);
+          if (elect_one()) mma_commit(&kv_empty[ring % C::NST]);
+          if (nblk == 1 && elect_one()) mma_commit(q_empty);
+          for (int j = 0; j < nblk && ok; j++) {
+            const int uV = ring + 2 * j + 1, sV = uV % C::NST;
+            const int uK = uV + 1, sK = uK % C::NST;
+            if (!(ok = wait(&kv_full[sV], uV / C::NST))) break;
+            const int key0 = (un.blk + j) * C::BN, left = un.keys - key0;
+            zero_tail(sV, left);
+            bool k_ready = false;
+            for (int t = 0; t < 2 && ok; t++) {
+              if (j < un.nb[t]) {
+                // O_t is overwritten by the unit's first product: the previous
+                // epilogue must have read it.
+                if (j == 0 && cu[t] > 0 && !(ok = wait(&o_empty[t], cu[t] - 1))) break;
+                // 16-key steps that some row of this tile sees.
+                const int seen = un.pos + min(un.tokens, (t + 1) * p.tpt) - key0;
+                if (!(ok = issue_o(t, sV, j, min((min(seen, left) + 15) >> 4, C::BN / 16)))) break;
+                if (j + 1 == un.nb[t]) last_o(t);
+              }
+              if (j + 1 < un.nb[t]) {
+                if (!k_ready) {
+                  if (!(ok = wait(&kv_full[sK], uK / C::NST))) break;
+                  tc_fence_after();
+                  k_ready = true;
                 }
-              }
-              if (!ok) break;
-              cp[t]++;
-              if (j + 1 == un.nb[t]) {
-                if (elect_one()) mma_commit(&o_full[t]);
-                cu[t]++;
+                issue_s(t, t, sK);
               }
             }
-            if (j + 1 < un.nb[t]) {
-              if (!k_ready) {
-                if (!(ok = wait(&kv_full[sK], uK / C::NST))) break;
-                tc_fence_after();
-                k_ready = true;
-              }
-              issue_s(t, sK);
+            if (!ok) break;
+            if (elect_one()) mma_commit(&kv_empty[sV]);
+            if (j + 1 < nblk) {
+              if (elect_one()) mma_commit(&kv_empty[sK]);
+              // The unit's last S MMAs are issued: Q may be replaced after them.
+              if (j + 2 == nblk && elect_one()) mma_commit(q_empty);
             }
           }
-          if (!ok) break;
-          if (elect_one()) mma_commit(&kv_empty[sV]);
-          if (more) {
-            if (elect_one()) mma_commit(&kv_empty[sK]);
-            // The unit's last S MMAs are issued: Q may be replaced after them.
-            if (j + 2 == nblk && elect_one()) mma_commit(q_empty);
+          ring += 2 * nblk;
+        } else {
+          // Step j reads K0 K1 V0 V1, or K0 V0 in the last of an odd number.
+          auto score = [&](int t, int j) {
+            const int u = ring + 4 * j + t, slot = u % C::NST;
+            if (!wait(&kv_full[slot], u / C::NST)) return false;
+            tc_fence_after();
+            issue_s(t, 0, slot);
+            if (elect_one()) mma_commit(&kv_empty[slot]);
+            return true;
+          };
+          for (int t = 0; t < 2 && ok; t++)
+            if (un.nb[t] > 0) ok = score(t, 0);
+          if (ok && nblk == 1 && elect_one()) mma_commit(q_empty);
+          for (int j = 0; j < nblk && ok; j++) {
+            for (int t = 0; t < 2 && ok; t++) {
+              if (j < un.nb[t]) {
+                const int u = ring + 4 * j + (j < un.nb[1] ? 2 + t : 1), sV = u % C::NST;
+                if (!(ok = wait(&kv_full[sV], u / C::NST))) break;
+                const int left = un.keys - (un.blk + j + (t ? un.nb[0] : 0)) * C::BN;
+                zero_tail(sV, left);
+                if (j == 0 && cu[t] > 0 && !(ok = wait(&o_empty[t], cu[t] - 1))) break;
+                if (!(ok = issue_o(t, sV, j, min((left + 15) >> 4, C::BN / 16)))) break;
+                if (elect_one()) mma_commit(&kv_empty[sV]);
+                if (j + 1 == un.nb[t]) last_o(t);
+              }
+              if (j + 1 < un.nb[t]) ok = score(t, j + 1);
+            }
+            if (ok && j + 2 == nblk && elect_one()) mma_commit(q_empty);
           }
+          ring += 2 * (un.nb[0] + un.nb[1]);
         }
-        ring += 2 * nblk;
       }
       // Every MMA this warp issued has completed before TMEM is released.
       if (elect_one()) mma_commit(drain);
@@ -629,7 +687,7 @@ __global__ void __launch_bounds__(384, 1)
     const uint32_t tO = tmem + lane_off + C::O_COL + t * D;
     const float sl2 = p.scale_log2;
     bool ok = true;
-    int cs = 0, cu = 0;  // key blocks and units of this tile so far
+    int cs = 0, cu = 0, cx = 0;  // key blocks and units of this tile, dual units so far
     for (int i = 0; ok; i++) {
       // The unit's slot is kept until its epilogue is done, which reads it
       // again: a row of scores leaves few registers.
@@ -641,8 +699,9 @@ __global__ void __launch_bounds__(384, 1)
       // query are not masked.
       int valid = 0x3fffffff;
       {
-        const int tok = row * p.recip >> 16;
-        if (tok < min(un.tokens - t * p.tpt, p.tpt)) valid = un.pos + t * p.tpt + tok + 1 - un.blk * C::BN;
+        const int tok = row * p.recip >> 16, t0 = un.dual ? 0 : t * p.tpt;  // the tile's first token
+        const int b0 = un.blk + (un.dual && t ? un.nb[0] : 0);
+        if (tok < min(un.tokens - t0, p.tpt)) valid = un.pos + t0 + tok + 1 - b0 * C::BN;
       }
       float m_used = -INFINITY;  // log2-domain max the P values are relative to
       float l = 0.0f;
@@ -736,13 +795,48 @@ __global__ void __launch_bounds__(384, 1)
         cu++;
         tc_fence_after();
       }
+      // Dual: tile 1 leaves its maximum and sum, and its O in TMEM, to tile 0.
+      float w0 = 1.0f, w1 = 0.0f;  // weights of the own and of tile 1's O
+      const bool joint = un.dual && t == 0;
+      const int nblk1 = joint ? un.nb[1] : 0;
+      if (un.dual) {
+        if (t == 1) {
+          if (cx > 0 && !(ok = wait(x_empty, cx - 1))) break;
+          exchange[row] = make_float2(m_used, l);
+          // (its O is complete: o_full was waited for)
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(x_full);
+            mbar_arrive(&u_empty[i % kUnitSlots]);
+          }
+          cx++;
+          continue;
+        }
+        if (!(ok = wait(x_full, cx))) break;
+        tc_fence_after();
+        const float2 other = exchange[row];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(x_empty);
+        cx++;
+        const float top = fmaxf(m_used, other.x);
+        if (top != -INFINITY) {
+          w0 = ex2_approx(m_used - top);
+          w1 = ex2_approx(other.x - top);
+          l = l * w0 + other.y * w1;
+          m_used = top;
+        }
+      }
       const bool none = m_used == -INFINITY;  // no key
       const float inv = none ? 0.0f : 1.0f / l;
       const float lse = none ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
+      w0 *= inv;
+      w1 *= inv;
       const int tok = row * p.recip >> 16, head = row - tok * p.group;
-      const int ntok = min(un.tokens - t * p.tpt, p.tpt);  // tokens of this tile (<= 0: none)
+      const int t0 = un.dual ? 0 : t * p.tpt;          // the tile's first token
+      const int ntok = min(un.tokens - t0, p.tpt);  // its tokens (<= 0: none)
       const bool live = tok < ntok;
-      const int kvh = un.kvh, q_row = un.q_row + t * p.tpt;  // the tile's first token
+      const int kvh = un.kvh, q_row = un.q_row + t0;
       const int part_at = un.part;
       __syncwarp();
       if (lane == 0) mbar_arrive(&u_empty[i % kUnitSlots]);
@@ -763,8 +857,19 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
 #pragma unroll
-        for (int x = 0; x < 32; x++)
-          v[x] = none ? 0.0f : __uint_as_float(o[x]) * inv;
+        for (int x = 0; x < 32; x++) v[x] = none ? 0.0f : __uint_as_float(o[x]) * w0;
+        if (nblk1 > 0) {
+          tmem_ld32(tO + D + c * 32, o);
+          tmem_wait_ld();
+          reg_fence32(o);
+          if (c == D / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty[1]);
+          }
+#pragma unroll
+          for (int x = 0; x < 32; x++) v[x] = w1 > 0.0f ? fmaf(__uint_as_float(o[x]), w1, v[x]) : v[x];
+        }
       };
       if (part_at >= 0) {
         const long long r = (long long)part_at * 256 + t * 128 + row;

@@ -13,7 +13,7 @@ int launch_decode(llmr_ctx *ctx, const RowsParams &r, float *parts) {
   p.group = r.H / r.Hk;
   p.scale_log2 = r.scale * 1.4426950408889634f;
   p.parts = parts;
-  p.counters = ctx->d_sync;
+  p.joins = reinterpret_cast<DecodeJoin *>(parts + (size_t)kDecodeCtas * 2 * C::PART);
   CUtensorMap mk, mv;
   int rc;
   if ((rc = make_map16(ctx, &mk, r.k, {D, r.page, r.Hk, r.num_pages}, {r.ks[1], r.ks[2], r.ks[0]},
@@ -26,7 +26,19 @@ int launch_decode(llmr_ctx *ctx, const RowsParams &r, float *parts) {
   const int want = 2 * ctx->num_sms;
   const int grid = want < kDecodeCtas ? want : kDecodeCtas;
   kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mk, mv, p);
-  return after_launch(ctx, "fa_decode");
+  if ((rc = after_launch(ctx, "fa_decode"))) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, (r.max_q * p.group + 3) / 4);
+  cfg.blockDim = dim3(128);
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto join = fa_decode_join_kernel<D, RW, OutT>;
+  CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, join, p));
+  return after_launch(ctx, "fa_decode_join");
 }
 
 template <int D, int RW>
@@ -46,16 +58,13 @@ int launch_decode_any(llmr_ctx *ctx, int D, int rows, llmr_dtype dt, llmr_dtype 
   if (rows <= 16)
     return D == 128 ? launch_decode_t<128, 1>(ctx, dt, od, r, parts)
                     : launch_decode_t<64, 1>(ctx, dt, od, r, parts);
-  if (rows <= 32)
-    return D == 128 ? launch_decode_t<128, 2>(ctx, dt, od, r, parts)
-                    : launch_decode_t<64, 2>(ctx, dt, od, r, parts);
-  return D == 128 ? launch_decode_t<128, 4>(ctx, dt, od, r, parts)
-                  : launch_decode_t<64, 4>(ctx, dt, od, r, parts);
+  return D == 128 ? launch_decode_t<128, 2>(ctx, dt, od, r, parts)
+                  : launch_decode_t<64, 2>(ctx, dt, od, r, parts);
 }
 
 size_t decode_parts_bytes(int rows, int D) {
-  const size_t r = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  return (size_t)kDecodeCtas * 2 * r * (D + 2) * sizeof(float);
+  const size_t r = rows <= 16 ? 16 : 32;
+  return (size_t)kDecodeCtas * (2 * r * (D + 2) * sizeof(float) + sizeof(DecodeJoin));
 }
 
 }  // namespace llmr
