@@ -338,10 +338,11 @@ int llmr_paged_plan(llmr_ctx *ctx, const llmr_plan_desc *d, const int32_t *ctx_l
                         (const void *)kv_lens, (const void *)positions, (const void *)slots,
                         (const void *)n_free_out})
     if (!a4(x)) return fail(ctx, LLMR_EINVAL, "an array is misaligned");
-  PlanParams p;
+  PlanParams p = {};
   p.n = (int)d->n_seqs;
   p.max_tokens = (int)d->max_tokens;
   p.page = (int)d->page_size;
+  while ((1 << p.log_page) < p.page) p.log_page++;
   p.num_pages = (int)d->num_pages;
   p.free_cap = (int)d->free_capacity;
   p.max_pages = (int)d->max_pages;
@@ -357,11 +358,11 @@ int llmr_paged_plan(llmr_ctx *ctx, const llmr_plan_desc *d, const int32_t *ctx_l
   p.slots = slots;
   p.n_free_out = n_free_out;
   p.err = ctx->d_err;
-  // One CTA until there is work for two rounds of its threads.
-  const long long items = (long long)d->max_tokens + d->n_seqs;
+  // One CTA until there is work for a second round of its threads.
+  const long long items = d->max_tokens > d->n_seqs ? d->max_tokens : d->n_seqs;
   const int threads = items <= 256 ? 256 : kPlanThreads;
   int ctas = 1;
-  while (ctas < 8 && items > 2ll * ctas * threads) ctas *= 2;
+  while (ctas < 8 && items > (long long)ctas * threads) ctas *= 2;
   const int smem = (3 * p.n + 2) * (int)sizeof(int);
   CUDA_TRY(ctx, set_smem_once(paged_plan_kernel, (3 * kPlanMaxSeqs + 2) * (int)sizeof(int)));
   cudaLaunchConfig_t cfg = {};
