@@ -603,13 +603,16 @@ def _rows(t, name: str, code, tokens: int, heads: int, dim: int, device: int):
     """(row stride, head stride) of a [tokens, heads, dim] tensor with dense elements."""
     if t.shape != (tokens, heads, dim):
         _refuse(f"{name} is {tuple(t.shape)}, not {(tokens, heads, dim)}")
-    st = t.stride()
-    if st[2] != 1 and tokens:
+    row, head, elem = t.stride()
+    if elem != 1 and tokens:
         _refuse(f"{name}: elements of a row must be dense")
-    if code is not None and _code(t, name) != code:
+    if code is not None and _TYPES[t.dtype] != code:
         _refuse(f"{name}: dtype {t.dtype} differs")
-    _place(t, name, device)
-    return _step(tokens, st[0]), _step(heads, st[1])
+    if t.get_device() != device:
+        _misplaced(name, device)
+    if tokens > 1 and heads > 1 and row > 0 and head > 0:
+        return row, head
+    return _step(tokens, row), _step(heads, head)
 
 
 def _out_rows(t, name: str, tokens: int, heads: int, dim: int, device: int):
@@ -617,14 +620,14 @@ def _out_rows(t, name: str, tokens: int, heads: int, dim: int, device: int):
     if t.dim() == 2:
         if t.shape != (tokens, heads * dim) or (tokens and t.stride(1) != 1):
             _refuse(f"{name} must be [{tokens}, {heads * dim}] or [{tokens}, {heads}, {dim}], dense rows")
-        _place(t, name, device)
+        if t.get_device() != device:
+            _misplaced(name, device)
         return _step(tokens, t.stride(0)), 0
     return _rows(t, name, None, tokens, heads, dim, device)
 
 
-def _place(t, name: str, device: int) -> None:
-    if t.get_device() != device:  # -1 on the host
-        _refuse(f"{name} must be on cuda:{device}")
+def _misplaced(name: str, device: int):  # get_device() is -1 on the host
+    _refuse(f"{name} must be on cuda:{device}")
 
 
 def _vector(t, name: str, length: int, device: int, kind="int32") -> None:
@@ -632,7 +635,13 @@ def _vector(t, name: str, length: int, device: int, kind="int32") -> None:
         _refuse(f"{name} must be a dense vector of {length}")
     if _TYPES[t.dtype] != kind:
         _refuse(f"{name} must be {'fp32' if kind == F32 else kind}, not {t.dtype}")
-    _place(t, name, device)
+    if t.get_device() != device:
+        _misplaced(name, device)
+
+
+def _at(t):
+    """The address of a tensor, or None."""
+    return None if t is None else t.data_ptr()
 
 
 def _lse(lse, heads: int, tokens: int, device: int) -> None:
@@ -640,7 +649,8 @@ def _lse(lse, heads: int, tokens: int, device: int) -> None:
         return
     if lse.shape != (heads, tokens) or not lse.is_contiguous() or _TYPES[lse.dtype] != F32:
         _refuse(f"lse must be fp32 [{heads}, {tokens}], dense")
-    _place(lse, "lse", device)
+    if lse.get_device() != device:
+        _misplaced("lse", device)
 
 
 def _query(q, name_k: str, kv_heads: int):
@@ -660,15 +670,16 @@ def _query(q, name_k: str, kv_heads: int):
 
 def _cache(t, name: str, code: int, shape, device: int):
     """(page, row, head) strides of a cache."""
-    if t.shape != shape or not t.numel():
+    if t.shape != shape or 0 in shape:
         _refuse(f"{name} is {tuple(t.shape)}, not {tuple(shape)}")
-    st = t.stride()
-    if st[3] != 1:
+    page, row, head, elem = t.stride()
+    if elem != 1:
         _refuse(f"{name}: elements of a row must be dense")
-    if _code(t, name) != code:
+    if _TYPES[t.dtype] != code:
         _refuse(f"{name}: dtype {t.dtype} differs")
-    _place(t, name, device)
-    return _step(shape[0], st[0]), _step(shape[1], st[1]), _step(shape[2], st[2])
+    if t.get_device() != device:
+        _misplaced(name, device)
+    return _step(shape[0], page), _step(shape[1], row), _step(shape[2], head)
 
 
 def _table(block_table, n: int, device: int):
@@ -679,7 +690,8 @@ def _table(block_table, n: int, device: int):
     st = block_table.stride()
     if rows != n or cols < 1 or (cols > 1 and st[1] != 1):
         _refuse(f"block_table must be [{n}, max_pages] with dense rows")
-    _place(block_table, "block_table", device)
+    if block_table.get_device() != device:
+        _misplaced("block_table", device)
     return cols, _step(rows, st[0])
 
 
@@ -707,7 +719,7 @@ def attention_causal(ctx: Context, q, k, v, o, cu_seqlens, *, scale: float, lse=
     d = CausalDesc(n, t, h, hk, dim, code, _code(o, "o"), scale, qr, kr, vr, orow, qh, kh, vh, oh)
     ctx.check(lib.llmr_attention_causal(ctx.handle, ctypes.byref(d), cu_seqlens.data_ptr(),
                                         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                                        _ptr(lse)))
+                                        _at(lse)))
 
 
 def attention_paged_workspace_bytes(*, n_seqs: int, total_tokens: int, max_q_len: int,
@@ -752,7 +764,7 @@ def attention_paged(ctx: Context, q, k_cache, v_cache, o, cu_q, kv_lens, block_t
     ctx.check(lib.llmr_attention_paged(ctx.handle, ctypes.byref(d), cu_q.data_ptr(),
                                        kv_lens.data_ptr(), block_table.data_ptr(), q.data_ptr(),
                                        k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
-                                       _ptr(lse)))
+                                       _at(lse)))
 
 
 def paged_plan(ctx: Context, ctx_lens, new_lens, free_pages, n_free, block_table, cu_q, kv_lens,
@@ -828,7 +840,8 @@ def paged_prologue(ctx: Context, q, k, v, q_out, k_cache, v_cache, positions, sl
         for x in (cos, sin):
             if x.shape != (rows, dim // 2) or not x.is_contiguous() or _TYPES[x.dtype] != F32:
                 _refuse(f"cos and sin must be fp32 [rows, {dim // 2}]")
-            _place(x, "cos and sin", dev)
+            if x.get_device() != dev:
+                _misplaced("cos and sin", dev)
         if positions is None:
             _refuse("cos and sin need positions")
         flags = (ROPE | ROPE_HALF) if half else ROPE
@@ -844,10 +857,10 @@ def paged_prologue(ctx: Context, q, k, v, q_out, k_cache, v_cache, positions, sl
         flags |= NORM_K
     d = PagedPrologueDesc(t, h, hk, dim, code_in, code, flags, eps, page, pages, rows, qr, kr, vr,
                           orow, qh, kh, vh, oh, *kc, *vc)
-    ctx.check(lib.llmr_paged_prologue(ctx.handle, ctypes.byref(d), _ptr(positions),
-                                      slots.data_ptr(), _ptr(q), k.data_ptr(), v.data_ptr(),
-                                      _ptr(q_gain), _ptr(k_gain), _ptr(cos), _ptr(sin),
-                                      _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr()))
+    ctx.check(lib.llmr_paged_prologue(ctx.handle, ctypes.byref(d), _at(positions),
+                                      slots.data_ptr(), _at(q), k.data_ptr(), v.data_ptr(),
+                                      _at(q_gain), _at(k_gain), _at(cos), _at(sin),
+                                      _at(q_out), k_cache.data_ptr(), v_cache.data_ptr()))
 
 
 # --------------------------------------------------------------------- peer buffers
