@@ -46,7 +46,7 @@ constexpr int kUnitSlots = 2;  // the unit in work and the next
 constexpr int kMaxRanges = 160;  // CTAs of a paged call (workspace)
 // What a unit costs besides its keys, in keys; blocks of 128 that a cut keeps
 // away from a unit's ends; least keys of a range.
-constexpr int kUnitKeys = 128;
+constexpr int kUnitKeys = 256;
 constexpr int kCutBlocks = 3;
 constexpr int kRangeKeys = 256;
 
@@ -167,10 +167,10 @@ struct FaRowsCfg {
   static constexpr int KV_OFF = 2 * TILE_BYTES;
   static constexpr int EPI_OFF = KV_OFF + NST * TILE_BYTES;  // 4 KB per softmax warp
   static constexpr int CTL_OFF = EPI_OFF + 8 * 4096;
-  // q_full, q_empty, kv_full[NST], kv_empty[NST], s_full[2], p_half[4],
+  // q_full[2], q_empty[2], kv_full[NST], kv_empty[NST], s_full[2], p_half[4],
   // o_full[2], o_empty[2], u_full[], u_empty[], u_ask, x_full, x_empty, clc,
   // drain
-  static constexpr int NBAR = 2 + 2 * NST + 2 + 4 + 2 + 2 + 2 * kUnitSlots + 5;
+  static constexpr int NBAR = 4 + 2 * NST + 2 + 4 + 2 + 2 + 2 * kUnitSlots + 5;
   static constexpr int UNIT_OFF = CTL_OFF + (NBAR * 8 + 15) / 16 * 16;
   static constexpr int CLC_OFF = UNIT_OFF + kUnitSlots * 48;
   static constexpr int X_OFF = CLC_OFF + 32;  // tile 1's (max, sum) of 128 rows for tile 0
@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(384, 1)
   uint8_t *smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
   uint8_t *sQ = smem, *sKV = smem + C::KV_OFF;
   uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + C::CTL_OFF);
-  uint64_t *q_empty = q_full + 1;
-  uint64_t *kv_full = q_full + 2;
+  uint64_t *q_empty = q_full + 2;  // Q tiles take the two places in turn
+  uint64_t *kv_full = q_full + 4;
   uint64_t *kv_empty = kv_full + C::NST;
   uint64_t *s_full = kv_empty + C::NST;
   uint64_t *p_half = s_full + 2;   // [t * 2 + half]
@@ -349,8 +349,10 @@ __global__ void __launch_bounds__(384, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
     for (int i = 0; i < C::NST; i++) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
@@ -422,17 +424,24 @@ __global__ void __launch_bounds__(384, 1)
           if (lane == 0) mbar_arrive(u_ask);
           continue;
         }
-        if (kq > 0 && !(ok = wait(q_empty, kq - 1))) break;
-        if (lane == 0) {
+        auto load_q = [&]() {
           const int tiles = un.tokens > p.tpt ? 2 : 1;
-          const int bytes = p.group * p.tpt * 128;  // per box
-          mbar_arrive_expect_tx(q_full, tiles * C::NCHUNK * bytes);
-          for (int t = 0; t < tiles; t++)
-            for (int c = 0; c < C::NCHUNK; c++)
-              tma_load_4d(sQ + t * C::TILE_BYTES + c * C::CHUNK_BYTES, &tmQ, q_full, c * 64, 0,
-                          un.q_row + t * p.tpt, un.kvh);
-        }
-        kq++;
+          for (int t = 0; t < tiles; t++, kq++) {
+            const int slot = kq & 1;
+            if (kq > 1 && !wait(&q_empty[slot], (kq >> 1) - 1)) return false;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&q_full[slot], C::NCHUNK * p.group * p.tpt * 128);
+              for (int c = 0; c < C::NCHUNK; c++)
+                tma_load_4d(sQ + slot * C::TILE_BYTES + c * C::CHUNK_BYTES, &tmQ, &q_full[slot], c * 64, 0,
+                            un.q_row + t * p.tpt, un.kvh);
+            }
+          }
+          return true;
+        };
+        // The first unit's Q goes ahead of its K and V; a later one's place may
+        // still be in use, so its first K does not wait for that.
+        const bool q_first = kq == 0;
+        if (q_first && !(ok = load_q())) break;
         // Lane l loads box l: rows (l / NCHUNK) * box_rows on, columns (l % NCHUNK) * 64 on.
         const int pc = lane / C::NCHUNK, cc = lane - pc * C::NCHUNK;
         const int *trow = PAGED ? p.rows.table + (long long)un.kv_row * p.rows.table_stride : nullptr;
@@ -450,6 +459,7 @@ __global__ void __launch_bounds__(384, 1)
           for (int load = 0; load < 2 * ways; load++) {
             const int kind = load / ways, way = load - kind * ways;
             if (way == 1 && j >= un.nb[1]) continue;
+            if (j == 0 && load == ways && !q_first && !(ok = load_q())) break;  // behind the K
             const int key0 = ((way ? blk1 : un.blk) + j) * C::BN;
             const int valid = min(C::BN, un.keys - key0);
             const int boxes = PAGED ? ((valid + box_rows - 1) >> log_box) * C::NCHUNK : C::NCHUNK;
@@ -481,7 +491,8 @@ __global__ void __launch_bounds__(384, 1)
       }
       if (*abort_flag && lane == 0) {
         // Abort path: let every armed copy land before the CTA exits.
-        if (kq > 0) mbar_wait_raw(q_full, (kq - 1) & 1, 100000000ull);
+        for (int u = kq - 2 < 0 ? 0 : kq - 2; u < kq; u++)
+          mbar_wait_raw(&q_full[u & 1], (u >> 1) & 1, 100000000ull);
         for (int u = issued - C::NST < 0 ? 0 : issued - C::NST; u < issued; u++)
           mbar_wait_raw(&kv_full[u % C::NST], (u / C::NST) & 1, 100000000ull);
       }
@@ -490,29 +501,43 @@ __global__ void __launch_bounds__(384, 1)
       constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
       constexpr uint32_t IDESC_S = idesc_mma_f32(128, C::BN, FMT, 0);
       constexpr uint32_t IDESC_O = idesc_mma_f32(128, D, FMT, 1);
-      const uint32_t sQa = smem_u32(sQ), sKVa = smem_u32(sKV);
-      auto issue_s = [&](int t, int qt, int slot) {
-        const uint32_t qa = sQa + qt * C::TILE_BYTES, ka = sKVa + slot * C::TILE_BYTES;
+      // One lane issues everything. A step inside a tile, or to another tile,
+      // adds to the descriptor's address field (16-byte units), so a group of
+      // MMAs costs its issuer little more than the instructions themselves.
+      const bool leader = elect_one();
+      const uint64_t q_desc = sdesc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc = sdesc_sw128(smem_u32(sKV), 16, 1024);
+      const uint64_t v_desc = sdesc_sw128(smem_u32(sKV), C::CHUNK_BYTES, 1024);
+      constexpr uint32_t TILE = C::TILE_BYTES >> 4;
+      auto commit = [&](uint64_t *bar) {
+        if (leader) mma_commit(bar);
+      };
+      // S of Q place qt and the K in `slot`, into buffer b.
+      auto issue_s = [&](int b, int qt, int slot) {
+        if (leader) {
+          const uint64_t qd = q_desc + qt * TILE, kd = k_desc + slot * TILE;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; kk++) {
-          const uint32_t off = (kk >> 2) * C::CHUNK_BYTES + (kk & 3) * 32;
-          if (elect_one())
-            mma_ss(tmem + t * 128, sdesc_sw128(qa + off, 16, 1024),
-                   sdesc_sw128(ka + off, 16, 1024), IDESC_S, kk > 0);
+          for (int kk = 0; kk < D / 16; kk++) {
+            const uint32_t off = ((kk >> 2) * C::CHUNK_BYTES + (kk & 3) * 32) >> 4;
+            mma_ss(tmem + b * 128, qd + off, kd + off, IDESC_S, kk > 0);
+          }
+          mma_commit(&s_full[b]);
         }
-        if (elect_one()) mma_commit(&s_full[t]);
       };
       bool ok = true;
       int ring = 0;           // K/V tiles of this CTA's earlier units
-      int kq = 0;             // units with a Q load so far
+      int kq = 0;             // Q tiles so far
       int cp[2] = {0, 0};     // key blocks of tile t so far
       int cu[2] = {0, 0};     // units of tile t so far
       FaUnit un;
       for (int i = 0; ok && next_unit(i, un); i++) {
         const int nblk = max(un.nb[0], un.nb[1]);
         if (nblk == 0) continue;
-        if (!(ok = wait(q_full, kq))) break;
-        kq++;
+        // The Q tiles' places, taken in turn.
+        const int tiles = un.dual ? 1 : 2, qs[2] = {kq & 1, (kq + 1) & 1};
+        for (int t = 0; t < tiles && ok; t++) ok = wait(&q_full[(kq + t) & 1], (kq + t) >> 1);
+        if (!ok) break;
+        kq += tiles;
         // Rows of V behind the last key, up to the next multiple of 16, take
         // part with P = 0 and may hold anything: they are zeroed.
         auto zero_tail = [&](int slot, int left) {
@@ -528,34 +553,37 @@ __global__ void __launch_bounds__(384, 1)
         };
         // O_t (+)= P_t V of step j, its first `steps` groups of 16 keys.
         auto issue_o = [&](int t, int slot, int j, int steps) {
-          const uint32_t va = sKVa + slot * C::TILE_BYTES;
+          const uint64_t vd = v_desc + slot * TILE;
+          const uint32_t o = tmem + C::O_COL + t * D, pt = tmem + t * 128;
           for (int half = 0; half < 2; half++) {
             if (!wait(&p_half[2 * t + half], cp[t])) return false;
             tc_fence_after();
+            if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < C::BN / 32; kk++) {
-              const int ks = half * (C::BN / 32) + kk;
-              if (ks < steps && elect_one())
-                mma_ts(tmem + C::O_COL + t * D, tmem + t * 128 + ks * 8,
-                       sdesc_sw128(va + ks * 2048, C::CHUNK_BYTES, 1024), IDESC_O,
-                       (j > 0 || ks > 0) ? 1u : 0u);
+              for (int kk = 0; kk < C::BN / 32; kk++) {
+                const int ks = half * (C::BN / 32) + kk;
+                if (ks < steps)
+                  mma_ts(o, pt + ks * 8, vd + (ks * 2048 >> 4), IDESC_O, (j > 0 || ks > 0) ? 1u : 0u);
+              }
             }
+            __syncwarp();
           }
           cp[t]++;
           return true;
         };
         auto last_o = [&](int t) {
-          if (elect_one()) mma_commit(&o_full[t]);
+          commit(&o_full[t]);
           cu[t]++;
         };
         if (!un.dual) {
           // Step j reads K_j, V_j for both tiles; tile 0 may end before tile 1.
           if (!(ok = wait(&kv_full[ring % C::NST], ring / C::NST))) break;
           tc_fence_after();
-          for (int t = 0; t < 2; t++)
-            if (un.nb[t] > 0) issue_s(t, t, ring % C::NST);
-          if (elect_one()) mma_commit(&kv_empty[ring % C::NST]);
-          if (nblk == 1 && elect_one()) mma_commit(q_empty);
+          for (int t = 0; t < 2; t++) {
+            if (un.nb[t] > 0) issue_s(t, qs[t], ring % C::NST);
+            if (un.nb[t] <= 1) commit(&q_empty[qs[t]]);  // its last S
+          }
+          commit(&kv_empty[ring % C::NST]);
           for (int j = 0; j < nblk && ok; j++) {
             const int uV = ring + 2 * j + 1, sV = uV % C::NST;
             const int uK = uV + 1, sK = uK % C::NST;
@@ -579,16 +607,13 @@ __global__ void __launch_bounds__(384, 1)
                   tc_fence_after();
                   k_ready = true;
                 }
-                issue_s(t, t, sK);
+                issue_s(t, qs[t], sK);
+                if (j + 2 == un.nb[t]) commit(&q_empty[qs[t]]);
               }
             }
             if (!ok) break;
-            if (elect_one()) mma_commit(&kv_empty[sV]);
-            if (j + 1 < nblk) {
-              if (elect_one()) mma_commit(&kv_empty[sK]);
-              // The unit's last S MMAs are issued: Q may be replaced after them.
-              if (j + 2 == nblk && elect_one()) mma_commit(q_empty);
-            }
+            commit(&kv_empty[sV]);
+            if (j + 1 < nblk) commit(&kv_empty[sK]);
           }
           ring += 2 * nblk;
         } else {
@@ -597,13 +622,13 @@ __global__ void __launch_bounds__(384, 1)
             const int u = ring + 4 * j + t, slot = u % C::NST;
             if (!wait(&kv_full[slot], u / C::NST)) return false;
             tc_fence_after();
-            issue_s(t, 0, slot);
-            if (elect_one()) mma_commit(&kv_empty[slot]);
+            issue_s(t, qs[0], slot);
+            commit(&kv_empty[slot]);
             return true;
           };
           for (int t = 0; t < 2 && ok; t++)
             if (un.nb[t] > 0) ok = score(t, 0);
-          if (ok && nblk == 1 && elect_one()) mma_commit(q_empty);
+          if (ok && nblk == 1) commit(&q_empty[qs[0]]);
           for (int j = 0; j < nblk && ok; j++) {
             for (int t = 0; t < 2 && ok; t++) {
               if (j < un.nb[t]) {
@@ -613,18 +638,18 @@ __global__ void __launch_bounds__(384, 1)
                 zero_tail(sV, left);
                 if (j == 0 && cu[t] > 0 && !(ok = wait(&o_empty[t], cu[t] - 1))) break;
                 if (!(ok = issue_o(t, sV, j, min((left + 15) >> 4, C::BN / 16)))) break;
-                if (elect_one()) mma_commit(&kv_empty[sV]);
+                commit(&kv_empty[sV]);
                 if (j + 1 == un.nb[t]) last_o(t);
               }
               if (j + 1 < un.nb[t]) ok = score(t, j + 1);
             }
-            if (ok && j + 2 == nblk && elect_one()) mma_commit(q_empty);
+            if (ok && j + 2 == nblk) commit(&q_empty[qs[0]]);
           }
           ring += 2 * (un.nb[0] + un.nb[1]);
         }
       }
       // Every MMA this warp issued has completed before TMEM is released.
-      if (elect_one()) mma_commit(drain);
+      commit(drain);
       mbar_wait_raw(drain, 0, 100000000ull);
     } else if (warp == 10) {
       // --------------------------------------------------------- scheduler
