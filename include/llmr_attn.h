@@ -452,7 +452,8 @@ int llmr_rope_tables(const int32_t *pos, uint32_t seq_len, uint32_t n_axes,
  * lse: fp32 [n_heads][total_tokens] natural-log sum-exp, or NULL. Scores,
  * softmax and sums are fp32; the softmax numerators enter the second product
  * in the inputs' type. A non-finite element of k or v reaches no sequence
- * but its own; within it, one in v may reach up to 127 rows before it. */
+ * but its own, and no row before it, except that one in v may reach the up to
+ * 142 rows before it. o overlaps none of the inputs. No workspace. */
 typedef struct {
   uint32_t n_seqs, total_tokens, n_heads, n_kv_heads, head_dim;
   llmr_dtype dtype;     /* of q, k, v: LLMR_F16 or LLMR_BF16 */
@@ -474,7 +475,7 @@ int llmr_attention_causal(llmr_ctx *ctx, const llmr_causal_desc *desc,
  * behind the last request are left as they were. What a page holds behind a
  * request's last key may be anything, NaN included. max_q_len bounds the
  * rows of any request (and picks the kernel). page_size: 16, 32, 64, 128 or
- * 256. lse as above. */
+ * 256. lse, non-finite elements and o as above. */
 typedef struct {
   uint32_t n_seqs, total_tokens, max_q_len, n_heads, n_kv_heads, head_dim;
   llmr_dtype dtype;     /* of q and the caches: LLMR_F16 or LLMR_BF16 */

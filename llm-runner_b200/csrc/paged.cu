@@ -109,7 +109,7 @@ int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r) {
     // 1500 tokens, 14 / 2 heads of 64: 20.1 us instead of 28.1; with more units
     // than SMs reading K and V for one tile costs more than that gains (1500
     // tokens, 32 / 8 heads of 128: 39 us instead of 35).
-    if ((long long)r.tokens / (2 * p.tpt) * r.Hk < ctx->num_sms) p.tu = p.tpt;
+    if ((long long)r.tokens / (2 * p.tpt) * r.Hk < ctx->total_sms) p.tu = p.tpt;
     const long long vt = (long long)r.tokens / p.tu + r.n, units = vt * r.Hk;
     if (units > 0x7fffffffLL) return fail(ctx, LLMR_EINVAL, "problem too large");
     p.vtiles = (int)vt;
@@ -408,6 +408,7 @@ int llmr_paged_prologue(llmr_ctx *ctx, const llmr_paged_prologue_desc *d,
     return fail(ctx, LLMR_EINVAL, "LLMR_ROPE needs cos/sin tables and positions");
   if (d->rope_rows > 0x7fffffffu) return fail(ctx, LLMR_EINVAL, "problem too large");
   const long long D = d->head_dim, H = d->n_heads, Hk = d->n_kv_heads, P = d->page_size;
+  if ((long long)d->total_tokens * (H + 2 * Hk) > (1ll << 33)) return fail(ctx, LLMR_EINVAL, "problem too large");
   PagedRopeParams p = {};
   p.tokens = (int)d->total_tokens;
   p.hq = (int)H;

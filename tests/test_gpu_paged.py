@@ -131,6 +131,22 @@ def test_causal_neighbours_do_not_leak(ctx):
     assert torch.equal(o[keep.cuda()], clean[keep.cuda()])
 
 
+@pytest.mark.parametrize("h,hk,d", [(128, 1, 64), (100, 1, 128), (65, 1, 64), (128, 2, 128)])
+def test_causal_large_groups(ctx, h, hk, d):
+    """One to two tokens per query tile, rows of the tile left over."""
+    run_causal(ctx, [70, 3], h, hk, d, BF16, BF16, pad=1, seed=h)
+
+
+def test_an_sm_budget_changes_no_result():
+    own = L.Context(0)
+    whole = run_causal(own, [900, 200], 16, 4, 128, BF16, BF16, seed=2)
+    own.set_sm_budget(7)
+    assert torch.equal(run_causal(own, [900, 200], 16, 4, 128, BF16, BF16, seed=2), whole)
+    for q in (1, 90):
+        Paged([q] * 5, [300, 2000, q, 700, 1500], 8, 2, 128, 32, BF16, seed=q).check(own)
+    own.close()
+
+
 def test_causal_same_bits_twice(ctx):
     a = run_causal(ctx, [700, 3, 250], 8, 2, 128, BF16, BF16, seed=1)
     b = run_causal(ctx, [700, 3, 250], 8, 2, 128, BF16, BF16, seed=1)
@@ -296,6 +312,53 @@ def test_many_requests(ctx):
     g = torch.Generator().manual_seed(3)
     kv = torch.randint(0, 400, (700,), generator=g).tolist()
     Paged([1] * 700, kv, 4, 2, 64, 16, F16, seed=1).check(ctx)
+
+
+def test_many_chunks(ctx):
+    """More requests than a CTA scans at once, some without rows."""
+    g = torch.Generator().manual_seed(4)
+    kv = torch.randint(20, 300, (900,), generator=g).tolist()
+    q = [17 * (i % 5 > 0) for i in range(900)]
+    Paged(q, kv, 4, 2, 64, 16, F16, seed=1).check(ctx)
+
+
+@pytest.mark.parametrize("q", [1, 3])
+@pytest.mark.parametrize("h,hk", [(128, 1), (100, 1), (33, 1), (32, 1)])
+def test_paged_large_groups(ctx, q, h, hk):
+    Paged([q, q], [700, 90], h, hk, 64, 16, BF16, seed=q).check(ctx)
+
+
+@pytest.mark.parametrize("q", [1, 100])
+def test_two_contexts_at_once(q):
+    """Calls of two contexts on two streams, each with its own workspace."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [L.Context(0, stream=s) for s in streams]
+    cases = [Paged([q] * 3, [3000, 900, 5000], 8, 2, 128, 16, BF16, seed=i) for i in range(2)]
+    alone = [c.run(x).clone() for c, x in zip(cases, ctxs)]
+    torch.cuda.synchronize()
+    outs = [torch.zeros_like(a) for a in alone]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, x, o in zip(cases, ctxs, outs):
+            L.attention_paged(x, c.q, c.kc, c.vc, o, c.cu, c.kv, c.table, scale=c.d ** -0.5, max_q_len=q)
+    for x in ctxs:
+        x.sync()
+    assert all(torch.equal(a, b) for a, b in zip(alone, outs))
+    for x in ctxs:
+        x.close()
+
+
+def test_shared_pages(ctx):
+    """Requests whose tables name the same pages (a common prefix)."""
+    p = Paged([1, 1, 1], [640, 700, 666], 8, 2, 128, 64, BF16, seed=3)
+    for i in (1, 2):
+        p.table[i, :10] = p.table[0, :10]
+        p.k[i][:640], p.v[i][:640] = p.k[0], p.v[0]
+    p.check(ctx)
+    p = Paged([50, 50], [640, 700], 8, 2, 128, 64, BF16, seed=3)
+    p.table[1, :9] = p.table[0, :9]
+    p.k[1][:576], p.v[1][:576] = p.k[0][:576], p.v[0][:576]
+    p.check(ctx)
 
 
 def test_cache_beyond_32_bit_offsets(ctx):
