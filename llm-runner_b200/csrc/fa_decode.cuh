@@ -125,9 +125,8 @@ struct DecodeSeg {
 // A request's length in the line per key/value head: its blocks (one for rows
 // without a key: they are written too) and kPairBlocks; 0 for a request without
 // rows.
-__device__ __forceinline__ int decode_blocks(const RowsParams &p, int r, int &row0, int &nq, int &nk) {
-  if (!request_rows(p, r, row0, nq, nk) || nq == 0) return 0;
-  return max(1, (nk + kDecodeBN - 1) / kDecodeBN) + kPairBlocks;
+__device__ __forceinline__ int decode_blocks(bool ok, int nq, int nk) {
+  return ok && nq > 0 ? max(1, (nk + kDecodeBN - 1) / kDecodeBN) + kPairBlocks : 0;
 }
 
 // Row r of a pair, columns col ..: acc / l to the output, and the row's
@@ -181,12 +180,28 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
     fence_barrier_init();
   }
   // ------------------------------------------------ the line of blocks, my range
-  // Sum of the requests' lengths in [i0, i0 + THREADS), and this thread's
-  // inclusive prefix within it.
-  auto block_scan = [&](int i0, long long &incl, int &mine, int &row0, int &nq, int &nk) {
-    const int r = i0 + tid;
-    mine = r < rp.n ? decode_blocks(rp, r, row0, nq, nk) : 0;
-    incl = mine;
+  // Each thread takes R neighbouring requests: the sum of all lengths from i0
+  // on (STRIDE requests), and the place of this thread's first.
+  constexpr int R = 4, STRIDE = R * C::THREADS;
+  int size[R], row0[R], nq[R], nk[R];
+  auto block_scan = [&](int i0, long long &begin) {
+    int a[R], e[R], k[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int r = min(i0 + tid * R + i, rp.n - 1);
+      a[i] = rp.cu[r];
+      e[i] = rp.cu[r + 1];
+      k[i] = rp.kv_lens[r];
+    }
+    long long mine = 0;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      size[i] = i0 + tid * R + i < rp.n
+                    ? decode_blocks(check_rows(rp, a[i], e[i], k[i], row0[i], nq[i], nk[i]), nq[i], nk[i])
+                    : 0;
+      mine += size[i];
+    }
+    long long incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long x = __shfl_up_sync(0xffffffffu, incl, o);
@@ -201,11 +216,11 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
       if (w == warp) incl += sum;
       sum += scan[w];
     }
+    begin = incl - mine;
     return sum;
   };
-  long long incl, total = 0;
-  int mine, row0, nq, nk;
-  for (int i0 = 0; i0 < rp.n; i0 += C::THREADS) total += block_scan(i0, incl, mine, row0, nq, nk);
+  long long begin, total = 0;
+  for (int i0 = 0; i0 < rp.n; i0 += STRIDE) total += block_scan(i0, begin);
   const long long line = total * rp.Hk;
   const long long most = max(1ll, line / kRangeBlocks);
   const int ctas = line == 0 ? 0 : most < (long long)gridDim.x ? (int)most : (int)gridDim.x;
@@ -216,19 +231,24 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
   const long long lo = range_begin(line, ctas, cta), hi = range_begin(line, ctas, cta + 1);
   {
     long long before = 0;
-    for (int i0 = 0; i0 < rp.n; i0 += C::THREADS) {
+    for (int i0 = 0; i0 < rp.n; i0 += STRIDE) {
       long long sum = total;
-      if (rp.n > C::THREADS) sum = block_scan(i0, incl, mine, row0, nq, nk);
-      // Requests lie end to end as [before + incl - mine, before + incl) * Hk.
-      const long long b = (before + incl - mine) * rp.Hk;
-      if (mine > 0 && b <= lo && lo < (before + incl) * rp.Hk) {
-        start.r = i0 + tid;
-        start.row0 = row0;
-        start.nq = nq;
-        start.nk = nk;
-        start.blocks = mine - kPairBlocks;
-        start.kvh = (int)((lo - b) / mine);
-        start.at = (int)(b + (long long)start.kvh * mine - lo);
+      if (rp.n > STRIDE) sum = block_scan(i0, begin);
+      // Requests lie end to end, each rp.Hk times its length.
+      long long b = (before + begin) * rp.Hk;
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const long long e = b + (long long)size[i] * rp.Hk;
+        if (b <= lo && lo < e) {
+          start.r = i0 + tid * R + i;
+          start.row0 = row0[i];
+          start.nq = nq[i];
+          start.nk = nk[i];
+          start.blocks = size[i] - kPairBlocks;
+          start.kvh = (int)((lo - b) / size[i]);
+          start.at = (int)(b + (long long)start.kvh * size[i] - lo);
+        }
+        b = e;
       }
       before += sum;
       if (before * rp.Hk > lo) break;
@@ -250,7 +270,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
     if (++sg.kvh < rp.Hk) return true;
     sg.kvh = 0;
     while (++sg.r < rp.n) {
-      sg.blocks = decode_blocks(rp, sg.r, sg.row0, sg.nq, sg.nk) - kPairBlocks;
+      const bool ok = request_rows(rp, sg.r, sg.row0, sg.nq, sg.nk);
+      sg.blocks = decode_blocks(ok, sg.nq, sg.nk) - kPairBlocks;
       if (sg.blocks > 0) return true;
     }
     return false;

@@ -26,7 +26,7 @@
 //   warp 8           TMA producer: Q, then K_j, V_j into an NST-slot ring
 //   warp 9           MMA issuer and TMEM owner
 //   warp 10          scheduler: finds the units, one ahead
-//   warp 11          CTA 0: looks through all requests for bad lengths
+//   warp 11          prompts, CTA 0: looks through all sequences for bad offsets
 // MMA order per key block j: PV0_j, S0_{j+1}, PV1_j, S1_{j+1}, each tile with
 // its own number of blocks. The first blocks need no mask; in those that reach
 // past a row's last key the scores are set to -inf (so P is exactly 0), P V
@@ -699,8 +699,8 @@ __global__ void __launch_bounds__(384, 1)
           hand_out(i);
         }
       }
-    } else if (blockIdx.x == 0) {
-      check_requests(p.rows, lane, 32);
+    } else if (!PAGED && blockIdx.x == 0) {
+      check_requests(p.rows, lane);  // (find_range has looked at all of them)
     }
   } else {
     reg_alloc<C::REG_SOFTMAX>();

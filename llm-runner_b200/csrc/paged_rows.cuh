@@ -32,19 +32,22 @@ struct RowsParams {
   int *err;
 };
 
-// Request r's rows, checked; false (and the error bit) if its offsets or
-// lengths are out of range.
-__device__ __forceinline__ bool request_rows(const RowsParams &p, int r, int &row0, int &nq,
-                                             int &nk) {
-  const int end = p.cu[r + 1];
-  row0 = p.cu[r];
-  const bool in = 0 <= row0 && row0 <= end && end <= p.tokens;
-  nq = in ? end - row0 : 0;
-  nk = p.paged ? p.kv_lens[r] : nq;
+// A request's rows from its offsets and length, checked; false (and the error
+// bit) if they are out of range.
+__device__ __forceinline__ bool check_rows(const RowsParams &p, int begin, int end, int keys, int &row0, int &nq,
+                                           int &nk) {
+  const bool in = 0 <= begin && begin <= end && end <= p.tokens;
+  row0 = begin;
+  nq = in ? end - begin : 0;
+  nk = p.paged ? keys : nq;
   const bool ok = in && nk >= 0 &&
                   (!p.paged || (nk <= (long long)p.max_pages * p.page && nq <= p.max_q));
   if (!ok) atomicOr(p.err, kErrInput);
   return ok;
+}
+__device__ __forceinline__ bool request_rows(const RowsParams &p, int r, int &row0, int &nq,
+                                             int &nk) {
+  return check_rows(p, p.cu[r], p.cu[r + 1], p.paged ? p.kv_lens[r] : 0, row0, nq, nk);
 }
 
 // The few-rows kernel's launch and the workspace of its parts (paged_decode.cu).
@@ -70,11 +73,22 @@ inline int make_map16(llmr_ctx *ctx, CUtensorMap *map, const void *base, const l
   return LLMR_OK;
 }
 
-// Reports requests that no row would lead to: one CTA's `count` threads look
-// at all of them.
-__device__ __forceinline__ void check_requests(const RowsParams &p, int first, int count) {
-  int row0, nq, nk;
-  for (int r = first; r < p.n; r += count) request_rows(p, r, row0, nq, nk);
+// Reports sequences that no row would lead to: one warp looks at all offsets,
+// eight at a time.
+__device__ __forceinline__ void check_requests(const RowsParams &p, int lane) {
+  bool bad = false;
+  for (int r0 = lane; r0 < p.n; r0 += 256) {
+    int a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int r = min(r0 + i * 32, p.n - 1);
+      a[i] = p.cu[r];
+      b[i] = p.cu[r + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) bad |= a[i] < 0 || a[i] > b[i] || b[i] > p.tokens;
+  }
+  if (bad) atomicOr(p.err, kErrInput);
 }
 
 }  // namespace llmr
