@@ -7,10 +7,13 @@
 // tokens still fills a tile, and the triangle wastes little: only blocks that
 // some row of the tile sees are visited.
 //
-// Work unit: (request, key/value head, 2 * tpt tokens[, part of the keys]).
+// Work unit: (request, key/value head, 2 * tpt tokens[, part of the keys]): two
+// tiles, whose softmax and MMAs overlap. A unit of one tile (a short chunk, or
+// all units where there are few) gives both softmax groups the same rows, each
+// with half of the keys; tile 0's group joins the two at the end.
 // Requests' offsets are device data, so each CTA finds its units itself.
 //  * Prompts: units are numbered without knowing the offsets. Request i
-//    starts at virtual tile cu[i] / (2 tpt) + i, which leaves room for its tiles
+//    starts at virtual tile cu[i] / tu + i, which leaves room for its tiles
 //    and at most one empty one behind them, and is found by searching cu. Units
 //    are handed out last tokens first (the longest rows first), by cluster
 //    launch control: a CTA takes over units whose CTAs have not started, so no
@@ -33,6 +36,14 @@
 // stops at the last key rounded up to 16, and the V rows in between are
 // zeroed in shared memory: what lies behind a request's keys may be NaN.
 //
+// Bound by the tensor pipe at the rate of M = 128, N = 128 instructions (about
+// 68 % of dense) where there are many blocks: 8192 tokens, 32 / 8 heads of 128
+// in 451 us = 1220 TFLOP/s of the causal flops; heads of 64 in 376 us (P V of
+// N = 64 costs what N = 128 does). The issuing lane must not add to that: with a
+// descriptor built and a lane elected per instruction the same took 481 and
+// 411 us. 6 chunks of 300 - 700 tokens behind 2k - 12k keys: 267 us. Bound by its
+// start and the unit boundary (8.2 us for 77 tokens) where there are few.
+//
 // Scores and softmax state are fp32, P is rounded to the inputs' type (half
 // a step, the rounding V's own type has; fp32 P would need a tf32 product at
 // a quarter of the rate), and the row sum takes P before that rounding.
@@ -44,8 +55,11 @@ namespace llmr {
 
 constexpr int kUnitSlots = 2;  // the unit in work and the next
 constexpr int kMaxRanges = 160;  // CTAs of a paged call (workspace)
-// What a unit costs besides its keys, in keys; blocks of 128 that a cut keeps
-// away from a unit's ends; least keys of a range.
+// What a unit costs besides its keys, in keys (128 to 512 differ by 3 %);
+// blocks of 128 that a cut keeps away from a unit's ends (a part costs about
+// two blocks to write and join; 6 took 200 tokens over 1500 keys from 32 to
+// 41 us); least keys of a range (with 1024, 20 tokens over 100 keys, 8 small
+// units, ran on two SMs: 24.6 us instead of 14).
 constexpr int kUnitKeys = 256;
 constexpr int kCutBlocks = 3;
 constexpr int kRangeKeys = 256;
@@ -751,11 +765,11 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
         for (int x = 0; x < 128; x += 2)
           mx[(x >> 1) & 3] = max3f(mx[(x >> 1) & 3], __uint_as_float(sbuf[x]), __uint_as_float(sbuf[x + 1]));
-        // The max moves only when this block passes it by more than kMaxExp.
+        // The max moves only when this block's P would pass 2^kMaxExp.
         const float m_new = max3f(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl2;
         const bool need = m_new > m_used + kMaxExp;
         if (__any_sync(0xffffffffu, need)) {
-          const float m_tgt = need ? m_new : m_used;
+          const float m_tgt = need ? m_new - kHeadroom : m_used;
           const float factor = need ? ex2_approx(m_used - m_tgt) : 1.0f;
           l *= factor;
           if (j > 0) {

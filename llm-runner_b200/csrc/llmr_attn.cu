@@ -664,7 +664,7 @@ int llmr_sync(llmr_ctx *ctx) {
     }
     if (h & kErrInput)
       return fail(ctx, LLMR_EINVAL, "a length, offset, slot, position or page in device memory is "
-                                    "out of range; the requests it belongs to were skipped");
+                                    "out of range; the rows of its request are invalid");
     return fail(ctx, LLMR_ENOMEM, "the free list holds fewer pages than the step needs; nothing "
                                   "was planned");
   }

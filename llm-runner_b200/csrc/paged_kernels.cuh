@@ -16,8 +16,8 @@ namespace llmr {
 // prefixes of n and need over the requests give every token and every fresh
 // page its place, so tokens and pages are then written independently of one
 // another: page x of the step (request order) is free_pages[n_free - 1 - x].
-// Latency is all that counts (a decode step moves a few KB), so it is one
-// launch: a cluster of 1 to 8 CTAs, each of which scans all requests itself
+// Latency is all that counts (a decode step moves a few KB: 256 requests 4.6 us,
+// 48 prompts of 96k tokens 8.9 us), so it is one launch: a cluster of 1 to 8 CTAs, each of which scans all requests itself
 // (cheaper than handing the prefixes over) and writes its share of the tokens
 // and pages. All reads of arrays that may be written in place come before the
 // cluster barrier, all writes after it.
@@ -213,7 +213,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_plan_kernel(const PlanP
 // a row as 8 elements of its first half and the 8 elements D/2 further on, so
 // that both pairings of the rotation, (2i, 2i+1) and (i, i + D/2), stay inside
 // a lane and every access is 16 bytes. A warp takes kRopeSteps rows per
-// group of ONE token, all loads issued before the first use.
+// group of ONE token, all loads issued before the first use. 8191 tokens, 32 / 8
+// heads of 128: 49 us, 4.2 TB/s. 4 rows per group and two CTAs per SM took 64 us, 1
+// and six 55, 2 and five 73 (spills), 2 and three 53.
 constexpr int kRopeSteps = 2;
 
 struct PagedRopeParams {

@@ -50,6 +50,12 @@ __device__ __forceinline__ bool request_rows(const RowsParams &p, int r, int &ro
   return check_rows(p, p.cu[r], p.cu[r + 1], p.paged ? p.kv_lens[r] : 0, row0, nq, nk);
 }
 
+// Softmax numerators are taken relative to 2^-kHeadroom times the maximum that
+// was current when they began: the largest is 2^kHeadroom then, and fp16 keeps
+// its 11 bits down to 2^-(14 + kHeadroom) of it. The maximum moves, and O and the
+// sum are rescaled, when a score would pass 2^15, the most an fp16 P may hold.
+constexpr float kHeadroom = 6.0f;
+
 // The few-rows kernel's launch and the workspace of its parts (paged_decode.cu).
 int launch_decode_any(llmr_ctx *ctx, int D, int rows, llmr_dtype dt, llmr_dtype od, const RowsParams &r,
                       float *parts);
