@@ -38,10 +38,10 @@
 //
 // Bound by the tensor pipe at the rate of M = 128, N = 128 instructions (about
 // 68 % of dense) where there are many blocks: 8192 tokens, 32 / 8 heads of 128
-// in 451 us = 1220 TFLOP/s of the causal flops; heads of 64 in 376 us (P V of
+// in 445 us = 1235 TFLOP/s of the causal flops; heads of 64 in 366 us (P V of
 // N = 64 costs what N = 128 does). The issuing lane must not add to that: with a
 // descriptor built and a lane elected per instruction the same took 481 and
-// 411 us. 6 chunks of 300 - 700 tokens behind 2k - 12k keys: 267 us. Bound by its
+// 411 us (with part of the exponentials on the FMA pipe, which costs 3 %). 6 chunks of 300 - 700 tokens behind 2k - 12k keys: 267 us. Bound by its
 // start and the unit boundary (8.2 us for 77 tokens) where there are few.
 //
 // Scores and softmax state are fp32, P is rounded to the inputs' type (half
@@ -786,42 +786,32 @@ __global__ void __launch_bounds__(384, 1)
           }
           m_used = m_tgt;
         }
-        // P = 2^(s*scale*log2e - m). A quarter of the pairs of a block without
-        // a mask runs on the FMA pipe; that routine does not reach 0.
+        // P = 2^(s*scale*log2e - m), every one by ex2 (the non-causal kernel takes
+        // a quarter on the FMA pipe; here that costs 3 %: 8192 tokens 458 us
+        // instead of 445, and a masked score would not reach 0 there).
         uint64_t part2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
         const uint64_t sl2x2 = f2_pack(sl2, sl2);
         const float m_sub = m_used == -INFINITY ? 0.0f : m_used;  // no key so far: all P are 0
         const uint64_t neg_mx2 = f2_pack(-m_sub, -m_sub);
-        auto write_p = [&](auto poly) {
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            const float *v = reinterpret_cast<const float *>(sbuf + c * 32);
-            uint32_t pk[16];
+        for (int c = 0; c < 4; c++) {
+          const float *v = reinterpret_cast<const float *>(sbuf + c * 32);
+          uint32_t pk[16];
 #pragma unroll
-            for (int x = 0; x < 16; x++) {
-              const float2 e = f2_unpack(f2_fma(f2_pack(v[2 * x], v[2 * x + 1]), sl2x2, neg_mx2));
-              uint64_t pp;
-              if (decltype(poly)::value && ((kExp2EmuMask >> x) & 1u))
-                pp = exp2_poly_x2(f2_pack(fmaxf(e.x, -125.0f), fmaxf(e.y, -125.0f)));
-              else
-                pp = f2_pack(ex2_approx(e.x), ex2_approx(e.y));
-              part2[x & 1] = f2_add(part2[x & 1], pp);
-              const float2 pf = f2_unpack(pp);
-              pk[x] = pack16x2<T>(pf.x, pf.y);
-            }
-            tmem_st16(tS + c * 16, pk);
-            if (c == 1 || c == 3) {
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_half[2 * t + (c == 3 ? 1 : 0)]);
-            }
+          for (int x = 0; x < 16; x++) {
+            const float2 e = f2_unpack(f2_fma(f2_pack(v[2 * x], v[2 * x + 1]), sl2x2, neg_mx2));
+            const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
+            part2[x & 1] = f2_add(part2[x & 1], f2_pack(p0, p1));
+            pk[x] = pack16x2<T>(p0, p1);
           }
-        };
-        if (masked)
-          write_p(std::false_type{});
-        else
-          write_p(std::true_type{});
+          tmem_st16(tS + c * 16, pk);
+          if (c == 1 || c == 3) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_half[2 * t + (c == 3 ? 1 : 0)]);
+          }
+        }
         const float2 s0 = f2_unpack(part2[0]), s1 = f2_unpack(part2[1]);
         l += (s0.x + s0.y) + (s1.x + s1.y);
         valid -= C::BN;
