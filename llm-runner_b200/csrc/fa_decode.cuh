@@ -181,6 +181,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
     *abort_flag = 0;
     fence_barrier_init();
   }
+  pdl_launch_dependents();  // the join's CTAs fit beside this kernel's and wait there
+  griddep_wait();
   // ------------------------------------------------ the line of blocks, my range
   // Each thread takes R neighbouring requests: the sum of all lengths from i0
   // on (STRIDE requests), and the place of this thread's first.
@@ -227,7 +229,6 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
   const long long most = max(1ll, line / kRangeBlocks);
   const int ctas = line == 0 ? 0 : most < (long long)gridDim.x ? (int)most : (int)gridDim.x;
   const int cta = blockIdx.x;
-  pdl_launch_dependents();  // the join's CTAs fit beside this kernel's and wait there
   if (tid == 0) p.joins[cta].last = -1;
   if (cta >= ctas) return;
   const long long lo = range_begin(line, ctas, cta), hi = range_begin(line, ctas, cta + 1);
@@ -556,6 +557,7 @@ __global__ void __launch_bounds__(128) fa_decode_join_kernel(const __grid_consta
   using C = DecodeCfg<D, RW>;
   constexpr int E = D / 32, U = 8;
   typedef typename std::conditional<E == 4, float4, float2>::type Vec;
+  pdl_launch_dependents();
   griddep_wait();
   const int first = blockIdx.x, r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const DecodeJoin join = p.joins[first];

@@ -401,7 +401,10 @@ __global__ void __launch_bounds__(384, 1)
   FaCut lo, hi;
   long long line = 0;
   int ranges = 1;
-  if constexpr (PAGED) pdl_launch_dependents();  // the join comes as soon as an SM is free
+  if constexpr (PAGED) {
+    pdl_launch_dependents();  // the join starts up as SMs get free
+    griddep_wait();
+  }
   if constexpr (PAGED) find_range(p, smem + C::EPI_OFF, lo, hi, line, ranges);
 
   // A whole warp's wait; all lanes get the same answer, also when it is given up.
@@ -966,6 +969,7 @@ __global__ void __launch_bounds__(384, 1)
 // so that their loads overlap; lane x first finds the weight of part x.
 template <int D, typename OutT>
 __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant__ FaRowsParams p) {
+  pdl_launch_dependents();
   griddep_wait();
   const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int E = D / 32, ROWS = 4, U = 4;

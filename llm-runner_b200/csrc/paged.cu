@@ -146,19 +146,15 @@ int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r) {
   if (regs * C::THREADS < C::REG_NEED)
     return fail(ctx, LLMR_ECUDA, "fa_rows: %d launch registers per thread are too few for the "
                 "register split", regs);
-  kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mq, mk, mv, p);
-  if ((rc = after_launch(ctx, "fa_rows")) || !PAGED) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 8);
-  cfg.blockDim = dim3(256);
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  auto join = fa_rows_join_kernel<D, OutT>;
-  CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, join, p));
+  if (!PAGED) {
+    // (Overlapped with the call before, ragged prompts took 9 % longer: CTAs of
+    // two grids that both take over units.)
+    kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mq, mk, mv, p);
+    return after_launch(ctx, "fa_rows");
+  }
+  CUDA_TRY(ctx, launch_overlapped(kern, dim3(grid), C::THREADS, C::SMEM_BYTES, ctx->stream, 1, mq, mk, mv, p));
+  if ((rc = after_launch(ctx, "fa_rows"))) return rc;
+  CUDA_TRY(ctx, launch_overlapped(fa_rows_join_kernel<D, OutT>, dim3(grid, 8), 256, 0, ctx->stream, 1, p));
   return after_launch(ctx, "fa_rows_join");
 }
 
@@ -197,10 +193,8 @@ int launch_paged_prologue(llmr_ctx *ctx, bool half, PagedRopeParams &p) {
   p.chunks = (rows + per_warp - 1) / per_warp;
   const long long warps = (long long)p.tokens * p.chunks;
   const unsigned grid = (unsigned)((warps + 7) / 8);
-  if (half)
-    paged_prologue_kernel<D, InT, OutT, true><<<grid, 256, 0, ctx->stream>>>(p);
-  else
-    paged_prologue_kernel<D, InT, OutT, false><<<grid, 256, 0, ctx->stream>>>(p);
+  auto kern = half ? paged_prologue_kernel<D, InT, OutT, true> : paged_prologue_kernel<D, InT, OutT, false>;
+  CUDA_TRY(ctx, launch_overlapped(kern, dim3(grid), 256, 0, ctx->stream, 1, p));
   return after_launch(ctx, "paged_prologue");
 }
 
@@ -375,19 +369,7 @@ int llmr_paged_plan(llmr_ctx *ctx, const llmr_plan_desc *d, const int32_t *ctx_l
   while (ctas < 8 && items > (long long)ctas * threads) ctas *= 2;
   const int smem = (3 * p.n + 2) * (int)sizeof(int);
   CUDA_TRY(ctx, set_smem_once(paged_plan_kernel, (3 * kPlanMaxSeqs + 2) * (int)sizeof(int)));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, paged_plan_kernel, p));
+  CUDA_TRY(ctx, launch_overlapped(paged_plan_kernel, dim3(ctas), threads, smem, ctx->stream, ctas, p));
   return after_launch(ctx, "paged_plan");
 NO_THROW_END(ctx)
 

@@ -25,19 +25,10 @@ int launch_decode(llmr_ctx *ctx, const RowsParams &r, float *parts) {
   CUDA_TRY(ctx, set_smem_once(kern, C::SMEM_BYTES));
   const int want = 2 * ctx->num_sms;
   const int grid = want < kDecodeCtas ? want : kDecodeCtas;
-  kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mk, mv, p);
+  CUDA_TRY(ctx, launch_overlapped(kern, dim3(grid), C::THREADS, C::SMEM_BYTES, ctx->stream, 1, mk, mv, p));
   if ((rc = after_launch(ctx, "fa_decode"))) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, (r.max_q * p.group + 3) / 4);
-  cfg.blockDim = dim3(128);
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  auto join = fa_decode_join_kernel<D, RW, OutT>;
-  CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, join, p));
+  CUDA_TRY(ctx, launch_overlapped(fa_decode_join_kernel<D, RW, OutT>, dim3(grid, (r.max_q * p.group + 3) / 4), 128,
+                                  0, ctx->stream, 1, p));
   return after_launch(ctx, "fa_decode_join");
 }
 

@@ -142,6 +142,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_plan_kernel(const PlanP
   __shared__ long long part[32][2];
   const int tid = threadIdx.x, rank = blockIdx.x, ranks = gridDim.x;
   const int warps = blockDim.x >> 5;
+  pdl_launch_dependents();
+  griddep_wait();
   const int free_n = *p.n_free;
   long long base_t = 0, base_p = 0;
   bool bad = false;
@@ -256,6 +258,8 @@ __global__ void __launch_bounds__(256, 4) paged_prologue_kernel(const PagedRopeP
   const int sub = lane % LANES, grp = lane / LANES;
   const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int t = (int)(item / p.chunks);
+  pdl_launch_dependents();
+  griddep_wait();
   if (t >= p.tokens) return;
   const int h0 = (int)(item - (long long)t * p.chunks) * (GROUPS * kRopeSteps);
   // The slot, the position and the rows are asked for together: a token's
