@@ -132,7 +132,7 @@ __device__ __forceinline__ int decode_blocks(bool ok, int nq, int nk) {
 }
 
 // Row r of a pair, columns col ..: acc / l to the output, and the row's
-// log-sum-exp. A row without a key is 0 and -inf.
+// log-sum-exp. A row without a key (l = 0) is 0 and -inf; a NaN score is a NaN l.
 __device__ __forceinline__ float elem(const float2 &v, int i) { return i ? v.y : v.x; }
 __device__ __forceinline__ float elem(const float4 &v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
@@ -143,7 +143,7 @@ __device__ __forceinline__ void finish_row(const DecodeParams &p, const DecodeSe
   constexpr int N = sizeof(Acc) / 4;
   const int tok = r / p.group, h = sg.kvh * p.group + r - tok * p.group;
   const long long row = sg.row0 + tok;
-  const bool none = top == -INFINITY;
+  const bool none = l == 0.0f;
   const float inv = none ? 0.0f : 1.0f / l;
   Pack<OutT, N> out;
 #pragma unroll
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
 #pragma unroll
         for (int w = 0; w < C::KW; w++) {
           const float2 e = ml[(w0 + w) * 16 + rr];
-          if (e.x != -INFINITY) l += e.y * ex2_approx(e.x - top);
+          l += e.x == -INFINITY ? e.y : e.y * ex2_approx(e.x - top);  // (its sum is 0, or NaN)
           const float4 v = *reinterpret_cast<const float4 *>(merge + ((w0 + w) * 16 + rr) * D +
                                                              (col ^ ((rr & 7) << 3)));
           acc.x += v.x;

@@ -857,9 +857,11 @@ __global__ void __launch_bounds__(384, 1)
           w1 = ex2_approx(other.x - top);
           l = l * w0 + other.y * w1;
           m_used = top;
+        } else {
+          l += other.y;  // 0, or NaN
         }
       }
-      const bool none = m_used == -INFINITY;  // no key
+      const bool none = l == 0.0f;  // no key (a NaN score is a NaN l)
       const float inv = none ? 0.0f : 1.0f / l;
       const float lse = none ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
       w0 *= inv;
@@ -1028,7 +1030,7 @@ __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant
     const int row = row0 + i, t = row >> 7, tr = row & 127;
     const int rt = tr * p.recip >> 16, tok = t * p.tpt + rt;
     if (rt >= p.tpt || tok >= join.tokens) continue;
-    const float inv = sum[i] > 0.0f ? 1.0f / sum[i] : 0.0f;
+    const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
     const int h = join.kvh * p.group + tr - rt * p.group, q_row = join.q_row + tok;
     Pack<OutT, E> out;
 #pragma unroll
@@ -1036,7 +1038,7 @@ __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant
     *reinterpret_cast<Pack<OutT, E> *>(static_cast<OutT *>(p.rows.o) + (long long)q_row * p.rows.os[0] +
                                        (long long)h * p.rows.os[1] + lane * E) = out;
     if (p.rows.lse && lane == 0)
-      p.rows.lse[(long long)h * p.rows.tokens + q_row] = sum[i] > 0.0f ? mx[i] + logf(sum[i]) : -INFINITY;
+      p.rows.lse[(long long)h * p.rows.tokens + q_row] = sum[i] == 0.0f ? -INFINITY : mx[i] + logf(sum[i]);
   }
 }
 

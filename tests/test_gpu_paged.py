@@ -301,6 +301,33 @@ def test_peaked_and_growing_scores(ctx):
         p.check(ctx)
 
 
+@pytest.mark.parametrize("q", [1, 3, 8, 60, 200])
+@pytest.mark.parametrize("kv", [1, 300, 9000])
+def test_a_nan_key_is_seen(ctx, q, kv):
+    """Rows that see a NaN key are NaN (and so is their LSE), also where it is the only one,
+    and requests beside it are not."""
+    kv = max(kv, q)
+    p = Paged([q, q], [kv, kv], 8, 2, 128, 16, BF16, seed=q)
+    at = kv - q                     # the first new token's own key: every row sees it
+    p.kc[int(p.table[0, at // 16]), at % 16] = math.nan
+    o = p.run(ctx).float()
+    assert o[:q].isnan().all() and p.lse[:, :q].isnan().all()
+    assert not o[q:].isnan().any() and not p.lse[:, q:].isnan().any()
+
+
+def test_causal_nan_rows(ctx):
+    q, k, v = randn(1, 300, 4, 64), randn(2, 300, 2, 64), randn(3, 300, 2, 64)
+    k[0], k[150] = math.nan, math.nan
+    o, lse = torch.zeros_like(q), torch.zeros((4, 300), device="cuda")
+    L.attention_causal(ctx, q, k, v, o, ints([0, 100, 300]), scale=0.125, lse=lse)
+    ctx.sync()
+    bad = torch.zeros(300, dtype=torch.bool, device="cuda")
+    bad[:100] = True
+    bad[150:] = True
+    assert o[bad].isnan().all() and lse[:, bad].isnan().all()
+    assert not o[~bad].isnan().any() and not lse[:, ~bad].isnan().any()
+
+
 def test_padded_bound_and_ragged_mix(ctx):
     """max_q_len above every request's rows; decodes and chunks in one call."""
     q = [1, 64, 1, 5, 0, 200, 1]
