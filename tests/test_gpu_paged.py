@@ -375,6 +375,57 @@ def test_two_contexts_at_once(q):
         x.close()
 
 
+def test_prompts_of_two_contexts_at_once():
+    """Grids that take over their own units only, while both are on the GPU."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [L.Context(0, stream=s) for s in streams]
+    lens = [900, 30, 2000, 1, 1300]
+    cases = [(randn(i, sum(lens), 16, 128), randn(i + 5, sum(lens), 4, 128), randn(i + 9, sum(lens), 4, 128))
+             for i in range(2)]
+    cu = ints(cumulative(lens))
+    alone = [run_causal(x, lens, 16, 4, 128, BF16, BF16, qkv=c) for c, x in zip(cases, ctxs)]
+    outs = [torch.zeros_like(a) for a in alone]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (q, k, v), x, o in zip(cases, ctxs, outs):
+            L.attention_causal(x, q, k, v, o, cu, scale=128 ** -0.5)
+    for x in ctxs:
+        x.sync()
+    assert all(torch.equal(a, b) for a, b in zip(alone, outs))
+    for x in ctxs:
+        x.close()
+
+
+def test_captured_prompts_replay_with_other_lengths():
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ctx = L.Context(0, stream=stream)
+        t, h, hk, d = 3000, 8, 2, 64
+        q, k, v = randn(1, t, h, d), randn(2, t, hk, d), randn(3, t, hk, d)
+        o, cu = torch.zeros_like(q), ints([0, 1000, 1000, 2500])
+        call = lambda: L.attention_causal(ctx, q, k, v, o, cu, scale=0.125)
+        call()
+        ctx.sync()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        call()
+        call()
+    with torch.cuda.stream(stream):
+        for lens in ([3000, 0, 0], [1, 1, 1], [700, 1500, 300]):
+            cu.copy_(ints(cumulative(lens)))
+            o.fill_(7)
+            g.replay()
+            ctx.sync()
+            got = o.clone()
+            o.fill_(7)
+            call()
+            ctx.sync()
+            assert torch.equal(got, o) and (o[sum(lens):] == 7).all()
+    torch.cuda.synchronize()
+    del g
+    ctx.close()
+
+
 def test_shared_pages(ctx):
     """Requests whose tables name the same pages (a common prefix)."""
     p = Paged([1, 1, 1], [640, 700, 666], 8, 2, 128, 64, BF16, seed=3)
