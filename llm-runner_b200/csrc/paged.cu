@@ -146,16 +146,17 @@ int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r) {
   if (regs * C::THREADS < C::REG_NEED)
     return fail(ctx, LLMR_ECUDA, "fa_rows: %d launch registers per thread are too few for the "
                 "register split", regs);
-  if (!PAGED) {
+  if constexpr (!PAGED) {
     // (Overlapped with the call before, ragged prompts took 9 % longer: CTAs of
     // two grids that both take over units.)
     kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mq, mk, mv, p);
     return after_launch(ctx, "fa_rows");
+  } else {
+    CUDA_TRY(ctx, launch_overlapped(kern, dim3(grid), C::THREADS, C::SMEM_BYTES, ctx->stream, 1, mq, mk, mv, p));
+    if ((rc = after_launch(ctx, "fa_rows"))) return rc;
+    CUDA_TRY(ctx, launch_overlapped(fa_rows_join_kernel<D, OutT>, dim3(grid, 8), 256, 0, ctx->stream, 1, p));
+    return after_launch(ctx, "fa_rows_join");
   }
-  CUDA_TRY(ctx, launch_overlapped(kern, dim3(grid), C::THREADS, C::SMEM_BYTES, ctx->stream, 1, mq, mk, mv, p));
-  if ((rc = after_launch(ctx, "fa_rows"))) return rc;
-  CUDA_TRY(ctx, launch_overlapped(fa_rows_join_kernel<D, OutT>, dim3(grid, 8), 256, 0, ctx->stream, 1, p));
-  return after_launch(ctx, "fa_rows_join");
 }
 
 template <int D, typename T, bool PAGED>
