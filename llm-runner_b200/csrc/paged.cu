@@ -193,9 +193,10 @@ int launch_paged_prologue(llmr_ctx *ctx, bool half, PagedRopeParams &p) {
   const int rows = (p.q ? p.hq : 0) + 2 * p.hk;
   p.chunks = (rows + per_warp - 1) / per_warp;
   const long long warps = (long long)p.tokens * p.chunks;
-  const unsigned grid = (unsigned)((warps + 7) / 8);
+  constexpr int per_cta = kRopeThreads / 32;
+  const unsigned grid = (unsigned)((warps + per_cta - 1) / per_cta);
   auto kern = half ? paged_prologue_kernel<D, InT, OutT, true> : paged_prologue_kernel<D, InT, OutT, false>;
-  CUDA_TRY(ctx, launch_overlapped(kern, dim3(grid), 256, 0, ctx->stream, 1, p));
+  CUDA_TRY(ctx, launch_overlapped(kern, dim3(grid), kRopeThreads, 0, ctx->stream, 1, p));
   return after_launch(ctx, "paged_prologue");
 }
 

@@ -215,10 +215,14 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_plan_kernel(const PlanP
 // a row as 8 elements of its first half and the 8 elements D/2 further on, so
 // that both pairings of the rotation, (2i, 2i+1) and (i, i + D/2), stay inside
 // a lane and every access is 16 bytes. A warp takes kRopeSteps rows per
-// group of ONE token, all loads issued before the first use. 8191 tokens, 32 / 8
-// heads of 128: 49 us, 4.2 TB/s. 4 rows per group and two CTAs per SM took 64 us, 1
-// and six 55, 2 and five 73 (spills), 2 and three 53.
+// group of ONE token, all loads issued before the first use. Small CTAs leave a
+// choice of register limits: 28 warps per SM at 72 registers. 8191 tokens, 32 / 8
+// heads of 128: 46 us, 4.5 TB/s; of 64: 23 us; 2000 tokens of 128: 11.1. 32 warps at
+// 64 registers (spills at heads of 64): 45, 24 and 12.1 us; in CTAs of 256 threads 49
+// and 26 at 8191. Rows per group in CTAs of 256, 8191 tokens of 128: 4 took 64 us (two
+// CTAs per SM), 1 took 55 (six).
 constexpr int kRopeSteps = 2;
+constexpr int kRopeThreads = 64, kRopeCtas = 14;  // CTAs per SM
 
 struct PagedRopeParams {
   int tokens, hq, hk, page, num_pages, rope_rows, chunks;  // chunks: warps per token
@@ -252,11 +256,12 @@ __device__ __forceinline__ void store8(T *dst, const float *x) {
 }
 
 template <int D, typename InT, typename OutT, bool HALF>
-__global__ void __launch_bounds__(256, 4) paged_prologue_kernel(const PagedRopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeCtas)
+paged_prologue_kernel(const PagedRopeParams p) {
   constexpr int LANES = D / 16, GROUPS = 32 / LANES;
   const int lane = threadIdx.x & 31;
   const int sub = lane % LANES, grp = lane / LANES;
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const long long item = (long long)blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
   const int t = (int)(item / p.chunks);
   pdl_launch_dependents();
   griddep_wait();
