@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_plan_kernel(const PlanP
 
 // ----------------------------------------------------------------- prologue
 // One pass over the new tokens' rows: read, RMSNorm and rotation in fp32
-// registers, one rounding, write. Bound by HBM. A group of D / 16 lanes holds
+// registers, one rounding, write. Bound by loads in flight. A group of D / 16 lanes holds
 // a row as 8 elements of its first half and the 8 elements D/2 further on, so
 // that both pairings of the rotation, (2i, 2i+1) and (i, i + D/2), stay inside
 // a lane and every access is 16 bytes. A warp takes kRopeSteps rows per
