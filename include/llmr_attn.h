@@ -472,7 +472,8 @@ int llmr_attention_causal(llmr_ctx *ctx, const llmr_causal_desc *desc,
  * keys, the new tokens' own included: key j is row j % page_size of page
  * block_table[i][j / page_size] of k_cache and v_cache [num_pages][page_size]
  * [n_kv_heads][head_dim]. Query row r (of n) attends to keys 0 ..
- * kv_lens[i] - n + r; one without a key gives o = 0 and lse = -inf. Rows
+ * kv_lens[i] - n + r; one without a key gives o = 0 and lse = -inf (one with
+ * keys whose scores are all -inf: NaN and -inf, in either operator). Rows
  * behind the last request are left as they were. What a page holds behind a
  * request's last key may be anything, NaN included. max_q_len bounds the
  * rows of any request (and picks the kernel). page_size: 16, 32, 64, 128 or

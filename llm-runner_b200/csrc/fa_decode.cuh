@@ -132,7 +132,8 @@ __device__ __forceinline__ int decode_blocks(bool ok, int nq, int nk) {
 }
 
 // Row r of a pair, columns col ..: acc / l to the output, and the row's
-// log-sum-exp. A row without a key (l = 0) is 0 and -inf; a NaN score is a NaN l.
+// log-sum-exp. A row that sees no key is 0 and -inf; one whose scores are all
+// -inf has l = 0 too, and is 0 / 0 = NaN and -inf; a NaN score is a NaN l.
 __device__ __forceinline__ float elem(const float2 &v, int i) { return i ? v.y : v.x; }
 __device__ __forceinline__ float elem(const float4 &v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
@@ -143,8 +144,8 @@ __device__ __forceinline__ void finish_row(const DecodeParams &p, const DecodeSe
   constexpr int N = sizeof(Acc) / 4;
   const int tok = r / p.group, h = sg.kvh * p.group + r - tok * p.group;
   const long long row = sg.row0 + tok;
-  const bool none = l == 0.0f;
-  const float inv = none ? 0.0f : 1.0f / l;
+  const bool none = sg.nk - sg.nq + tok < 0;
+  const float inv = 1.0f / l;
   Pack<OutT, N> out;
 #pragma unroll
   for (int i = 0; i < N; i++) out.v[i] = from_f32<OutT>(none ? 0.0f : elem(acc, i) * inv);
@@ -595,7 +596,7 @@ __global__ void __launch_bounds__(128) fa_decode_join_kernel(const __grid_consta
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  DecodeSeg sg = {};
+  DecodeSeg sg = {};  // (more than one block of keys, few rows: each sees some)
   sg.row0 = join.row0;
   sg.kvh = join.kvh;
   finish_row<D, OutT>(p, sg, r, lane * E, *reinterpret_cast<const Vec *>(acc), top, l);

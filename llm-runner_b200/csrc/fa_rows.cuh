@@ -861,13 +861,16 @@ __global__ void __launch_bounds__(384, 1)
           l += other.y;  // 0, or NaN
         }
       }
-      const bool none = l == 0.0f;  // no key (a NaN score is a NaN l)
+      const int tok = row * p.recip >> 16, head = row - tok * p.group;
+      const int t0 = un.dual ? 0 : t * p.tpt;          // the tile's first token
+      // A row that sees no key is 0 and -inf, and so is a part that adds nothing to
+      // its row. Scores that are all -inf are l = 0 too: 0 / 0 = NaN. (A NaN score
+      // is a NaN l.)
+      const bool none = un.part >= 0 ? l == 0.0f : un.pos + t0 + tok < 0;
       const float inv = none ? 0.0f : 1.0f / l;
       const float lse = none ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
       w0 *= inv;
       w1 *= inv;
-      const int tok = row * p.recip >> 16, head = row - tok * p.group;
-      const int t0 = un.dual ? 0 : t * p.tpt;          // the tile's first token
       const int ntok = min(un.tokens - t0, p.tpt);  // its tokens (<= 0: none)
       const bool live = tok < ntok;
       const int kvh = un.kvh, q_row = un.q_row + t0;
@@ -998,7 +1001,7 @@ __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
       const float ls = x0 + lane < parts ? p.part_lse[part_row(x0 + lane, i)] : -INFINITY;
-      w[i] = ls == -INFINITY ? 0.0f : expf(ls - mx[i]);  // 0: saw no key
+      w[i] = ls == -INFINITY ? 0.0f : expf(ls - mx[i]);  // 0: adds nothing
       sum[i] += w[i];
     }
     const int n = min(32, parts - x0);
@@ -1030,7 +1033,7 @@ __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant
     const int row = row0 + i, t = row >> 7, tr = row & 127;
     const int rt = tr * p.recip >> 16, tok = t * p.tpt + rt;
     if (rt >= p.tpt || tok >= join.tokens) continue;
-    const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
+    const float inv = 1.0f / sum[i];  // (every row of a unit that was cut sees a key)
     const int h = join.kvh * p.group + tr - rt * p.group, q_row = join.q_row + tok;
     Pack<OutT, E> out;
 #pragma unroll
@@ -1038,7 +1041,7 @@ __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant
     *reinterpret_cast<Pack<OutT, E> *>(static_cast<OutT *>(p.rows.o) + (long long)q_row * p.rows.os[0] +
                                        (long long)h * p.rows.os[1] + lane * E) = out;
     if (p.rows.lse && lane == 0)
-      p.rows.lse[(long long)h * p.rows.tokens + q_row] = sum[i] == 0.0f ? -INFINITY : mx[i] + logf(sum[i]);
+      p.rows.lse[(long long)h * p.rows.tokens + q_row] = mx[i] + logf(sum[i]);
   }
 }
 

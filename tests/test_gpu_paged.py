@@ -859,3 +859,49 @@ def test_the_current_device_stays(ctx):
     before = torch.cuda.current_device()
     run_causal(ctx, [10], 4, 2, 64, BF16, BF16)
     assert torch.cuda.current_device() == before
+
+
+# --------------------------------------------------------------- infinite scores
+
+def check_infinite(o, lse, q, k, v, scale, dead, dtype, what):
+    """Rows of one request whose first `dead` see scores of -inf alone: 0 / 0 and log 0."""
+    w, wl, weight = R.rows_attention(q, k, v, scale)
+    assert o[:dead].isnan().all() and (lse[:, :dead] == -math.inf).all(), what
+    finite = k.clone()
+    finite[..., 0] = finite[..., 0].nan_to_num(neginf=0.0)
+    R.check_attention(o[dead:], lse[:, dead:], w[dead:], wl[:, dead:], weight[dead:], dtype, q.shape[2],
+                      k.shape[0], float(v.abs().max()), R.score_size(q, finite, scale), what)
+
+
+@pytest.mark.parametrize("q", [1, 4, 8, 20, 200])
+@pytest.mark.parametrize("kv", [1, 300, 9000])
+def test_rows_of_infinite_scores(ctx, q, kv):
+    """Rows that see keys, each with a score of -inf, are no rows without a key."""
+    kv, dead = max(kv, q), (q + 1) // 2
+    p = Paged([q, q], [kv, kv], 8, 2, 128, 16, BF16, seed=q)
+    p.q[:, :, 0] = p.q[:, :, 0].abs() + 0.5
+    at = torch.arange(kv - q + dead, device="cuda")     # what the first `dead` rows see
+    p.kc[p.table[0].long()[at // 16], at % 16, :, 0] = -math.inf
+    p.k[0][at, :, 0] = -math.inf
+    o, scale = p.run(ctx), p.d ** -0.5
+    check_infinite(o[:q], p.lse[:, :q], p.q[:q], p.k[0], p.v[0], scale, dead, BF16, (q, kv))
+    check_infinite(o[q:], p.lse[:, q:], p.q[q:], p.k[1], p.v[1], scale, 0, BF16, (q, kv))
+
+
+@pytest.mark.parametrize("h,hk,d", [(8, 2, 128), (14, 2, 64), (32, 8, 128)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens", [[100, 700, 3], [5000]])
+def test_causal_rows_of_infinite_scores(ctx, h, hk, d, dtype, lens):
+    t = sum(lens)
+    q, k, v = (randn(i, t, n, d, dtype=dtype) for i, n in ((1, h), (2, hk), (3, hk)))
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    dead = [2 * n // 5 for n in lens]
+    cu = cumulative(lens)
+    for at, x in zip(cu, dead):
+        k[at:at + x, :, 0] = -math.inf
+    o, lse = torch.zeros_like(q), torch.zeros((h, t), device="cuda")
+    L.attention_causal(ctx, q, k, v, o, ints(cu), scale=d ** -0.5, lse=lse)
+    ctx.sync()
+    for at, n, x in zip(cu, lens, dead):
+        part = slice(at, at + n)
+        check_infinite(o[part], lse[:, part], q[part], k[part], v[part], d ** -0.5, x, dtype, (lens, at))
