@@ -436,7 +436,9 @@ int llmr_rope_tables(const int32_t *pos, uint32_t seq_len, uint32_t n_axes,
  * when the kernels run, so a captured step replays with other lengths. What is
  * out of range there is never followed: rows of the requests concerned are
  * left out or unspecified, the others are right, and llmr_sync returns
- * LLMR_EINVAL. Query head h uses key/value head
+ * LLMR_EINVAL. (A request is concerned if its own offsets, length or pages are
+ * out of range, if it begins before the end of an earlier one, and in rows that
+ * another claims too.) Query head h uses key/value head
  * h / (n_heads / n_kv_heads). head_dim is 64 or 128. Element strides of 0
  * select the dense default [token][head][dim]; bases and strides must be
  * multiples of 16 bytes. The calls run on the context's device whatever the

@@ -19,6 +19,8 @@
 //    launch control: a CTA takes over units whose CTAs have not started, so no
 //    counter in memory is needed. It asks when the last loads of its unit are
 //    under way and no sooner: a unit held early is one that an idle CTA lacks.
+//    The search needs ascending offsets. Where some are not, it may miss sequences
+//    that are in order themselves, and warp 11 hands all their units out again.
 //  * Paged chunks: few units of very different lengths, so all units' keys
 //    (and kUnitKeys more for each unit's ends) are laid end to end and cut into one
 //    range per CTA. A unit that a cut falls into leaves parts in the
@@ -29,7 +31,8 @@
 //   warp 8           TMA producer: Q, then K_j, V_j into an NST-slot ring
 //   warp 9           MMA issuer and TMEM owner
 //   warp 10          scheduler: finds the units, one ahead
-//   warp 11          prompts, CTA 0: looks through all sequences for bad offsets
+//   warp 11          prompts: looks through all sequences for bad offsets, and
+//                    goes on for the scheduler behind its last unit
 // MMA order per key block j: PV0_j, S0_{j+1}, PV1_j, S1_{j+1}, each tile with
 // its own number of blocks. The first blocks need no mask; in those that reach
 // past a row's last key the scores are set to -inf (so P is exactly 0), P V
@@ -63,6 +66,8 @@ constexpr int kMaxRanges = 160;  // CTAs of a paged call (workspace)
 constexpr int kUnitKeys = 256;
 constexpr int kCutBlocks = 3;
 constexpr int kRangeKeys = 256;
+// Prompts with a bad offset: the most CTAs that all units are dealt out to.
+constexpr int kMaxShares = 256;
 
 // A unit that a cut falls into, entered by the CTA that begins it: its parts
 // are that CTA's second part and the first parts of the CTAs up to `last`.
@@ -78,6 +83,7 @@ struct FaRowsParams {
   int vtiles;             // prompts: virtual tiles of all requests
   int units;              // prompts: vtiles * Hk
   int dynamic;            // prompts: units are taken over by cluster launch control
+  int shares;             // prompts: CTAs that units are dealt out to if an offset is bad
   float scale_log2;
   float *part_o, *part_lse;  // paged: [2 * CTA + 0 / 1][256 rows]([D])
   FaJoin *joins;             // paged: [CTA]
@@ -147,6 +153,37 @@ __device__ __forceinline__ bool prompt_unit(const FaRowsParams &p, int u, FaUnit
   return true;
 }
 
+// Prompts whose offsets are not all in order: gives each unit of one share of the
+// sequences that are, and that begin behind the earlier ones (so a row has one
+// sequence). Whole warp; false once give() is.
+template <typename Give>
+__device__ __forceinline__ bool deal_units(const FaRowsParams &p, int share, Give give) {
+  const RowsParams &rp = p.rows;
+  const int lane = threadIdx.x & 31, tu = p.tu;
+  FaUnit un;
+  int end = 0;  // of the sequences so far
+  int at = 0;   // their units, modulo p.shares
+  for (int r0 = 0; r0 < rp.n; r0 += 32) {
+    int row0 = 0, nq = 0, nk = 0;
+    if (r0 + lane < rp.n) request_rows(rp, r0 + lane, row0, nq, nk);
+    for (unsigned left = __ballot_sync(0xffffffffu, nq > 0); left; left &= left - 1) {
+      const int first = __shfl_sync(0xffffffffu, row0, __ffs(left) - 1);
+      const int rows = __shfl_sync(0xffffffffu, nq, __ffs(left) - 1);
+      if (first < end) continue;
+      end = first + rows;
+      const long long units = (long long)((rows + tu - 1) / tu) * rp.Hk;
+      for (long long x = share < at ? share - at + p.shares : share - at; x < units; x += p.shares) {
+        unit_rows(un, tu, (int)(x % rp.Hk), first, rows, rows, (int)(x / rp.Hk));
+        un.kv_row = first;
+        unit_blocks(un, p.tpt, 0, (un.keys + 127) / 128);
+        if (!give(un)) return false;
+      }
+      at = (int)((at + units) % p.shares);
+    }
+  }
+  return true;
+}
+
 // Paged: where tile i of a request begins, in keys from the request's first:
 // tile j counts its last token's position (as if it were full) and kUnitKeys.
 __host__ __device__ __forceinline__ long long tile_begin(long long ctx, long long tu, long long i) {
@@ -187,7 +224,9 @@ struct FaRowsCfg {
   static constexpr int NBAR = 4 + 2 * NST + 2 + 4 + 2 + 2 + 2 * kUnitSlots + 5;
   static constexpr int UNIT_OFF = CTL_OFF + (NBAR * 8 + 15) / 16 * 16;
   static constexpr int CLC_OFF = UNIT_OFF + kUnitSlots * 48;
-  static constexpr int X_OFF = CLC_OFF + 32;  // tile 1's (max, sum) of 128 rows for tile 0
+  static constexpr int END_OFF = CLC_OFF + 32;  // units handed out (or -1), then kMaxShares bits
+  // Tile 1's (max, sum) of 128 rows for tile 0.
+  static constexpr int X_OFF = END_OFF + (4 + kMaxShares / 8 + 15) / 16 * 16;
   static constexpr int SMEM_BYTES = X_OFF + 1024 + 1024;
   static constexpr int THREADS = 384;
   static constexpr int REG_SOFTMAX = 200, REG_OTHER = 104, REG_LAUNCH = 168;
@@ -356,6 +395,7 @@ __global__ void __launch_bounds__(384, 1)
   auto unit_slot = [&](int i) {
     return reinterpret_cast<FaUnit *>(smem + C::UNIT_OFF + (i % kUnitSlots) * 48);
   };
+  int *end_state = reinterpret_cast<int *>(smem + C::END_OFF);
   float2 *exchange = reinterpret_cast<float2 *>(smem + C::X_OFF);
   void *clc_resp = smem + C::CLC_OFF;
   uint32_t *tmem_base_slot = reinterpret_cast<uint32_t *>(smem + C::CLC_OFF + 16);
@@ -686,8 +726,12 @@ __global__ void __launch_bounds__(384, 1)
         });
       } else {
         int u = blockIdx.x, asked = 0;
+        // The CTAs that this one runs for, itself the first, as far as units are
+        // dealt out to them: bit u % 32 of lane u / 32.
+        uint32_t mine = u < p.shares && lane == u >> 5 ? 1u << (u & 31) : 0u;
         bool ok = true, have = true;
-        for (int i = 0; ok && have; i++) {
+        int i = 0;
+        for (;; i++) {
           if (i > 0 && !(ok = wait(u_ask, i - 1))) break;
           if (i >= kUnitSlots && !(ok = wait(&u_empty[i % kUnitSlots], i / kUnitSlots - 1))) break;
           for (bool first = i == 0;; first = false) {
@@ -703,6 +747,7 @@ __global__ void __launch_bounds__(384, 1)
               }
               asked++;
               u = clc_answer(clc_resp);
+              if ((unsigned)u < (unsigned)p.shares && lane == u >> 5) mine |= 1u << (u & 31);
               fence_proxy_async_smem();
               __syncwarp();
             } else if (!first) {
@@ -711,13 +756,36 @@ __global__ void __launch_bounds__(384, 1)
             have = u >= 0;
             if (!have || prompt_unit(p, u, un)) break;
           }
-          if (!ok) break;
-          if (!have) un.kvh = -1;
+          if (!ok || !have) break;
           hand_out(i);
         }
+        if (lane == 0) end_state[0] = ok ? i : -1;
+        if (lane < kMaxShares / 32) end_state[1 + lane] = (int)mine;
+        __syncwarp();
+        asm volatile("bar.arrive 1, 64;" ::: "memory");
       }
-    } else if (!PAGED && blockIdx.x == 0) {
-      check_requests(p.rows, lane);  // (find_range has looked at all of them)
+    } else if (!PAGED) {  // (paged: find_range has looked at all of them)
+      const bool bad = check_requests(p.rows, lane);
+      // The scheduler's end, which comes whatever its own (bounded) waits end with.
+      __syncwarp();
+      asm volatile("bar.sync 1, 64;" ::: "memory");
+      int i = end_state[0];
+      bool ok = i >= 0;
+      for (int share = 0; ok && bad && share < p.shares; share++)
+        if (end_state[1 + (share >> 5)] >> (share & 31) & 1)
+          ok = deal_units(p, share, [&](const FaUnit &un) {
+            if (i >= kUnitSlots && !wait(&u_empty[i % kUnitSlots], i / kUnitSlots - 1)) return false;
+            if (lane == 0) {
+              *unit_slot(i) = un;
+              mbar_arrive(&u_full[i % kUnitSlots]);
+            }
+            i++;
+            return true;
+          });
+      if (ok && (i < kUnitSlots || wait(&u_empty[i % kUnitSlots], i / kUnitSlots - 1)) && lane == 0) {
+        unit_slot(i)->kvh = -1;
+        mbar_arrive(&u_full[i % kUnitSlots]);
+      }
     }
   } else {
     reg_alloc<C::REG_SOFTMAX>();

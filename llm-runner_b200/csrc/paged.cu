@@ -124,6 +124,8 @@ int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r) {
     // With an SM budget the grid is that small and strides over the units.
     p.dynamic = units > ctx->num_sms && ctx->num_sms == ctx->total_sms;
     grid = p.dynamic || units < ctx->num_sms ? (int)units : ctx->num_sms;
+    p.shares = grid < ctx->num_sms ? grid : ctx->num_sms;
+    if (p.shares > kMaxShares) p.shares = kMaxShares;
   }
   CUtensorMap mq, mk, mv;
   int rc;

@@ -79,9 +79,9 @@ inline int make_map16(llmr_ctx *ctx, CUtensorMap *map, const void *base, const l
   return LLMR_OK;
 }
 
-// Reports sequences that no row would lead to: one warp looks at all offsets,
-// eight at a time.
-__device__ __forceinline__ void check_requests(const RowsParams &p, int lane) {
+// Whether some offset is out of range or order, which is reported: one warp looks
+// at all of them, eight at a time.
+__device__ __forceinline__ bool check_requests(const RowsParams &p, int lane) {
   bool bad = false;
   for (int r0 = lane; r0 < p.n; r0 += 256) {
     int a[8], b[8];
@@ -95,6 +95,7 @@ __device__ __forceinline__ void check_requests(const RowsParams &p, int lane) {
     for (int i = 0; i < 8; i++) bad |= a[i] < 0 || a[i] > b[i] || b[i] > p.tokens;
   }
   if (bad) atomicOr(p.err, kErrInput);
+  return __any_sync(0xffffffffu, bad);
 }
 
 }  // namespace llmr

@@ -905,3 +905,148 @@ def test_causal_rows_of_infinite_scores(ctx, h, hk, d, dtype, lens):
     for at, n, x in zip(cu, lens, dead):
         part = slice(at, at + n)
         check_infinite(o[part], lse[:, part], q[part], k[part], v[part], d ** -0.5, x, dtype, (lens, at))
+
+
+# ------------------------------------------------- bad offsets beside good requests
+
+# Offsets, tokens, and the sequences that stay right: in order and in range themselves,
+# behind the earlier ones, and in no row that another ascending pair of offsets claims.
+BAD_OFFSETS = [([0, 1000, 0, 0], 1000, [0]), ([0, 1000, -1, 2000], 2000, [0]),
+               ([0, 100, 9999, 400, 700], 700, [0, 3]), ([-5, 300, 1200, 1200, 1300], 1300, [1, 3]),
+               ([0, 500, 400, 2 ** 31 - 1, 900, 1500], 1500, [0, 4]),
+               ([700, 1500, -2 ** 31, 0, 650], 1500, [0]), ([0, 300, 250, 260, 900, 1500], 1500, [4]),
+               ([2 ** 31 - 1] * 40 + [0, 333, 1000], 1000, [40, 41])]
+
+
+@pytest.mark.parametrize("cu,tokens,good", BAD_OFFSETS)
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 64), (14, 2, 64), (32, 8, 128), (8, 8, 128)])
+@pytest.mark.parametrize("budget", [0, 5])
+def test_bad_offsets_leave_other_sequences(cu, tokens, good, h, hk, d, budget):
+    own = L.Context(0)
+    own.set_sm_budget(budget)
+    q, k, v = (randn(i, tokens, n, d) for i, n in ((1, h), (2, hk), (3, hk)))
+    o, lse = torch.full_like(q, 7.0), torch.full((h, tokens), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    L.attention_causal(own, q, k, v, o, ints(cu), scale=d ** -0.5, lse=lse)
+    with pytest.raises(L.LlmrError) as e:
+        own.sync()
+    assert e.value.status == L.EINVAL
+    for i in good:
+        part = slice(cu[i], cu[i + 1])
+        w, wl, weight = R.rows_attention(q[part], k[part], v[part], d ** -0.5)
+        R.check_attention(o[part], lse[:, part], w, wl, weight, BF16, d, cu[i + 1] - cu[i],
+                          float(v[part].abs().max()), R.score_size(q[part], k[part], d ** -0.5), (cu, i))
+    own.close()
+
+
+@pytest.mark.parametrize("big", [False, True])
+def test_bad_offsets_among_many_sequences(ctx, big):
+    """Bad values here and there between hundreds of sequences, some of them long."""
+    g = torch.Generator().manual_seed(11)
+    lens = torch.randint(0, 90 if big else 9, (900,), generator=g).tolist()
+    lens[300] = 1500
+    cu, tokens = cumulative(lens), sum(lens)
+    for at, x in ((0, -1), (17, 2 ** 30), (299, -7), (400, 0), (401, tokens + 1), (650, -2 ** 31), (900, -2)):
+        cu[at] = x
+    h, hk, d = 8, 2, 64
+    q, k, v = (randn(i, tokens, n, d, dtype=F16) for i, n in ((1, h), (2, hk), (3, hk)))
+    o = torch.full_like(q, 7.0)
+    L.attention_causal(ctx, q, k, v, o, ints(cu), scale=0.125)
+    with pytest.raises(L.LlmrError):
+        ctx.sync()
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        if 0 <= a < b <= tokens:
+            part = slice(a, b)
+            w, _, weight = R.rows_attention(q[part], k[part], v[part], 0.125)
+            R.check_attention(o[part], None, w, None, weight, F16, d, b - a, float(v[part].abs().max()),
+                              R.score_size(q[part], k[part], 0.125), i)
+
+
+def test_captured_prompts_report_bad_offsets_and_recover():
+    """A replay with bad offsets, then one with good ones: the verdict belongs to its launch."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        own = L.Context(0, stream=stream)
+        t, h, hk, d = 3000, 16, 4, 64
+        q, k, v = randn(1, t, h, d), randn(2, t, hk, d), randn(3, t, hk, d)
+        o, cu = torch.zeros_like(q), ints([0, 1000, 1800, 3000])
+        call = lambda: L.attention_causal(own, q, k, v, o, cu, scale=0.125)
+        call()
+        own.sync()
+        want = o.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        call()
+    with torch.cuda.stream(stream):
+        for bad in ([0, 1000, -1, 3000], [0, 1000, 1 << 30, 3000]):
+            cu.copy_(ints(bad))
+            o.fill_(7)
+            g.replay()
+            with pytest.raises(L.LlmrError):
+                own.sync()
+            assert torch.equal(o[:1000], want[:1000])
+            cu.copy_(ints([0, 1000, 1800, 3000]))
+            o.fill_(7)
+            g.replay()
+            own.sync()
+            assert torch.equal(o, want)
+    torch.cuda.synchronize()
+    del g
+    own.close()
+
+
+@pytest.mark.parametrize("q", [1, 5, 130])
+@pytest.mark.parametrize("fault", ["page_high", "page_low", "kv_long", "kv_negative", "cu_high", "cu_low", "rows"])
+def test_bad_requests_leave_the_others(ctx, q, fault):
+    """Five requests, the third (with bad offsets its neighbour too) at fault."""
+    p = Paged([q] * 5, [500, 2700, 900, 3000, q], 8, 2, 128, 16, BF16, seed=1)
+    kw, concerned = {}, [2]
+    if fault.startswith("page"):
+        p.table[2, 3] = p.kc.shape[0] if fault == "page_high" else -9
+    elif fault.startswith("kv"):
+        p.kv[2] = 1 << 20 if fault == "kv_long" else -4
+    elif fault.startswith("cu"):
+        p.cu[3] = 99 * q if fault == "cu_high" else -3
+        concerned = [2, 3]
+    else:    # more rows than max_q_len allows
+        p = Paged([q, q, q + 1, q, q], [500, 2700, 900, 3000, q], 8, 2, 128, 16, BF16, seed=1)
+        kw["max_q"] = q
+    with pytest.raises(L.LlmrError) as e:
+        p.run(ctx, **kw)
+    assert e.value.status == L.EINVAL
+    at = 0
+    for i, n in enumerate(p.q_lens):
+        if i not in concerned:
+            rows = slice(at, at + n)
+            w, wl, weight = R.rows_attention(p.q[rows], p.k[i], p.v[i], p.d ** -0.5)
+            R.check_attention(p.o[rows], p.lse[:, rows], w, wl, weight, BF16, p.d, p.kv_list[i],
+                              float(p.v[i].abs().max()), R.score_size(p.q[rows], p.k[i], p.d ** -0.5), (fault, i))
+        at += n
+
+
+def test_bad_offsets_in_two_contexts_at_once():
+    """Where another grid holds SMs, CTAs take over units of the first of their grid."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [L.Context(0, stream=s) for s in streams]
+    t, cu = 6000, ints([0, 1700, -3, 2500, 4200, 9999, 4300, 6000])
+    good = [slice(0, 1700), slice(2500, 4200), slice(4300, 6000)]
+    cases = [(randn(i, t, 16, 128), randn(i + 5, t, 4, 128), randn(i + 9, t, 4, 128)) for i in range(2)]
+    torch.cuda.synchronize()
+    want = []
+    for (q, k, v), x in zip(cases, ctxs):
+        alone = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        L.attention_causal(x, q, k, v, alone, ints([0, 1700, 2500, 4200, 4300, 6000]), scale=128 ** -0.5)
+        x.sync()
+        want.append(alone)
+    outs = [[torch.zeros_like(a) for _ in range(10)] for a in want]
+    torch.cuda.synchronize()
+    for r in range(10):
+        for (q, k, v), x, o in zip(cases, ctxs, outs):
+            L.attention_causal(x, q, k, v, o[r], cu, scale=128 ** -0.5)
+    for x in ctxs:
+        with pytest.raises(L.LlmrError):
+            x.sync()
+    assert all(torch.equal(o[part], w[part]) for w, os in zip(want, outs) for o in os for part in good)
+    for x in ctxs:
+        x.close()
