@@ -98,8 +98,9 @@ void *llmr_get_stream(llmr_ctx *ctx);
 const char *llmr_last_error(llmr_ctx *ctx);
 /* Wait for all work on the context stream; reports device-side timeouts
  * (LLMR_ETIMEOUT) and what the causal and paged operators found wrong in
- * device memory (LLMR_EINVAL: a length, offset, slot, position or page out of
- * range; LLMR_ENOMEM: llmr_paged_plan ran out of pages). Replaces
+ * device memory (LLMR_ENOMEM: llmr_paged_plan ran out of pages; LLMR_EINVAL: a
+ * length, offset, slot, position or page out of range). One condition a call, in
+ * this order: after an error, call it until it returns LLMR_OK. Replaces
  * RenderGraph.checkpoint/flush (lib/vulkan/graph.c3:96-107). */
 int llmr_sync(llmr_ctx *ctx);
 /* Number of kernels this context has launched (for launch accounting). */

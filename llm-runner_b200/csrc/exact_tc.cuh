@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(192, 1)
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(err, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(err, 1);
 }
 
 }  // namespace llmr

@@ -960,7 +960,7 @@ __global__ void __launch_bounds__(384, 1)
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, 1);
   if (threadIdx.x == 0) LLMR_TL(21);
   if constexpr (FUSED) {
     // Every wait of this CTA on the piece counters is over. The last CTA to

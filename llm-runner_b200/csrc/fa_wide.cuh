@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(192, 1)
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -864,7 +864,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     tc_fence_after();
     tmem_dealloc_pair(tmem, C::TMEM_COLS);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, 1);
 }
 
 }  // namespace llmr

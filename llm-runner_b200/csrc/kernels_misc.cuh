@@ -24,7 +24,7 @@ __global__ void wait_timeout_probe_kernel(int *err, unsigned long long limit_ns)
     fence_barrier_init();
   }
   __syncthreads();
-  if (threadIdx.x == 0 && !mbar_wait_for(&bar, 0, &abort_flag, limit_ns)) atomicExch(err, 1);
+  if (threadIdx.x == 0 && !mbar_wait_for(&bar, 0, &abort_flag, limit_ns)) atomicOr(err, 1);
 }
 
 // batch_head_norm / perhead_rmsnorm mirror: in place on fp32 [S, H*D].

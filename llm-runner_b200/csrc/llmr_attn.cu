@@ -656,17 +656,22 @@ int llmr_sync(llmr_ctx *ctx) {
   int h = 0;
   CUDA_TRY(ctx, cudaMemcpy(&h, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost));
   if (h) {
-    CUDA_TRY(ctx, cudaMemset(ctx->d_err, 0, sizeof(int)));
-    if (h & kErrTimeout) {
+    // One condition a call: the others stay for the next one.
+    const int bit = h & kErrTimeout ? kErrTimeout : h & kErrPages ? kErrPages : h;
+    const int rest = h & ~bit;
+    CUDA_TRY(ctx, cudaMemcpy(ctx->d_err, &rest, sizeof(int), cudaMemcpyHostToDevice));
+    const char *more = rest ? " (another condition follows with the next llmr_sync)" : "";
+    if (bit == kErrTimeout) {
       // A kernel that gave up may have left its counters part-way.
       CUDA_TRY(ctx, cudaMemset(ctx->d_sync, 0, kSyncInts * sizeof(int)));
-      return fail(ctx, LLMR_ETIMEOUT, "a device-side wait exceeded its limit; results are invalid");
+      return fail(ctx, LLMR_ETIMEOUT, "a device-side wait exceeded its limit; results are invalid%s", more);
     }
-    if (h & kErrInput)
-      return fail(ctx, LLMR_EINVAL, "a length, offset, slot, position or page in device memory is "
-                                    "out of range; the rows of its request are invalid");
-    return fail(ctx, LLMR_ENOMEM, "the free list holds fewer pages than the step needs; nothing "
-                                  "was planned");
+    if (bit == kErrPages)
+      return fail(ctx, LLMR_ENOMEM, "the free list holds fewer pages than the step needs; nothing "
+                                    "was planned%s", more);
+    return fail(ctx, LLMR_EINVAL, "a length, offset, slot, position or page in device memory is "
+                                  "out of range; the rows of its request are invalid (of a plan: "
+                                  "nothing was planned)");
   }
   return LLMR_OK;
 }

@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(192, 1)
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -494,7 +494,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     tc_fence_after();
     tmem_dealloc_pair(tmem, C::TMEM_COLS);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, 1);
 }
 
 }  // namespace llmr
@@ -722,7 +722,7 @@ __global__ void __launch_bounds__(192, 1)
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, 1);
 }
 
 }  // namespace llmr

@@ -1050,3 +1050,44 @@ def test_bad_offsets_in_two_contexts_at_once():
     assert all(torch.equal(o[part], w[part]) for w, os in zip(want, outs) for o in os for part in good)
     for x in ctxs:
         x.close()
+
+
+# -------------------------------------------------- more than one error before a sync
+
+def statuses(ctx):
+    out = []
+    for _ in range(4):
+        try:
+            ctx.sync()
+            return out
+        except L.LlmrError as e:
+            out.append(e.status)
+    return out
+
+
+@pytest.mark.parametrize("pages_first", [False, True])
+@pytest.mark.parametrize("timeout", [False, True])
+def test_sync_reports_every_condition(ctx, pages_first, timeout):
+    """A bad slot and a step without pages between two syncs: neither hides the other."""
+    k, v = randn(1, 3, 2, 64), randn(2, 3, 2, 64)
+    kc, vc = (torch.zeros((2, 16, 2, 64), dtype=BF16, device="cuda") for _ in range(2))
+
+    def bad_slot():
+        L.paged_prologue(ctx, None, k, v, None, kc, vc, None, ints([0, 32, 5]))
+
+    plans = []
+
+    def no_pages():
+        plans.append(run_plan(ctx, [40, 3], [20, 50], 16, free_n=2))
+
+    calls = [no_pages, bad_slot] if pages_first else [bad_slot, no_pages]
+    if timeout:
+        calls.insert(1, lambda: ctx.check(L.lib.llmr_selftest_wait_timeout(ctx.handle, 20_000_000)))
+    for f in calls:
+        f()
+    assert statuses(ctx) == [L.ETIMEOUT] * timeout + [L.ENOMEM, L.EINVAL]
+    assert plans[0][1]()[1] == [0, 0, 0]        # cu_q: nothing was planned
+    assert torch.equal(kc[0, [0, 5]], k[[0, 2]])
+    bad_slot()
+    bad_slot()
+    assert statuses(ctx) == [L.EINVAL]
