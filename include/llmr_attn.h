@@ -83,7 +83,8 @@ int llmr_ctx_reserve(llmr_ctx *ctx, size_t bytes);
 int llmr_set_stream(llmr_ctx *ctx, void *stream);
 /* Limit the persistent kernels of this context to `sms` SMs (0 = all SMs of
  * the device), leaving the rest to work that runs beside them, e.g. the
- * NCCL send/receive kernels of the sequence-sharded ring. No reference
+ * NCCL send/receive kernels of the sequence-sharded ring. Short kernels
+ * (prologues, the planner, joins of parts) are not limited. No reference
  * counterpart (the reference is single-GPU). */
 int llmr_ctx_set_sm_budget(llmr_ctx *ctx, int sms);
 /* Diagnostic builds only (compiled with -DLLMR_TIMELINE, `make TIMELINE=1`):

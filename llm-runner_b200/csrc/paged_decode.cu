@@ -23,7 +23,9 @@ int launch_decode(llmr_ctx *ctx, const RowsParams &r, float *parts) {
     return rc;
   auto kern = fa_decode_kernel<D, RW, T, OutT>;
   CUDA_TRY(ctx, set_smem_once(kern, C::SMEM_BYTES));
-  const int want = 2 * ctx->num_sms;
+  // Two CTAs share an SM only where there is no free one: under a budget, one CTA
+  // for each of its SMs.
+  const int want = ctx->num_sms < ctx->total_sms ? ctx->num_sms : 2 * ctx->num_sms;
   const int grid = want < kDecodeCtas ? want : kDecodeCtas;
   CUDA_TRY(ctx, launch_overlapped(kern, dim3(grid), C::THREADS, C::SMEM_BYTES, ctx->stream, 1, mk, mv, p));
   if ((rc = after_launch(ctx, "fa_decode"))) return rc;

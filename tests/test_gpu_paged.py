@@ -1091,3 +1091,45 @@ def test_sync_reports_every_condition(ctx, pages_first, timeout):
     bad_slot()
     bad_slot()
     assert statuses(ctx) == [L.EINVAL]
+
+
+# ------------------------------------------------------------------- the SM budget
+
+def captured_kernels(stream, call):
+    """(name, CTAs) of the kernels that a call launches, from a capture of it."""
+    from cuda.bindings import driver
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g, stream=stream):
+        call()
+    graph = driver.CUgraph(int(g.raw_cuda_graph()))
+    _, _, n = driver.cuGraphGetNodes(graph)
+    _, nodes, n = driver.cuGraphGetNodes(graph, n)
+    out = []
+    for node in nodes:
+        err, p = driver.cuGraphKernelNodeGetParams(node)
+        assert err == driver.CUresult.CUDA_SUCCESS
+        err, name = driver.cuFuncGetName(p.func)
+        assert err == driver.CUresult.CUDA_SUCCESS
+        out.append((name.decode(), p.gridDimX * p.gridDimY * p.gridDimZ))
+    return out
+
+
+@pytest.mark.parametrize("budget", [1, 7, 40, 100])
+@pytest.mark.parametrize("q", [1, 4, 8, 90])
+def test_attention_keeps_to_the_sm_budget(budget, q):
+    """A CTA per SM of the budget: CTAs go to free SMs first, also where two fit one SM."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        own = L.Context(0, stream=stream)
+        own.set_sm_budget(budget)
+        p = Paged([q] * 40, [300, 2000, q, 700, 1500] * 8, 8, 2, 128, 32, BF16, seed=q)
+        p.check(own)
+        cu = ints([0, 15 * q, 40 * q])
+        k, v = randn(1, p.t, 2, 128), randn(2, p.t, 2, 128)
+    torch.cuda.synchronize()
+    paged = captured_kernels(stream, lambda: L.attention_paged(
+        own, p.q, p.kc, p.vc, p.o, p.cu, p.kv, p.table, scale=0.1, max_q_len=q))
+    causal = captured_kernels(stream, lambda: L.attention_causal(own, p.q, k, v, p.o, cu, scale=0.1))
+    seen = [(n, ctas) for n, ctas in paged + causal if "join" not in n]
+    assert len(seen) == 2 and all(ctas <= budget for _, ctas in seen), seen
+    own.close()
