@@ -85,7 +85,8 @@ struct FaRowsParams {
   int dynamic;            // prompts: units are taken over by cluster launch control
   int shares;             // prompts: CTAs that units are dealt out to if an offset is bad
   float scale_log2;
-  float *part_o, *part_lse;  // paged: [2 * CTA + 0 / 1][256 rows]([D])
+  float *part_o;    // paged: [2 * CTA + 0 / 1][256 rows][D], relative to the part's maximum
+  float2 *part_ml;  // paged: [2 * CTA + 0 / 1][256 rows] (maximum, sum), in powers of 2
   FaJoin *joins;             // paged: [CTA]
 };
 
@@ -931,18 +932,16 @@ __global__ void __launch_bounds__(384, 1)
       }
       const int tok = row * p.recip >> 16, head = row - tok * p.group;
       const int t0 = un.dual ? 0 : t * p.tpt;          // the tile's first token
-      // A row that sees no key is 0 and -inf, and so is a part that adds nothing to
-      // its row. Scores that are all -inf are l = 0 too: 0 / 0 = NaN. (A NaN score
-      // is a NaN l.)
-      const bool none = un.part >= 0 ? l == 0.0f : un.pos + t0 + tok < 0;
-      const float inv = none ? 0.0f : 1.0f / l;
-      const float lse = none ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
+      // A row that sees no key (a prompt's sees its own) is 0 and -inf. Scores that
+      // are all -inf are l = 0 too: 0 / 0 = NaN. (A NaN score is a NaN l.)
+      const int part_at = PAGED ? un.part : -1;
+      const bool none = PAGED && un.pos + t0 + tok < 0;
+      const float inv = part_at >= 0 ? 1.0f : none ? 0.0f : 1.0f / l;
       w0 *= inv;
       w1 *= inv;
       const int ntok = min(un.tokens - t0, p.tpt);  // its tokens (<= 0: none)
       const bool live = tok < ntok;
       const int kvh = un.kvh, q_row = un.q_row + t0;
-      const int part_at = un.part;
       __syncwarp();
       if (lane == 0) mbar_arrive(&u_empty[i % kUnitSlots]);
       if (ntok <= 0) continue;
@@ -984,7 +983,7 @@ __global__ void __launch_bounds__(384, 1)
           chunk(c, v);
           if (live) store_row_chunk<float>(p.part_o + r * D + c * 32, v);
         }
-        if (live) p.part_lse[r] = lse;
+        if (live) p.part_ml[r] = make_float2(m_used, l);
         continue;
       }
       // Stores of whole 128-byte row segments through the warp's staging
@@ -1022,7 +1021,8 @@ __global__ void __launch_bounds__(384, 1)
         __syncwarp();
       }
       if (p.rows.lse && live)
-        p.rows.lse[(long long)(kvh * p.group + head) * p.rows.tokens + q_row + tok] = lse;
+        p.rows.lse[(long long)(kvh * p.group + head) * p.rows.tokens + q_row + tok] =
+            none ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
     }
   }
 
@@ -1037,8 +1037,9 @@ __global__ void __launch_bounds__(384, 1)
 }
 
 // Joins the parts of the units that cuts fell into (paged): o = sum_s w_s o_s
-// with w_s = exp(lse_s) / sum exp(lse), parts in the order of the keys. One
-// CTA per (range, 32 of its unit's rows), a warp for 4 rows, 4 parts at a time
+// / sum_s w_s l_s with w_s = 2^(m_s - max m), parts in the order of the keys.
+// (Their log-sum-exps instead of (m, l) cost a row of large scores |lse| 2^-24 of
+// each weight.) One CTA per (range, 32 of its unit's rows), a warp for 4 rows, 4 parts at a time
 // so that their loads overlap; lane x first finds the weight of part x.
 template <int D, typename OutT>
 __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant__ FaRowsParams p) {
@@ -1059,7 +1060,7 @@ __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant
   for (int i = 0; i < ROWS; i++) mx[i] = -INFINITY;
   for (int x = lane; x < parts; x += 32)
 #pragma unroll
-    for (int i = 0; i < ROWS; i++) mx[i] = fmaxf(mx[i], p.part_lse[part_row(x, i)]);
+    for (int i = 0; i < ROWS; i++) mx[i] = fmaxf(mx[i], p.part_ml[part_row(x, i)].x);
 #pragma unroll
   for (int i = 0; i < ROWS; i++)
 #pragma unroll
@@ -1068,9 +1069,9 @@ __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant
     float w[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-      const float ls = x0 + lane < parts ? p.part_lse[part_row(x0 + lane, i)] : -INFINITY;
-      w[i] = ls == -INFINITY ? 0.0f : expf(ls - mx[i]);  // 0: adds nothing
-      sum[i] += w[i];
+      const float2 e = x0 + lane < parts ? p.part_ml[part_row(x0 + lane, i)] : make_float2(-INFINITY, 0.0f);
+      w[i] = e.x == -INFINITY ? 0.0f : ex2_approx(e.x - mx[i]);  // 0: adds nothing
+      sum[i] += w[i] * e.y;
     }
     const int n = min(32, parts - x0);
     for (int x = 0; x < n; x += U) {
@@ -1109,7 +1110,7 @@ __global__ void __launch_bounds__(256) fa_rows_join_kernel(const __grid_constant
     *reinterpret_cast<Pack<OutT, E> *>(static_cast<OutT *>(p.rows.o) + (long long)q_row * p.rows.os[0] +
                                        (long long)h * p.rows.os[1] + lane * E) = out;
     if (p.rows.lse && lane == 0)
-      p.rows.lse[(long long)h * p.rows.tokens + q_row] = mx[i] + logf(sum[i]);
+      p.rows.lse[(long long)h * p.rows.tokens + q_row] = (mx[i] + log2f(sum[i])) * 0.69314718055994531f;
   }
 }
 

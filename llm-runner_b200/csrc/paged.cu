@@ -88,10 +88,10 @@ const char *bad_paged(const llmr_paged_desc *d) {
   return nullptr;
 }
 
-// Workspace of the paged chunk kernel: two parts per CTA (O and log-sum-exp of
+// Workspace of the paged chunk kernel: two parts per CTA (O, maximum and sum of
 // 256 rows) and its unit to join.
 size_t chunk_parts_bytes(int D) {
-  return (size_t)kMaxRanges * (2 * 256 * (D + 1) * sizeof(float) + sizeof(FaJoin));
+  return (size_t)kMaxRanges * (2 * 256 * (D + 2) * sizeof(float) + sizeof(FaJoin));
 }
 
 template <int D, typename T, typename OutT, bool PAGED>
@@ -108,8 +108,8 @@ int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r) {
   if (PAGED) {
     grid = ctx->num_sms < kMaxRanges ? ctx->num_sms : kMaxRanges;
     p.part_o = static_cast<float *>(ctx->ws);
-    p.part_lse = p.part_o + (size_t)2 * kMaxRanges * 256 * D;
-    p.joins = reinterpret_cast<FaJoin *>(p.part_lse + (size_t)2 * kMaxRanges * 256);
+    p.part_ml = reinterpret_cast<float2 *>(p.part_o + (size_t)2 * kMaxRanges * 256 * D);
+    p.joins = reinterpret_cast<FaJoin *>(p.part_ml + (size_t)2 * kMaxRanges * 256);
   } else {
     // Fewer units than SMs: units of one tile, whose keys both softmax groups
     // share, so that a unit takes half as long and there are twice as many.

@@ -1133,3 +1133,34 @@ def test_attention_keeps_to_the_sm_budget(budget, q):
     seen = [(n, ctas) for n, ctas in paged + causal if "join" not in n]
     assert len(seen) == 2 and all(ctas <= budget for _, ctas in seen), seen
     own.close()
+
+
+# ------------------------------------------------------------- joins of large scores
+
+@pytest.mark.parametrize("q", [1, 8, 20, 130])
+@pytest.mark.parametrize("kv", [3001, 9000, 20011])
+@pytest.mark.parametrize("d", [64, 128])
+def test_joins_of_large_scores(ctx, q, kv, d):
+    """Every score is 30720, so all keys weigh the same, and V is 1 in the first half and -1 in
+    the second: what the parts of a split row weigh against one another shows alone."""
+    p = Paged([q], [kv], 8, 2, d, 16, F16, seed=3)
+    p.q.zero_()
+    p.q[..., 0] = 256
+    for x, c in ((p.kc, p.k), (p.vc, p.v)):
+        x.zero_()
+        c[0].zero_()
+    p.kc[..., 0] = 120
+    p.k[0][..., 0] = 120
+    p.v[0][:kv // 2] = 1
+    p.v[0][kv // 2:] = -1
+    at = torch.arange(kv, device="cuda")
+    p.vc[p.table[0].long()[at // 16], at % 16] = p.v[0]
+    o = p.run(ctx, out_dtype=F32, scale=1.0).double()
+    w, wl, _ = R.rows_attention(p.q, p.k[0], p.v[0], 1.0)
+    # The numerators are one value c 2^e of 11 bits, and O sums +-1 of them: exact (below
+    # 2^24 steps). l adds 32 of them at a time in fp32, then 4 such sums, then blocks of
+    # 128 keys: 40 + kv / 64 roundings at most, parts included. The rounding of c itself is
+    # common to all keys, half a step of o.
+    tol = (40 + kv / 64) * 2.0 ** -24 + w.abs() * R.half_step(F16)
+    assert ((o - w).abs() <= tol).all(), ((o - w).abs() / tol).max().item()
+    assert ((p.lse.double() - wl).abs() <= 2.0 ** -23 * wl).all()
