@@ -1164,3 +1164,161 @@ def test_joins_of_large_scores(ctx, q, kv, d):
     tol = (40 + kv / 64) * 2.0 ** -24 + w.abs() * R.half_step(F16)
     assert ((o - w).abs() <= tol).all(), ((o - w).abs() / tol).max().item()
     assert ((p.lse.double() - wl).abs() <= 2.0 ** -23 * wl).all()
+
+
+# ------------------------------------------------------- large plans, four places a thread
+
+def check_large_plan(ctx, ctx_lens, new_lens, page, room, shift, inplace=False):
+    """A plan whose positions and slots begin `shift` elements behind a 16-byte boundary."""
+    held = [-(-c // page) for c in ctx_lens]
+    last = [-(-(c + n) // page) for c, n in zip(ctx_lens, new_lens)]
+    need, n = sum(last) - sum(held), len(ctx_lens)
+    order = torch.randperm(sum(held) + need + 9, generator=torch.Generator().manual_seed(room)).tolist()
+    table, at = [], 0
+    for a in held:
+        table.append(order[at:at + a] + [-1] * (max(last) - a))
+        at += a
+    free = order[at:]
+    dev, c, nf, fp = ints(table), ints(ctx_lens), ints([len(free)]), ints(free)
+    pos, slots = (torch.full((room + 8,), -55, dtype=torch.int32, device="cuda") for _ in range(2))
+    cu = torch.full((n + 1,), -55, dtype=torch.int32, device="cuda")
+    kv, nfo = (c, nf) if inplace else (torch.zeros_like(c), torch.zeros_like(nf))
+    L.paged_plan(ctx, c, ints(new_lens), fp, nf, dev, cu, kv, pos[shift:shift + room], slots[shift:shift + room],
+                 nfo, page_size=page, num_pages=len(order))
+    ctx.sync()
+    want = R.plan(ctx_lens, new_lens, free, table, page, room)
+    got = [x.cpu().tolist() for x in (dev, cu, kv, pos[shift:shift + room], slots[shift:shift + room])]
+    assert (*got, int(nfo)) == want
+    for x in (pos, slots):      # nothing beside the arrays
+        assert (x[:shift] == -55).all() and (x[shift + room:] == -55).all()
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("over", [0, 1, 2, 3])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+def test_large_plan(ctx, page, over, shift):
+    """More than 32768 places: four of a thread across requests' borders, a ragged end."""
+    g = torch.Generator().manual_seed(4 * over + shift)
+    new = [0, 1, 1, 1, 0, 0, 2, 1, 9000, 0, 3, 1, 1, 20000, 5, 0, 1] + torch.randint(0, 3, (600,), generator=g).tolist()
+    new += [4001 - shift, 0, 0]
+    ctx_lens = torch.randint(0, 300, (len(new),), generator=g).tolist()
+    ctx_lens[8], ctx_lens[13] = page, page - 1
+    room = (max(sum(new), 32768) + 4) // 4 * 4 + 4 + over
+    check_large_plan(ctx, ctx_lens, new, page, room, shift, inplace=over == 1)
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_large_plan_that_fills_its_places(ctx, shift):
+    """No place behind the last token, and one request alone."""
+    for total in (32769, 40002, 65536):
+        check_large_plan(ctx, [77], [total], 64, total, shift)
+        check_large_plan(ctx, [3] * (total // 8) if total // 8 <= 4096 else [3] * 4096,
+                         [8] * min(total // 8, 4096), 16, max(total, 32769), shift)
+
+
+def test_large_plan_reports_a_bad_page(ctx):
+    """One table entry and one free page out of range: their tokens get no slot, the others do."""
+    page, c, new = 64, [100, 0, 200], [30000, 100, 9000]
+    held = [2, 0, 4]
+    need = [-(-30100 // page) - 2, 2, -(-9200 // page) - 4]
+    order = list(range(sum(held) + sum(need)))
+    table = [order[:2] + [-1] * (need[0] + 2), [-1] * (need[0] + 4), order[2:6] + [-1] * need[0]]
+    free = order[6:]
+    bad_free = len(free) - 1 - (need[0] + 1)      # the second request's second page
+    free[bad_free] = 1 << 20
+    table[2][3] = -4                              # where the third's tokens begin
+    room = sum(new) + 5
+    dev, cu, kv, pos, slots, nfo = (ints(x) for x in (table, [0] * 4, [0] * 3, [0] * room, [0] * room, [0]))
+    L.paged_plan(ctx, ints(c), ints(new), ints(free), ints([len(free)]), dev, cu, kv, pos, slots, nfo,
+                 page_size=page, num_pages=len(order))
+    assert statuses(ctx) == [L.EINVAL]
+    want = R.plan(c, new, free, table, page, room)
+    slot = [s if 0 <= s < len(order) * page else -1 for s in want[4]]
+    assert slots.tolist() == slot and slot.count(-1) == 5 + (100 - 64) + (256 - 200)
+    assert pos.tolist() == want[3] and cu.tolist() == want[1]
+
+
+# ------------------------------------------- which V a split row meets, block by block
+
+def paged_v(p, i, kv, v):
+    """Puts v [kv, heads, D] into request i's pages."""
+    at = torch.arange(kv, device="cuda")
+    page = p.vc.shape[1]
+    p.vc[p.table[i].long()[at // page], at % page] = v
+
+
+@pytest.mark.parametrize("q", [1, 8, 20, 130])
+@pytest.mark.parametrize("h,hk,d", [(8, 2, 128), (4, 1, 64)])
+def test_every_block_of_v_counts(ctx, q, h, hk, d):
+    """V is zero but for 64 keys at a time, so a block that is lost, doubled or swapped at a border
+    of a range, a page or a tile is the whole result."""
+    kv = 20011
+    p = Paged([q], [kv], h, hk, d, 16, BF16, seed=5)
+    x = torch.einsum("nhd,mhd->hnm", p.q.double(), p.k[0].double().repeat_interleave(h // hk, 1)) * d ** -0.5
+    at = torch.arange(kv, device="cuda")
+    x = x.masked_fill(at[None] > kv - q + torch.arange(q, device="cuda")[:, None], -math.inf)
+    prob = torch.softmax(x, -1)
+    v = p.v[0].clone()
+    smax = R.score_size(p.q, p.k[0], d ** -0.5)
+    worst = 0.0
+    for b in range(0, kv, 64):
+        part = slice(b, min(b + 64, kv))
+        one = torch.zeros_like(v)
+        one[part] = v[part]
+        paged_v(p, 0, kv, one)
+        o = p.run(ctx).double()
+        wide = v[part].double().repeat_interleave(h // hk, 1)
+        w, weight = (torch.einsum("hnm,mhd->nhd", prob[..., part], y) for y in (wide, wide.abs()))
+        bound = R.attention_bound(w, weight, BF16, BF16, d, kv, float(v.abs().max()), smax)
+        worst = max(worst, ((o - w).abs() / bound).max().item())
+        assert worst <= 1, (b, worst)
+        assert bound[-1].mean() < 0.05 * weight[-1].mean()    # (a lost block would show)
+
+
+@pytest.mark.parametrize("q", [1, 5, 60])
+def test_every_block_of_v_counts_in_a_batch(ctx, q):
+    """The same over many requests: V of every seventh block of 64 keys, in turn."""
+    kv = [700, 5000, 64, 8191, 2, 129, 3000, 6000, 300, 4097]
+    kv = [max(q, n) for n in kv]
+    p = Paged([q] * len(kv), kv, 8, 2, 128, 32, BF16, seed=6)
+    full = [v.clone() for v in p.v]
+    for turn in range(7):
+        for i, n in enumerate(kv):
+            keep = (torch.arange(n, device="cuda") // 64 % 7 == turn)[:, None, None]
+            p.v[i] = torch.where(keep, full[i], 0)
+            paged_v(p, i, n, p.v[i])
+        p.check(ctx)
+
+
+# ------------------------------------------------------------------- strided paged calls
+
+@pytest.mark.parametrize("q", [1, 4, 8, 90])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+def test_paged_strides(ctx, q, d, out_dtype):
+    """q inside a fused projection and head-major, o with gaps, with heads outside and flat, and a
+    block table that is part of a wider one."""
+    h, hk = 8, 2
+    p = Paged([q, 0, q + 1, q], [700, 40, 3000, q], h, hk, d, 16, BF16, pad=2, seed=q)
+    want = p.check(ctx, out_dtype=out_dtype).clone()
+    want_lse = p.lse.clone()
+    fused = randn(9, p.t, (h + 2 * hk) * d)
+    fused[:, :h * d] = p.q.flatten(1)
+    major = p.q.transpose(0, 1).contiguous().transpose(0, 1)
+    spread = torch.zeros((p.t, h, d + 64), dtype=BF16, device="cuda")
+    spread[..., :d] = p.q
+    wide_table = torch.full((4, p.table.shape[1] + 9), 1 << 20, dtype=torch.int32, device="cuda")
+    cols = slice(3, 3 + p.table.shape[1])
+    wide_table[:, cols] = p.table
+    for query in (fused[:, :h * d].unflatten(1, (h, d)), major, spread[..., :d]):
+        flat = torch.full((p.t, h * d + 64), 7.0, dtype=out_dtype, device="cuda")
+        outer = torch.full((h, p.t, d), 7.0, dtype=out_dtype, device="cuda")
+        gaps = torch.full((p.t, h, d + 64), 7.0, dtype=out_dtype, device="cuda")
+        for o, got in ((flat[:, :h * d], flat[:, :h * d].unflatten(1, (h, d))),
+                       (outer.transpose(0, 1), outer.transpose(0, 1)), (gaps[..., :d], gaps[..., :d])):
+            lse = torch.full((h, p.t), 7.0, device="cuda")
+            L.attention_paged(ctx, query, p.kc, p.vc, o, p.cu, p.kv, wide_table[:, cols], scale=d ** -0.5,
+                              max_q_len=q + 1, lse=lse)
+            ctx.sync()
+            assert torch.equal(got, want) and torch.equal(lse, want_lse)
+        assert (flat[:, h * d:] == 7).all() and (gaps[..., d:] == 7).all()
