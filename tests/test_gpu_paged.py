@@ -1322,3 +1322,42 @@ def test_paged_strides(ctx, q, d, out_dtype):
             ctx.sync()
             assert torch.equal(got, want) and torch.equal(lse, want_lse)
         assert (flat[:, h * d:] == 7).all() and (gaps[..., d:] == 7).all()
+
+
+# ------------------------------------------------- a prompt that is not cached, both steps
+
+@pytest.mark.parametrize("h,hk,d,half", [(8, 2, 128, True), (14, 2, 64, False)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_uncached_prompts_norm_rope_and_attention(ctx, h, hk, d, half, dtype):
+    """Norm + RoPE into dense q and k: the prologue with slots 0 .. tokens - 1 and dense buffers as a
+    cache, which attention_causal then reads."""
+    lens, page = [77, 1, 300, 45], 16
+    t = sum(lens)
+    rows = -(-t // page) * page
+    fused = randn(1, t, (h + 2 * hk) * d, dtype=dtype)
+    q, k, v = (x.unflatten(1, (-1, d)) for x in fused.split((h * d, hk * d, hk * d), 1))
+    angle = torch.arange(400)[:, None].double() * 10000.0 ** (-torch.arange(0, d, 2).double() / d)
+    cos, sin = angle.cos().float().cuda(), angle.sin().float().cuda()
+    gains = [torch.rand(d, generator=torch.Generator().manual_seed(i)).cuda() + 0.5 for i in range(2)]
+    pos = torch.cat([torch.arange(n) for n in lens]).int().cuda()
+    slots = torch.arange(t, dtype=torch.int32, device="cuda")
+    q_rot = torch.zeros((t, h, d), dtype=dtype, device="cuda")
+    k_rot, v_rot = (torch.zeros((rows, hk, d), dtype=dtype, device="cuda") for _ in range(2))
+    L.paged_prologue(ctx, q, k, v, q_rot, k_rot.view(-1, page, hk, d), v_rot.view(-1, page, hk, d), pos, slots,
+                     q_gain=gains[0], k_gain=gains[1], cos=cos, sin=sin, half=half)
+    o = torch.zeros_like(q_rot)
+    L.attention_causal(ctx, q_rot, k_rot[:t], v_rot[:t], o, ints(cumulative(lens)), scale=d ** -0.5)
+    ctx.sync()
+    for x, gain, got in ((q, gains[0], q_rot), (k, gains[1], k_rot[:t])):
+        w = R.rotate(R.norm(x, gain, 1e-6), cos[pos.long()], sin[pos.long()], half)
+        size = w.abs().amax(-1, keepdim=True)
+        tol = w.abs() * R.half_step(dtype) + size * (16 + d / 2) * 2.0 ** -24 + 2.0 ** -25
+        assert ((got.double() - w).abs() <= tol).all()
+    assert torch.equal(v_rot[:t], v)
+    at = 0
+    for n in lens:
+        part = slice(at, at + n)
+        w, _, weight = R.rows_attention(q_rot[part], k_rot[part], v[part], d ** -0.5)
+        R.check_attention(o[part], None, w, None, weight, dtype, d, n, float(v[part].abs().max()),
+                          R.score_size(q_rot[part], k_rot[part], d ** -0.5), at)
+        at += n
