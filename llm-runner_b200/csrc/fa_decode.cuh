@@ -39,14 +39,14 @@ constexpr int kDecodeBN = 64;     // keys per block
 template <int D, int RW>
 struct DecodeCfg {
   static constexpr int BN = kDecodeBN, WARPS = 4, THREADS = 32 * (WARPS + 1);
+  static_assert(RW == 1 || RW == 2, "one or two row tiles");
   static constexpr int KW = WARPS / RW, KEYS = BN / KW;  // a warp's keys of a block
-  static constexpr int SUB = KEYS < 32 ? KEYS : 32;      // its keys at a time
   static constexpr int ROWS = 16 * RW;
   static constexpr int NCHUNK = D / 64;
   static constexpr int CHUNK_BYTES = BN * 128;
   static constexpr int TILE_BYTES = BN * D * 2;
-  static constexpr int MERGE_BYTES = KW > 1 ? WARPS * 16 * D * 4 : 0;  // [warp][16 rows][D] fp32
-  static constexpr int NST = (KW > 1 ? 4 : 6) * (128 / D);
+  static constexpr int MERGE_BYTES = WARPS * 16 * D * 4;  // [warp][16 rows][D] fp32
+  static constexpr int NST = 4 * (128 / D);
   static constexpr int MERGE_OFF = NST * TILE_BYTES;
   static constexpr int ML_OFF = MERGE_OFF + MERGE_BYTES;  // [warp][16] (max, sum)
   static constexpr int CTL_OFF = ML_OFF + WARPS * 16 * 8;
@@ -378,31 +378,27 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
       const bool tail = key0 + C::BN > sg.nk - sg.nq + 1;  // some row may not see all keys
       const bool cut = key0 + C::BN > sg.nk;                // some key is behind the last
       if (idle) wait(&full[vslot], (used + 1) / C::NST);
-      // SUB keys at a time: their scores, P and product.
-#pragma unroll 1
-      for (int k1 = 0; k1 < C::KEYS && !idle; k1 += C::SUB) {
-        const int k0 = key0 + kw * C::KEYS + k1 + qc;  // this lane's first key
-        float s[C::SUB / 8][4] = {};
+      if (!idle) {
+        const int k0 = key0 + kw * C::KEYS + qc;  // this lane's first key
+        float s[C::KEYS / 8][4] = {};
 #pragma unroll
         for (int kk = 0; kk < D / 16; kk++)
 #pragma unroll
-          for (int h = 0; h < C::SUB / 16; h++) {
+          for (int h = 0; h < C::KEYS / 16; h++) {
             uint32_t b[4];
-            ldmatrix4(b, ring + kslot * C::TILE_BYTES + (krow + k1 + h * 16) * 128 + (kk >> 2) * C::CHUNK_BYTES +
+            ldmatrix4(b, ring + kslot * C::TILE_BYTES + (krow + h * 16) * 128 + (kk >> 2) * C::CHUNK_BYTES +
                              ((((kk & 3) * 2 + kpiece) ^ (krow & 7)) << 4));
             mma_16816<T>(s[2 * h], qf[kk], b[0], b[1]);
             mma_16816<T>(s[2 * h + 1], qf[kk], b[2], b[3]);
           }
-        if (k1 + C::SUB == C::KEYS) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&empty[kslot]);
-        }
-        uint32_t pf[C::SUB / 16][4];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[kslot]);
+        uint32_t pf[C::KEYS / 16][4];
 #pragma unroll
         for (int i = 0; i < 2; i++) {  // rows qa, qa + 8
           float top = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < C::SUB / 8; n++)
+          for (int n = 0; n < C::KEYS / 8; n++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               float &x = s[n][2 * i + e];
@@ -426,7 +422,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
           const float sub = mx[i] == -INFINITY ? 0.0f : mx[i];  // no key so far: all P are 0
           float part = 0.0f;
 #pragma unroll
-          for (int n = 0; n < C::SUB / 8; n++) {
+          for (int n = 0; n < C::KEYS / 8; n++) {
             const float x0 = ex2_approx(fmaf(s[n][2 * i], p.scale_log2, -sub));
             const float x1 = ex2_approx(fmaf(s[n][2 * i + 1], p.scale_log2, -sub));
             part += x0 + x1;
@@ -434,9 +430,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
           }
           sum[i] += part;
         }
-        if (k1 == 0) wait(&full[vslot], (used + 1) / C::NST);
+        wait(&full[vslot], (used + 1) / C::NST);
 #pragma unroll
-        for (int h = 0; h < C::SUB / 16; h++) {
+        for (int h = 0; h < C::KEYS / 16; h++) {
           // Values behind the last key may be anything: they count as 0.
           uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
           if (cut) {
@@ -449,7 +445,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
 #pragma unroll
           for (int n2 = 0; n2 < D / 16; n2++) {
             uint32_t b[4];
-            ldmatrix4_trans(b, ring + vslot * C::TILE_BYTES + (vrow + k1 + h * 16) * 128 +
+            ldmatrix4_trans(b, ring + vslot * C::TILE_BYTES + (vrow + h * 16) * 128 +
                                    (n2 >> 2) * C::CHUNK_BYTES +
                                    ((((n2 & 3) * 2 + vpiece) ^ (vrow & 7)) << 4));
             if (cut) {
@@ -487,60 +483,48 @@ __global__ void __launch_bounds__(DecodeCfg<D, RW>::THREADS, 2)
         if (col == 0) reinterpret_cast<float2 *>(part + C::ROWS * D)[r] = make_float2(top, l);
       }
     };
-    if constexpr (C::KW == 1) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int r = rw * 16 + qa + i * 8;
-        if (r < nrows) {
+    for (int i = 0; i < 2; i++)
+      if ((lane & 3) == 0) ml[warp * 16 + qa + i * 8] = make_float2(mx[i], sum[i]);
+    named_barrier(1, 32 * C::WARPS);
+    // Each share's O is brought to the rows' common maximum.
 #pragma unroll
-          for (int n = 0; n < D / 8; n++)
-            put(r, n * 8 + qc, make_float2(o[n][2 * i], o[n][2 * i + 1]), mx[i], sum[i]);
-        }
+    for (int i = 0; i < 2; i++) {
+      const int rr = qa + i * 8;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < C::KW; w++) top = fmaxf(top, ml[(rw * C::KW + w) * 16 + rr].x);
+      const float f = mx[i] == -INFINITY ? 0.0f : ex2_approx(mx[i] - top);
+      float *row = merge + (warp * 16 + rr) * D;
+      if (rw * 16 + rr < nrows) {
+#pragma unroll
+        for (int n = 0; n < D / 8; n++)
+          *reinterpret_cast<float2 *>(row + ((n * 8 + qc) ^ (qa << 3))) =
+              make_float2(o[n][2 * i] * f, o[n][2 * i + 1] * f);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-        if ((lane & 3) == 0) ml[warp * 16 + qa + i * 8] = make_float2(mx[i], sum[i]);
-      named_barrier(1, 32 * C::WARPS);
-      // Each share's O is brought to the rows' common maximum.
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int rr = qa + i * 8;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < C::KW; w++) top = fmaxf(top, ml[(rw * C::KW + w) * 16 + rr].x);
-        const float f = mx[i] == -INFINITY ? 0.0f : ex2_approx(mx[i] - top);
-        float *row = merge + (warp * 16 + rr) * D;
-        if (rw * 16 + rr < nrows) {
-#pragma unroll
-          for (int n = 0; n < D / 8; n++)
-            *reinterpret_cast<float2 *>(row + ((n * 8 + qc) ^ (qa << 3))) =
-                make_float2(o[n][2 * i] * f, o[n][2 * i + 1] * f);
-        }
-      }
-      named_barrier(1, 32 * C::WARPS);
-      for (int x = tid; x < nrows * (D / 4); x += 32 * C::WARPS) {
-        const int r = x / (D / 4), col = (x - r * (D / 4)) * 4;
-        const int w0 = (r >> 4) * C::KW, rr = r & 15;
-        float top = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < C::KW; w++) top = fmaxf(top, ml[(w0 + w) * 16 + rr].x);
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < C::KW; w++) {
-          const float2 e = ml[(w0 + w) * 16 + rr];
-          l += e.x == -INFINITY ? e.y : e.y * ex2_approx(e.x - top);  // (its sum is 0, or NaN)
-          const float4 v = *reinterpret_cast<const float4 *>(merge + ((w0 + w) * 16 + rr) * D +
-                                                             (col ^ ((rr & 7) << 3)));
-          acc.x += v.x;
-          acc.y += v.y;
-          acc.z += v.z;
-          acc.w += v.w;
-        }
-        put(r, col, acc, top, l);
-      }
-      named_barrier(1, 32 * C::WARPS);  // merge and ml may be written again
     }
+    named_barrier(1, 32 * C::WARPS);
+    for (int x = tid; x < nrows * (D / 4); x += 32 * C::WARPS) {
+      const int r = x / (D / 4), col = (x - r * (D / 4)) * 4;
+      const int w0 = (r >> 4) * C::KW, rr = r & 15;
+      float top = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < C::KW; w++) top = fmaxf(top, ml[(w0 + w) * 16 + rr].x);
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < C::KW; w++) {
+        const float2 e = ml[(w0 + w) * 16 + rr];
+        l += e.x == -INFINITY ? e.y : e.y * ex2_approx(e.x - top);  // (its sum is 0, or NaN)
+        const float4 v = *reinterpret_cast<const float4 *>(merge + ((w0 + w) * 16 + rr) * D +
+                                                           (col ^ ((rr & 7) << 3)));
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
+      }
+      put(r, col, acc, top, l);
+    }
+    named_barrier(1, 32 * C::WARPS);  // merge and ml may be written again
     if (b0 == 0 && !whole && tid == 0) {
       const long long end = range_begin(line, ctas, cta) + sg.at + kPairBlocks + sg.blocks - 1;
       p.joins[cta] = DecodeJoin{range_owner(line, ctas, end), sg.row0, sg.nq, sg.kvh};
