@@ -34,12 +34,21 @@ class OnDevice {
   bool ok_ = false, changed_ = false;
 };
 
-// An exception (the host is out of memory) ends as a status at the C boundary.
+// An exception (the host is out of memory) ends as a status at the C boundary,
+// with a message where there is memory for one.
+int out_of_memory(llmr_ctx *ctx) {
+  try {
+    return fail(ctx, LLMR_ENOMEM, "the host is out of memory");
+  } catch (...) {
+    if (ctx) ctx->err.clear();  // not an older call's
+    return LLMR_ENOMEM;
+  }
+}
 #define NO_THROW_BEGIN try {
-#define NO_THROW_END(ctx)        \
-  }                              \
-  catch (...) {                  \
-    return LLMR_ENOMEM;          \
+#define NO_THROW_END(ctx)      \
+  }                            \
+  catch (...) {                \
+    return out_of_memory(ctx); \
   }
 #define ENTER(ctx)                                   \
   if (!(ctx)) return LLMR_EINVAL;                    \
