@@ -40,12 +40,14 @@
 // zeroed in shared memory: what lies behind a request's keys may be NaN.
 //
 // Bound by the tensor pipe at the rate of M = 128, N = 128 instructions (about
-// 68 % of dense) where there are many blocks: 8192 tokens, 32 / 8 heads of 128
-// in 445 us = 1235 TFLOP/s of the causal flops; heads of 64 in 366 us (P V of
-// N = 64 costs what N = 128 does). The issuing lane must not add to that: with a
-// descriptor built and a lane elected per instruction the same took 481 and
-// 411 us (with part of the exponentials on the FMA pipe, which costs 3 %). 6 chunks of 300 - 700 tokens behind 2k - 12k keys: 267 us. Bound by its
-// start and the unit boundary (8.2 us for 77 tokens) where there are few.
+// 68 % of dense) where there are many blocks. Device time of ten calls in a row:
+// 8192 tokens, 32 / 8 heads of 128, 438 us = 1256 TFLOP/s of the causal flops;
+// heads of 64 362 us (P V of N = 64 costs what N = 128 does); 6 chunks of 300 -
+// 700 tokens behind 2k - 12k keys 258 us. Many more calls in a row run under the
+// power cap (the 8192 tokens then take 514 us, the chunks 312). The issuing lane
+// must not add to that: with a descriptor built and a lane elected per
+// instruction the 8192 tokens took 8 % longer, with heads of 64 12 %. Where there
+// are few blocks, bound by its start and the unit boundary (77 tokens: 8.2 us).
 //
 // Scores and softmax state are fp32, P is rounded to the inputs' type (half
 // a step, the rounding V's own type has; fp32 P would need a tf32 product at
@@ -58,11 +60,12 @@ namespace llmr {
 
 constexpr int kUnitSlots = 2;  // the unit in work and the next
 constexpr int kMaxRanges = 160;  // CTAs of a paged call (workspace)
-// What a unit costs besides its keys, in keys (128 to 512 differ by 3 %);
+// What a unit costs besides its keys, in keys (24 x 5 drafted tokens: 256 38.0 us,
+// 128 39.2, 512 39.1; 200 tokens over 1500 keys 28.5, 28.3, 29.8);
 // blocks of 128 that a cut keeps away from a unit's ends (a part costs about
-// two blocks to write and join; 6 took 200 tokens over 1500 keys from 32 to
-// 41 us); least keys of a range (with 1024, 20 tokens over 100 keys, 8 small
-// units, ran on two SMs: 24.6 us instead of 14).
+// two blocks to write and join; 6 took the 200 tokens from 28.5 to 37.6 us and
+// the drafted ones from 38.0 to 41.2); least keys of a range (with 1024, 20 tokens
+// over 100 keys, 8 small units, ran on two SMs: 20.7 us instead of 12.7).
 constexpr int kUnitKeys = 256;
 constexpr int kCutBlocks = 3;
 constexpr int kRangeKeys = 256;
@@ -859,8 +862,8 @@ __global__ void __launch_bounds__(384, 1)
           m_used = m_tgt;
         }
         // P = 2^(s*scale*log2e - m), every one by ex2 (the non-causal kernel takes
-        // a quarter on the FMA pipe; here that costs 3 %: 8192 tokens 458 us
-        // instead of 445, and a masked score would not reach 0 there).
+        // a quarter on the FMA pipe; here that took 8192 tokens 3 % longer, and a
+        // masked score would not reach 0 there).
         uint64_t part2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
         const uint64_t sl2x2 = f2_pack(sl2, sl2);
         const float m_sub = m_used == -INFINITY ? 0.0f : m_used;  // no key so far: all P are 0

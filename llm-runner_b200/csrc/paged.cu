@@ -122,9 +122,11 @@ int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r) {
   } else {
     // Fewer units than SMs: units of one tile, whose keys both softmax groups
     // share, so that a unit takes half as long and there are twice as many.
-    // 1500 tokens, 14 / 2 heads of 64: 20.1 us instead of 28.1; with more units
-    // than SMs reading K and V for one tile costs more than that gains (1500
-    // tokens, 32 / 8 heads of 128: 39 us instead of 35).
+    // 1500 tokens, 14 / 2 heads of 64: 17.0 us instead of 25.1; 700 tokens, 32 / 8
+    // heads of 128: 15.5 and 18.9. With more units than SMs reading K and V for
+    // one tile mostly costs more than that gains (1500 tokens, 32 / 8 heads of
+    // 128: 33.3 us instead of 30.1), but not just above one unit per SM (3000
+    // tokens, 14 / 2 heads of 64, 167 units: 37.7 and 43.8).
     if ((long long)r.tokens / (2 * p.tpt) * r.Hk < ctx->total_sms) p.tu = p.tpt;
     const long long vt = (long long)r.tokens / p.tu + r.n, units = vt * r.Hk;
     if (units > 0x7fffffffLL) return fail(ctx, LLMR_EINVAL, "problem too large");
@@ -159,7 +161,8 @@ int launch_fa_rows(llmr_ctx *ctx, const RowsParams &r) {
                 "register split", regs);
   if constexpr (!PAGED) {
     // (Overlapped with the call before, ragged prompts took 9 % longer: CTAs of
-    // two grids that both take over units.)
+    // two grids that both take over units. Grids that do not take over units were
+    // not measured overlapped.)
     kern<<<grid, C::THREADS, C::SMEM_BYTES, ctx->stream>>>(mq, mk, mv, p);
     return after_launch(ctx, "fa_rows");
   } else {
@@ -187,9 +190,9 @@ int launch_fa_rows_any(llmr_ctx *ctx, int D, llmr_dtype dt, llmr_dtype od, const
 }
 
 // Query rows per (request, key/value head) up to which the decode kernel runs.
-// 32 requests over 4096 keys, 8 key/value heads of 128: 32 rows 96 us there and
-// 110 us in fa_rows, 48 rows 172 and 112; one request over 32768: 35 and 42, 98
-// and 43.
+// 32 requests over 4096 keys, 8 key/value heads of 128: 32 rows 95 us there and
+// 106 us in fa_rows; one request over 32768: 33.6 and 38.4. (48 rows, in a form
+// that held up to 64, took 172 us and 112; one request 98 and 43.)
 constexpr uint32_t kDecodeRows = 32;
 
 uint32_t rows_per_head(const llmr_paged_desc *d) {

@@ -16,8 +16,9 @@ namespace llmr {
 // prefixes of n and need over the requests give every token and every fresh
 // page its place, so tokens and pages are then written independently of one
 // another: page x of the step (request order) is free_pages[n_free - 1 - x].
-// Latency is all that counts (a decode step moves a few KB: 256 requests 4.6 us,
-// 48 prompts of 96k tokens 8.9 us), so it is one launch: a cluster of 1 to 8 CTAs, each of which scans all requests itself
+// Latency is all that counts (a decode step moves a few KB: 256 requests 4.0 us
+// of device time, 48 prompts of 96k tokens 8.6 us, issue on 8 SMs), so it is one
+// launch: a cluster of 1 to 8 CTAs, each of which scans all requests itself
 // (cheaper than handing the prefixes over) and writes its share of the tokens
 // and pages. All reads of arrays that may be written in place come before the
 // cluster barrier, all writes after it.
@@ -217,9 +218,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_plan_kernel(const PlanP
 // a lane and every access is 16 bytes. A warp takes kRopeSteps rows per
 // group of ONE token, all loads issued before the first use. Small CTAs leave a
 // choice of register limits: 28 warps per SM at 72 registers. 8191 tokens, 32 / 8
-// heads of 128: 46 us, 4.5 TB/s; of 64: 23 us; 2000 tokens of 128: 11.1. 32 warps at
-// 64 registers (spills at heads of 64): 45, 24 and 12.1 us; in CTAs of 256 threads 49
-// and 26 at 8191. Rows per group in CTAs of 256, 8191 tokens of 128: 4 took 64 us (two
+// heads of 128: 46 us, 4.5 TB/s; of 64: 23 us; 2000 tokens of 128: 10.9. 32 warps at
+// 64 registers (spills at heads of 64): 45, 24 and 12.1 us; 24 warps at 80: 49.5, 24.3
+// and 11.2; in CTAs of 256 threads 49 and 26 at 8191. From fp32 (4 bytes of spill at
+// 72 registers) 48.8, 26.6 and 11.7 us = 6.2 TB/s; 24 warps, no spill: 50.2, 26.9, 11.5. Rows per group in CTAs of 256, 8191 tokens of 128: 4 took 64 us (two
 // CTAs per SM), 1 took 55 (six).
 constexpr int kRopeSteps = 2;
 constexpr int kRopeThreads = 64, kRopeCtas = 14;  // CTAs per SM
