@@ -488,7 +488,7 @@ typedef struct {
   llmr_dtype out_dtype; /* of o */
   float scale;
   uint32_t page_size, num_pages;
-  uint32_t max_pages;       /* columns of block_table */
+  uint32_t max_pages;       /* columns of block_table; * page_size at most 2^31 - 256 */
   uint64_t table_stride;    /* elements between rows of block_table; 0 = max_pages */
   uint64_t q_row_stride, o_row_stride, q_head_stride, o_head_stride;
   uint64_t k_page_stride, k_row_stride, k_head_stride;

@@ -91,8 +91,9 @@ const char *bad_paged(const llmr_paged_desc *d) {
   if (!is16(d->dtype) || !known(d->out_dtype)) return "q and the caches must be fp16 or bf16";
   if (!(d->scale > 0.0f) || !isfinite(d->scale)) return "scale must be finite and > 0";
   if (d->n_seqs > 0x3fffffffu || d->total_tokens > 0x3fffffffu) return "problem too large";
-  if (d->max_pages < 1 || (uint64_t)d->max_pages * d->page_size > 0x7fffffffull)
-    return "max_pages must be at least 1 and max_pages * page_size below 2^31";
+  // (A length rounded up to a block of keys, and the end of its last block, are ints.)
+  if (d->max_pages < 1 || (uint64_t)d->max_pages * d->page_size > 0x7fffff00ull)
+    return "max_pages must be at least 1 and max_pages * page_size at most 2^31 - 256";
   if (d->table_stride && d->table_stride < d->max_pages) return "table_stride is below max_pages";
   return nullptr;
 }

@@ -152,3 +152,15 @@ def test_prologue_refuses(change, word):
     refused(lambda: L.paged_prologue(NoDevice(0 if not change else -1), a["q"], a["k"], a["v"], a["q_out"], a["kc"], a["vc"], a["pos"],
                                      a["slots"], q_gain=a["q_gain"], k_gain=a["k_gain"], cos=a["cos"],
                                      sin=a["sin"], half=True), word)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_the_longest_context(page):
+    """Lengths of more than 2^31 - 256 keys are refused: rounded up to a block of 128 they pass an int."""
+    def size(max_pages):
+        d = L.PagedDesc(n_seqs=1, total_tokens=1, max_q_len=1, n_heads=4, n_kv_heads=1, head_dim=64,
+                        dtype=L.F16, out_dtype=L.F16, scale=1.0, page_size=page, num_pages=4,
+                        max_pages=max_pages)
+        return L.lib.llmr_attention_paged_workspace_bytes(ctypes.byref(d))
+    most = (2 ** 31 - 256) // page
+    assert size(most) > 0 and size(most + 1) == 0
