@@ -278,6 +278,8 @@ class Context:
         self.check(lib.llmr_ctx_set_sm_budget(self.handle, sms))
 
     def sync(self) -> None:
+        """Waits for the stream; raises LlmrError for one condition that kernels met (a
+        time-out, missing pages, a bad value in device memory). Others stay for the next call."""
         self.check(lib.llmr_sync(self.handle))
 
     def profile(self, on: bool = True) -> None:
