@@ -41,13 +41,13 @@
 //
 // Bound by the tensor pipe at the rate of M = 128, N = 128 instructions (about
 // 68 % of dense) where there are many blocks. Device time of ten calls in a row:
-// 8192 tokens, 32 / 8 heads of 128, 438 us = 1256 TFLOP/s of the causal flops;
-// heads of 64 362 us (P V of N = 64 costs what N = 128 does); 6 chunks of 300 -
+// 8192 tokens, 32 / 8 heads of 128, 434 us = 1268 TFLOP/s of the causal flops;
+// heads of 64 363 us (P V of N = 64 costs what N = 128 does); 6 chunks of 300 -
 // 700 tokens behind 2k - 12k keys 258 us. Many more calls in a row run under the
-// power cap (the 8192 tokens then take 514 us, the chunks 312). The issuing lane
+// power cap (the 8192 tokens then take 508 us, the chunks 307). The issuing lane
 // must not add to that: with a descriptor built and a lane elected per
 // instruction the 8192 tokens took 8 % longer, with heads of 64 12 %. Where there
-// are few blocks, bound by its start and the unit boundary (77 tokens: 8.2 us).
+// are few blocks, bound by its start and the unit boundary (77 tokens: 8.0 us).
 //
 // Scores and softmax state are fp32, P is rounded to the inputs' type (half
 // a step, the rounding V's own type has; fp32 P would need a tf32 product at
@@ -940,6 +940,7 @@ __global__ void __launch_bounds__(384, 1)
       const int part_at = PAGED ? un.part : -1;
       const bool none = PAGED && un.pos + t0 + tok < 0;
       const float inv = part_at >= 0 ? 1.0f : none ? 0.0f : 1.0f / l;
+      const float lse = none ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
       w0 *= inv;
       w1 *= inv;
       const int ntok = min(un.tokens - t0, p.tpt);  // its tokens (<= 0: none)
@@ -1024,8 +1025,7 @@ __global__ void __launch_bounds__(384, 1)
         __syncwarp();
       }
       if (p.rows.lse && live)
-        p.rows.lse[(long long)(kvh * p.group + head) * p.rows.tokens + q_row + tok] =
-            none ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
+        p.rows.lse[(long long)(kvh * p.group + head) * p.rows.tokens + q_row + tok] = lse;
     }
   }
 
