@@ -1361,3 +1361,115 @@ def test_uncached_prompts_norm_rope_and_attention(ctx, h, hk, d, half, dtype):
         R.check_attention(o[part], None, w, None, weight, dtype, d, n, float(v[part].abs().max()),
                           R.score_size(q_rot[part], k_rot[part], d ** -0.5), at)
         at += n
+
+
+# ------------------------------------------- overlapped starts behind other kinds of work
+
+@pytest.mark.parametrize("max_q", [1, 160])
+@pytest.mark.parametrize("captured", [False, True])
+def test_steps_wait_for_copies_and_other_streams(max_q, captured):
+    """A step's kernels start while the one before ends; here that is a copy, a memset, or a wait for
+    late work of another stream, between calls of the library and in a capture."""
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(main):
+        ctx = L.Context(0, stream=main)
+        plain, mixed = Server(ctx), Server(ctx)
+        for s in (plain, mixed):
+            feed(s, 0)
+            s.step(s.room)
+        ctx.sync()
+        late_new, late_qkv = torch.zeros_like(mixed.new), torch.zeros_like(mixed.qkv)
+        late_lens = torch.zeros_like(mixed.lens)
+
+    def step():
+        # Behind library kernels (the step before): a memset, then inputs that another stream makes late.
+        mixed.o.zero_()
+        fork = torch.cuda.Event()
+        fork.record(main)
+        with torch.cuda.stream(side):
+            side.wait_event(fork)
+            torch.cuda._sleep(2_000_000)
+            mixed.new.copy_(late_new)
+            mixed.qkv.copy_(late_qkv)
+            join = torch.cuda.Event()
+            join.record(side)
+        main.wait_event(join)
+        mixed.step(max_q)
+        # A copy between two library kernels: its target is the next call's input.
+        mixed.lens.add_(1)
+        mixed.lens.sub_(1)
+        late_lens.copy_(mixed.lens)
+
+    with torch.cuda.stream(main):
+        if captured:
+            state = [x.clone() for x in (mixed.lens, mixed.n_free, mixed.table)]
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=main):
+                step()
+            for x, y in zip((mixed.lens, mixed.n_free, mixed.table), state):
+                x.copy_(y)
+        for i in (2, 4, 5):
+            feed(plain, i)
+            late_new.copy_(plain.new)
+            late_qkv.copy_(plain.qkv)
+            plain.o.zero_()
+            plain.step(max_q)
+            g.replay() if captured else step()
+            ctx.sync()
+            assert torch.equal(plain.o, mixed.o) and torch.equal(plain.lens, mixed.lens)
+            assert torch.equal(plain.table, mixed.table) and torch.equal(late_lens, mixed.lens)
+    torch.cuda.synchronize()
+    if captured:
+        del g
+    ctx.close()
+
+
+def test_prompts_and_paged_calls_in_turn(ctx):
+    """Grids with and without an overlapped start behind one another, each reading what the one before
+    wrote: prologue, prompts, a paged call over the same keys."""
+    h, hk, d, t = 8, 2, 128, 300
+    q, k, v = (randn(i, t, n, d) for i, n in ((1, h), (2, hk), (3, hk)))
+    gain = torch.rand(d, generator=torch.Generator().manual_seed(1)).cuda() + 0.5
+    rows = 304
+    table = torch.arange(rows // 16, dtype=torch.int32, device="cuda").view(1, -1)
+    slots, cu, lens = torch.arange(t, dtype=torch.int32, device="cuda"), ints([0, t]), ints([t])
+    ctx.reserve(L.attention_paged_workspace_bytes(n_seqs=1, total_tokens=t, max_q_len=t, n_heads=h,
+                                                  n_kv_heads=hk, head_dim=d))
+    first = None
+    for turn in range(12):
+        q_rot = torch.full_like(q, math.nan)
+        kc, vc = (torch.full((rows // 16, 16, hk, d), math.nan, dtype=BF16, device="cuda") for _ in range(2))
+        a, b, c = (torch.full_like(q, math.nan) for _ in range(3))
+        for o in (a, c):
+            L.paged_prologue(ctx, q, k, v, q_rot, kc, vc, None, slots, q_gain=gain, k_gain=gain)
+            L.attention_causal(ctx, q_rot, kc.view(-1, hk, d)[:t], vc.view(-1, hk, d)[:t], o, cu, scale=d ** -0.5)
+        L.attention_paged(ctx, q_rot, kc, vc, b, cu, lens, table, scale=d ** -0.5, max_q_len=t)
+        ctx.sync()
+        first = first or (a, b)
+        assert torch.equal(a, first[0]) and torch.equal(c, first[0]) and torch.equal(b, first[1])
+        # (half a step each of both kernels' numerators and outputs)
+        assert (a.double() - b.double()).abs().max() <= 4 * R.half_step(BF16) * float(v.abs().max())
+
+
+@pytest.mark.parametrize("q", [1, 90])
+def test_paged_and_fused_calls_share_a_workspace(ctx, q):
+    """The fused attention call stages its operands where the paged call keeps its parts."""
+    from llmr_attn import configs as C
+    from llmr_attn.runner import to_device
+    dit = to_device(C.prepare(C.C3, L.rope_tables, seq_len=640, n_heads=2), out_dtype="f32")
+    ctx.reserve(L.workspace_bytes(dit.desc()))
+    p = Paged([q] * 3, [3000, 900, 20000], 8, 2, 128, 16, BF16, seed=q)
+    want = p.check(ctx).clone()
+    dit.run(ctx)
+    ctx.sync()
+    want_dit = dit.o.clone()
+    for _ in range(15):
+        p.o.fill_(7)
+        dit.o.fill_(7)
+        for _ in range(3):
+            L.attention_paged(ctx, p.q, p.kc, p.vc, p.o, p.cu, p.kv, p.table, scale=p.d ** -0.5, max_q_len=q)
+            dit.run(ctx)
+        L.attention_paged(ctx, p.q, p.kc, p.vc, p.o, p.cu, p.kv, p.table, scale=p.d ** -0.5, max_q_len=q)
+        ctx.sync()
+        assert torch.equal(p.o, want) and torch.equal(dit.o, want_dit)
